@@ -140,6 +140,9 @@ mi355_status mi355_tensor_memset(mi355_context* ctx, const mi355_tensor* t, uint
  * b2 % a2 == 0, b3 % a3 == 0 (src0 broadcast by the ratio).
  * src0: F16, Q8_0, Q4_0 or Q4_1, rows contiguous (nb[0] = type size).
  * src1: F32 (any strides) or, with F16 src0, F16.  dst: F32, nb[0] = 4.
+ * src1 may also hold the rows already quantized (mi355_rms_norm,
+ * mi355_quantize_rows): Q8_0 with Q8_0 / Q4_0 weights, Q8_1 with Q4_1 ones, in
+ * 2-D products; the same bits as with the F32 rows they were made of.
  * Q8_0/Q4_0 quantize src1 to Q8_0 and Q4_1 to Q8_1 (x86 variant) exactly as
  * ggml-cpu's from_float, then combine exact int32 block dots in fp32.  F16
  * converts src1 to F16 (round to nearest even) and accumulates in fp32. */
@@ -238,6 +241,135 @@ int mi355_supports_flash_attn_ext(const mi355_tensor* q, const mi355_tensor* k, 
 mi355_status mi355_flash_attn_ext(mi355_context* ctx, const mi355_tensor* q, const mi355_tensor* k,
                                   const mi355_tensor* v, const mi355_tensor* mask, float scale, float max_bias,
                                   float logit_softcap, const mi355_tensor* dst);
+
+/* ---- Transformer layers around the quantized products ------------------------
+ * The nodes between the MUL_MATs of a layer that keeps its tokens in a cache: a
+ * decoder, or the memory a video model attends to.  The reference runs such
+ * layers on ggml's general backends (its text encoder, sam3.cpp:3928-4069, and
+ * the tracker's memory attention, sam3.cpp:9062-9660); these entry points have
+ * ggml's tensor layouts, with device pointers for the int32 operands. */
+
+/* ggml_add, ggml_rms_norm, ggml_mul and the next MUL_MAT's from_float in one
+ * pass over the rows: h = x + add (add NULL: h = x), sum = h (sum NULL: not
+ * kept), dst = h / sqrt(mean(h^2) + eps) * w (w device F32 [ne0], NULL: no
+ * weight).  x, add and sum: F32 or F16, the same type and ne; dst: F32, F16,
+ * Q8_0 or Q8_1 (the x86 from_float, as MUL_MAT quantizes src1), the same ne.
+ * Rows of ne0 <= 32768 contiguous elements, any row strides; ne0 % 32 == 0 for
+ * Q8_0 and Q8_1.  h and every later step are fp32 as ggml's nodes are (the sum
+ * of squares in double); sum and F16 outputs round once, and the norm is
+ * h's before that rounding.  sum may be x or add, and dst x, add or sum, as
+ * the same tensor; any other overlap is not allowed. */
+int mi355_supports_rms_norm(const mi355_tensor* x, const mi355_tensor* add, const mi355_tensor* sum,
+                            const mi355_tensor* dst);
+mi355_status mi355_rms_norm(mi355_context* ctx, const mi355_tensor* x, const mi355_tensor* add, const float* w,
+                            float eps, const mi355_tensor* sum, const mi355_tensor* dst);
+
+/* ggml's to_float, the counterpart of mi355_quantize_rows: contiguous ggml rows
+ * src of type (Q8_0, Q8_1, Q4_0 or Q4_1) -> every row of the F32 or F16 tensor
+ * dst (nb[0] contiguous, any row strides).  F16 rounds the F32 value once. */
+mi355_status mi355_dequantize_rows(mi355_context* ctx, int type, const void* src, const mi355_tensor* dst);
+
+/* Rotary positions over one to four axes (ggml_rope_multi; sam3_apply_rope's
+ * axial rotation is two axes with restart).  src, dst [ne0, n_head, n_tokens,
+ * batch], F32 or F16, the same type and ne, rows contiguous, any other strides;
+ * dst may be src.  The first n_dims elements of a head turn in pairs, the others
+ * are copied.  pos: device int32 [axes][batch][n_tokens], axes being the axes up
+ * to the last with pairs.  Pair i turns by
+ *   pos[axis(i)] * freq_scale * freq_base ^ (-e / size),
+ * restart 0: e = i, size = n_dims / 2 (the axes share the frequencies out);
+ * restart 1: e = i's place among its axis's pairs, size = sections[axis].
+ * sections: pairs of each axis, n_dims / 2 in all; MI355_ROPE_CONSECUTIVE: the
+ * first sections[0] pairs have axis 0, and so on; MI355_ROPE_INTERLEAVED (three
+ * axes): pair i has axis i % 3 = a for a = 1, 2 while i < 3 sections[a], and axis 0
+ * otherwise.  Angles are taken modulo a turn in 64-bit fixed point, so far
+ * positions lose nothing.  inverse 1 turns back (the gradient). */
+typedef enum { MI355_ROPE_ADJACENT = 0, MI355_ROPE_HALVES = 1 } mi355_rope_pairs; /* (2i, 2i+1); (i, i + n_dims/2) */
+typedef enum { MI355_ROPE_CONSECUTIVE = 0, MI355_ROPE_INTERLEAVED = 1 } mi355_rope_order;
+typedef struct mi355_rope_params {
+    int32_t n_dims; /* even, 2 .. 256, at most ne0 */
+    int32_t pairs;  /* mi355_rope_pairs */
+    int32_t order;  /* mi355_rope_order */
+    int32_t restart;
+    int32_t inverse;
+    int32_t sections[4];
+    float freq_base; /* > 0 */
+    float freq_scale;
+} mi355_rope_params;
+int mi355_supports_rope_multi(const mi355_tensor* src, const mi355_rope_params* p, const mi355_tensor* dst);
+mi355_status mi355_rope_multi(mi355_context* ctx, const mi355_tensor* src, const int32_t* pos,
+                              const mi355_rope_params* p, const mi355_tensor* dst);
+
+/* A cache of keys and values in 8 bits, in blocks of block_tokens tokens that
+ * sequences hold through a table.  Block b, head h is block_tokens rows of
+ * head_dim bytes at k + ((b * n_head_kv + h) * block_tokens) * head_dim (v alike),
+ * with one F32 scale at k_scale[b * n_head_kv + h]: byte u stands for
+ * (u - 128) * scale.  All device memory of the caller's, of any initial content;
+ * k and v 16-byte aligned. */
+typedef struct mi355_kv_cache {
+    uint8_t* k;
+    uint8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t n_blocks;
+    int32_t n_head_kv;
+    int32_t block_tokens; /* 16, 32, 64 or 128 */
+    int32_t head_dim;     /* 64, 96 or 128 */
+} mi355_kv_cache;
+/* n_seq sequences in it: token t of sequence s is row t % block_tokens of block
+ * table[s * max_blocks + t / block_tokens]; n_kv[s] is its length, the tokens of
+ * the call included (taken as 0 below 0, and as max_blocks * block_tokens above
+ * that).  Device int32.  A block id outside 0 .. n_blocks - 1 is never followed:
+ * its tokens are not written, not read and not attended to. */
+typedef struct mi355_kv_seqs {
+    const int32_t* table;
+    const int32_t* n_kv;
+    int32_t n_seq;
+    int32_t max_blocks;
+} mi355_kv_seqs;
+
+/* Writes the last n_new[s] tokens of every sequence s (device int32; NULL: all
+ * n_tokens): row i of k and v [head_dim, n_tokens, n_head_kv, n_seq] (F32 or
+ * F16, the same type, rows contiguous, any other strides) becomes token
+ * n_kv[s] - n_new[s] + i; rows from n_new[s] on are not read.  Per block and
+ * head, with top the largest magnitude among its new elements:
+ *   scale = top / 127, or max(scale, top / 127) where the block keeps tokens
+ *           before the first new one;
+ *   byte  = 128 + x / scale rounded to nearest, ties to even, within 1 .. 255
+ *           (scale 0: 128); kept tokens whose scale grew are rounded anew from
+ *           the values they stood for.
+ * A NaN or infinity makes its block's scale NaN or infinite and the block's
+ * values with it, until it is written from its first row again.  A block may be
+ * written through one sequence only in one call. */
+mi355_status mi355_kv_cache_write(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
+                                  const mi355_tensor* k, const mi355_tensor* v, const int32_t* n_new);
+/* Reads tokens back as (byte - 128) * scale in fp32, F16 rounded once: row i of
+ * k and v [head_dim, n_tokens, n_head_kv, n_seq] (F32 or F16, as above; either may
+ * be NULL) takes token pos[s * n_tokens + i] of sequence s (device int32; NULL:
+ * token i).  Rows whose token is outside 0 .. n_kv[s] - 1 are left as they are. */
+mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
+                                 const int32_t* pos, const mi355_tensor* k, const mi355_tensor* v);
+/* FLASH_ATTN_EXT over the cache.  q [head_dim, n_q, n_head, n_seq] and dst
+ * [head_dim, n_head, n_q, n_seq], each F32 or F16, rows contiguous, any other
+ * strides; n_head a multiple of n_head_kv (query head h reads head
+ * h / (n_head / n_head_kv)).  Sequence s has n_q[s] queries (device int32; NULL: all
+ * n_q); rows of dst from n_q[s] on are left as they are.  Query i stands at position
+ * p = n_kv[s] - n_q[s] + i and attends to tokens t < n_kv[s], with causal t <= p,
+ * and with window > 0 t > p - window; a query that attends to nothing gives zeros.
+ * Scores, softmax and outputs accumulate in fp32.  An F16 q enters the matrix
+ * products as it is and an F32 q as two halves (22 bits); the probabilities enter
+ * as F16 for an F16 dst and as two halves for an F32 dst; the cache's bytes
+ * are exact in F16.
+ * mi355_kv_cache_attn_workspace_size: bytes of the context's workspace that these
+ * sizes need (0: none); a call grows it on demand, except under stream capture,
+ * where it has to be there (mi355_reserve_workspace).  Graphs captured from one context
+ * share its workspace: replay them one after another. */
+int mi355_supports_kv_cache_attn(const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
+                                 const mi355_tensor* dst);
+size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache* cache,
+                                          const mi355_kv_seqs* seqs, const mi355_tensor* q);
+mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
+                                 const mi355_tensor* q, const int32_t* n_q, float scale, int causal, int32_t window,
+                                 const mi355_tensor* dst);
 
 /* ---- SAM3 ViT image encoder ----------------------------------------------
  * The graph sam3_build_vit_graph builds (sam3.cpp:3836-3853) run on this

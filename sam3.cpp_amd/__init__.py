@@ -27,6 +27,8 @@ F32, F16, Q4_0, Q4_1, Q8_0, Q8_1 = 0, 1, 2, 3, 8, 9
 ACT_X86, ACT_REF = 0, 1
 MMQ_F16, MMQ_INT8, MMQ_AUTO = 0, 1, 2
 LAYOUT_GGML, LAYOUT_INT8 = 0, 1
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+ROPE_CONSECUTIVE, ROPE_INTERLEAVED = 0, 1
 TYPE_SIZE = {F32: 4, F16: 2, Q4_0: 18, Q4_1: 20, Q8_0: 34, Q8_1: 36}
 BLCK = {F32: 1, F16: 1, Q4_0: 32, Q4_1: 32, Q8_0: 32, Q8_1: 32}
 
@@ -73,6 +75,23 @@ class HieraBlock(C.Structure):
                 ("norm1_w", C.c_void_p), ("norm1_b", C.c_void_p), ("qkv_b", C.c_void_p), ("proj_b", C.c_void_p),
                 ("norm2_w", C.c_void_p), ("norm2_b", C.c_void_p), ("fc1_b", C.c_void_p), ("fc2_b", C.c_void_p),
                 ("dim_proj_b", C.c_void_p)]
+
+
+class RopeParams(C.Structure):
+    """struct mi355_rope_params."""
+    _fields_ = [("n_dims", C.c_int32), ("pairs", C.c_int32), ("order", C.c_int32), ("restart", C.c_int32),
+                ("inverse", C.c_int32), ("sections", C.c_int32 * 4), ("freq_base", C.c_float), ("freq_scale", C.c_float)]
+
+
+class KvCache(C.Structure):
+    """struct mi355_kv_cache (device pointers)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_blocks", C.c_int32), ("n_head_kv", C.c_int32), ("block_tokens", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class KvSeqs(C.Structure):
+    """struct mi355_kv_seqs (device pointers)."""
+    _fields_ = [("table", C.c_void_p), ("n_kv", C.c_void_p), ("n_seq", C.c_int32), ("max_blocks", C.c_int32)]
 
 
 class HieraBlockInfo(C.Structure):
@@ -153,6 +172,16 @@ def lib():
         "mi355_mul_mat_block_dots": (I, [P, T, T, P]),
         "mi355_soft_max_ext": (I, [P, T, T, F, F, T]),
         "mi355_flash_attn_ext": (I, [P, T, T, T, T, F, F, F, T]),
+        "mi355_supports_rms_norm": (I, [T, T, T, T]),
+        "mi355_rms_norm": (I, [P, T, T, P, F, T, T]),
+        "mi355_dequantize_rows": (I, [P, I, P, T]),
+        "mi355_supports_rope_multi": (I, [T, C.POINTER(RopeParams), T]),
+        "mi355_rope_multi": (I, [P, T, P, C.POINTER(RopeParams), T]),
+        "mi355_kv_cache_write": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, T, P]),
+        "mi355_kv_cache_read": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), P, T, T]),
+        "mi355_supports_kv_cache_attn": (I, [C.POINTER(KvCache), C.POINTER(KvSeqs), T, T]),
+        "mi355_kv_cache_attn_workspace_size": (SZ, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T]),
+        "mi355_kv_cache_attn": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, P, F, I, C.c_int32, T]),
         "mi355_vit_workspace_size": (SZ, [C.POINTER(VitHparams)]),
         "mi355_vit_prefix": (I, [P, C.POINTER(VitHparams), P, T, P, P, P, P]),
         "mi355_vit_block_forward": (I, [P, C.POINTER(VitHparams), C.POINTER(VitBlock), P]),
@@ -316,6 +345,39 @@ def from_torch(x, t: int, ne, nb=None) -> Tensor:
     return T
 
 
+def rope_params(n_dims: int, sections, freq_base: float = 10000.0, pairs: int = ROPE_ADJACENT, order: int = ROPE_CONSECUTIVE,
+                restart: bool = False, inverse: bool = False, freq_scale: float = 1.0) -> RopeParams:
+    """mi355_rope_params; sections: pairs of each axis, up to four, n_dims / 2 in all."""
+    p = RopeParams(n_dims=n_dims, pairs=pairs, order=order, restart=int(restart), inverse=int(inverse), freq_base=freq_base,
+                   freq_scale=freq_scale)
+    for i, s in enumerate(sections):
+        p.sections[i] = s
+    return p
+
+
+def kv_cache(k, v, k_scale, v_scale) -> KvCache:
+    """mi355_kv_cache over torch tensors: k, v uint8 [n_blocks, n_head_kv, block_tokens, head_dim], scales float32
+    [n_blocks, n_head_kv], all contiguous."""
+    n, h, bt, d = k.shape
+    if v.shape != k.shape or any(tuple(x.shape) != (n, h) for x in (k_scale, v_scale)) or not all(
+            x.is_contiguous() for x in (k, v, k_scale, v_scale)):
+        raise ValueError("kv_cache: k, v [n_blocks, n_head_kv, block_tokens, head_dim], scales [n_blocks, n_head_kv], contiguous")
+    if any(x.element_size() != 1 for x in (k, v)) or any(str(x.dtype) != "torch.float32" for x in (k_scale, v_scale)):
+        raise ValueError("kv_cache: k, v hold bytes and the scales float32")
+    c = KvCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, h, bt, d)
+    c._keep = (k, v, k_scale, v_scale)
+    return c
+
+
+def kv_seqs(table, n_kv) -> KvSeqs:
+    """mi355_kv_seqs over torch int32 tensors: table [n_seq, max_blocks], n_kv [n_seq]."""
+    if any(str(x.dtype) != "torch.int32" or not x.is_contiguous() for x in (table, n_kv)) or tuple(n_kv.shape) != (table.shape[0],):
+        raise ValueError("kv_seqs: table [n_seq, max_blocks] and n_kv [n_seq], int32 and contiguous")
+    s = KvSeqs(table.data_ptr(), n_kv.data_ptr(), table.shape[0], table.shape[1])
+    s._keep = (table, n_kv)
+    return s
+
+
 class Context:
     """mi355_context on a device and stream (default: torch's current stream)."""
 
@@ -403,6 +465,33 @@ class Context:
 
     def soft_max_ext(self, src: Tensor, dst: Tensor, scale: float):
         self._check(self.L.mi355_soft_max_ext(self.h, C.byref(src), None, scale, 0.0, C.byref(dst)))
+
+    # ---- transformer layers around the products (w, pos, n_new, n_q: device addresses, 0 for none)
+    def rms_norm(self, x: Tensor, dst: Tensor, eps: float, add: Tensor | None = None, w: int = 0, sum: Tensor | None = None):
+        """dst = rms_norm(x + add) * w, dst F32, F16, Q8_0 or Q8_1; sum receives x + add."""
+        self._check(self.L.mi355_rms_norm(self.h, x, add, w or None, eps, sum, dst))
+
+    def dequantize_rows(self, t: int, src_ptr: int, dst: Tensor):
+        self._check(self.L.mi355_dequantize_rows(self.h, t, src_ptr, dst))
+
+    def rope_multi(self, src: Tensor, pos: int, params: RopeParams, dst: Tensor):
+        self._check(self.L.mi355_rope_multi(self.h, src, pos, params, dst))
+
+    def kv_cache_write(self, cache: KvCache, seqs: KvSeqs, k: Tensor, v: Tensor, n_new: int = 0):
+        self._check(self.L.mi355_kv_cache_write(self.h, cache, seqs, k, v, n_new or None))
+
+    def kv_cache_read(self, cache: KvCache, seqs: KvSeqs, k: Tensor | None, v: Tensor | None, pos: int = 0):
+        self._check(self.L.mi355_kv_cache_read(self.h, cache, seqs, pos or None, k, v))
+
+    def kv_cache_attn(self, cache: KvCache, seqs: KvSeqs, q: Tensor, dst: Tensor, scale: float, n_q: int = 0, causal: bool = True,
+                      window: int = 0):
+        self._check(self.L.mi355_kv_cache_attn(self.h, cache, seqs, q, n_q or None, scale, 1 if causal else 0, window, dst))
+
+    def kv_cache_attn_workspace_size(self, cache: KvCache, seqs: KvSeqs, q: Tensor) -> int:
+        return int(self.L.mi355_kv_cache_attn_workspace_size(self.h, cache, seqs, q))
+
+    def reserve_workspace(self, size: int):
+        self._check(self.L.mi355_reserve_workspace(self.h, size))
 
     def model_file_load(self, f: "ModelFile", index: int, dst_type: int, dst_ptr: int, dst_bytes: int):
         self._check(self.L.mi355_model_file_load(self.h, f.h, index, dst_type, C.c_void_p(dst_ptr), dst_bytes))

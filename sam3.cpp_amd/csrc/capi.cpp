@@ -88,6 +88,29 @@ mi355_status ensure_buffer(mi355_context* ctx, void** buf, size_t* size, size_t 
     return MI355_STATUS_SUCCESS;
 }
 
+static bool capturing(const mi355_context* ctx) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    return ctx->stream && hipStreamIsCapturing(ctx->stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone;
+}
+
+mi355_status ensure_ws(mi355_context* ctx, size_t bytes) {
+    const bool cap = bytes > 0 && (bytes > ctx->ws_size || !ctx->ws_captured) && capturing(ctx);
+    if (bytes <= ctx->ws_size) {
+        ctx->ws_captured = ctx->ws_captured || cap;
+        return MI355_STATUS_SUCCESS;
+    }
+    if (cap)
+        return fail(ctx, MI355_STATUS_ALLOC_FAILED, "a captured call needs %zu bytes of workspace, the context has %zu (mi355_reserve_workspace)",
+                    bytes, ctx->ws_size);
+    if (ctx->ws_captured) {
+        ctx->retired.push_back(ctx->ws);
+        ctx->ws = nullptr;
+        ctx->ws_size = 0;
+        ctx->ws_captured = false;
+    }
+    return ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, bytes);
+}
+
 }  // namespace mi355
 
 namespace {
@@ -130,6 +153,7 @@ struct MmPlan {
 };
 
 // The int8-MFMA kernel takes plain 2-D GEMMs with block-quantized weights.
+bool q8_rows(const mi355_tensor* s1) { return s1->type == T_Q8_0 || s1->type == T_Q8_1; }  // src1 quantized already
 bool mm_i8_eligible(const mi355_tensor* s0, const mi355_tensor* s1) {
     return (s0->type == T_Q8_0 || s0->type == T_Q4_0 || s0->type == T_Q4_1) && s0->ne[2] == 1 && s0->ne[3] == 1 &&
            s1->ne[2] == 1 && s1->ne[3] == 1 && s0->ne[0] % 32 == 0;
@@ -160,7 +184,7 @@ int device_cus(int device) {
 // kernel: the MI355_MMQ_* route when the operands are eligible for it
 MmPlan mm_plan(const mi355_tensor* s0, const mi355_tensor* s1, int cus, bool split = true, int kernel = 0) {
     const bool prep = s0->layout == MI355_LAYOUT_INT8;
-    const bool i8 = prep || kernel != MI355_MMQ_F16;
+    const bool i8 = prep || kernel != MI355_MMQ_F16 || q8_rows(s1);  // (8-bit rows are the int8 operand already)
     MmPlan pl;
     if (s0->type == T_F32) return pl;
     const int64_t K = s1->ne[0], M = s1->ne[1], Z = s1->ne[2] * s1->ne[3];
@@ -249,8 +273,6 @@ mi355_status check_soft_max(mi355_context* ctx, const mi355_tensor* src, const m
     return MI355_STATUS_SUCCESS;
 }
 
-mi355_status ensure_ws(mi355_context* ctx, size_t bytes) { return ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, bytes); }
-
 
 // ggml_mul_mat shape rules (ggml.c ggml_can_mul_mat / ggml_compute_forward_mul_mat)
 // plus what the kernels here implement.
@@ -265,7 +287,8 @@ mi355_status check_mul_mat(mi355_context* ctx, const mi355_tensor* s0, const mi3
     const int t0 = s0->type;
     if (!(t0 == T_F32 || t0 == T_F16 || t0 == T_Q8_0 || t0 == T_Q4_0 || t0 == T_Q4_1))
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: src0 type %d not supported", t0);
-    if (!(s1->type == T_F32 || (s1->type == T_F16 && t0 == T_F16)))
+    const bool q8 = (s1->type == T_Q8_0 && (t0 == T_Q8_0 || t0 == T_Q4_0)) || (s1->type == T_Q8_1 && t0 == T_Q4_1);
+    if (!(s1->type == T_F32 || (s1->type == T_F16 && t0 == T_F16) || q8))
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: src1 type %d with src0 type %d not supported", s1->type, t0);
     if (d->type != T_F32) return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: dst type %d not supported", d->type);
     const int64_t K = s0->ne[0];
@@ -282,6 +305,15 @@ mi355_status check_mul_mat(mi355_context* ctx, const mi355_tensor* s0, const mi3
     if (d->nb[0] != 4) return fail(ctx, MI355_STATUS_INVALID_ARG, "mul_mat: dst nb[0] must be 4");
     if (s1->nb[0] != type_size(s1->type) && s1->type != T_F32)
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: strided F16 src1 elements");
+    if (q8) {
+        if (s1->ne[2] != 1 || s1->ne[3] != 1 || s0->ne[2] != 1 || s0->ne[3] != 1)
+            return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: quantized src1 rows take 2-D operands");
+        if (s1->nb[1] < row_size(s1->type, K) ||
+            ((reinterpret_cast<uintptr_t>(s1->data) | (uintptr_t)s1->nb[1]) & (s1->type == T_Q8_1 ? 3 : 1)))
+            return fail(ctx, MI355_STATUS_INVALID_ARG, "mul_mat: quantized src1 rows must be whole and 2-byte (Q8_1: 4-byte) aligned");
+        if (K < ((int64_t)1 << 30) && s0->ne[1] < ((int64_t)1 << 30) && s1->ne[1] < ((int64_t)1 << 30) && !i8_extents_ok(s0, s1))
+            return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: operands beyond the kernels' 1 GiB buffer extents");
+    }
     const int64_t lim = (int64_t)1 << 30;
     if (K >= lim || s0->ne[1] >= lim || s1->ne[1] >= lim || s1->ne[2] * s1->ne[3] > 65535)
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: dimensions beyond kernel limits");
@@ -342,6 +374,22 @@ ActI8 act_i8(char* ws, const MmPlan& pl, int wtype, int64_t M, int64_t K) {
     return a;
 }
 
+// src1 -> a8: quantized, or the blocks of 8-bit rows taken apart.
+mi355_status fill_act_i8(mi355_context* ctx, mi355_context* tctx, const mi355_tensor* s0, const mi355_tensor* s1, const ActI8& a8,
+                         char* ws, const MmPlan& pl) {
+    if (q8_rows(s1)) {
+        Timed tu(tctx, "unpack_q8");
+        return hip_check(ctx, tu.done(launch_unpack_q8(s1->data, s1->nb[1], s1->type, a8.M, a8.K, ws, const_cast<uint32_t*>(a8.dl),
+                                                       const_cast<uint32_t*>(a8.dh), const_cast<void*>(a8.s), ctx->stream)),
+                         "unpack_q8 launch");
+    }
+    Timed tq8(tctx, "quantize_mmq_i8");
+    return hip_check(ctx, tq8.done(launch_quantize_mmq_i8(view_of(s1), s0->type == T_Q4_1, a8.K, 2 * a8.nst,
+                                                          reinterpret_cast<int8_t*>(ws), reinterpret_cast<uint16_t*>(ws + pl.q),
+                                                          reinterpret_cast<uint16_t*>(const_cast<void*>(a8.s)), ctx->stream)),
+                     "quantize_mmq_i8 launch");
+}
+
 // MUL_MAT of validated operands with the workspace ws (at least
 // mm_plan(...).total() bytes): the activation conversion, then the GEMM.
 // timed = false: no timing events (the no-allocation entry point).
@@ -360,21 +408,13 @@ mi355_status mul_mat_run(mi355_context* ctx, const mi355_tensor* s0, const mi355
                            "repack_weights launch");
             if (st != MI355_STATUS_SUCCESS) return st;
         }
-        if (ctx->skinny && mmq8_few_ok(wr, view_of(s1))) {
+        if (ctx->skinny && !q8_rows(s1) && mmq8_few_ok(wr, view_of(s1))) {
             Timed tf(tctx, "mmq8_few");
             return hip_check(ctx, tf.done(launch_mmq8_few(wr, view_of(s1), matd_of(d), pl.ks, ctx->stream)), "mmq8_few launch");
         }
         const ActI8 a8 = act_i8(ws, pl, s0->type, M, K);
-        {
-            Timed tq8(tctx, "quantize_mmq_i8");
-            st = hip_check(ctx, tq8.done(launch_quantize_mmq_i8(view_of(s1), s0->type == T_Q4_1, K, 2 * a8.nst,
-                                                                reinterpret_cast<int8_t*>(ws),
-                                                                reinterpret_cast<uint16_t*>(ws + pl.q),
-                                                                reinterpret_cast<uint16_t*>(const_cast<void*>(a8.s)),
-                                                                ctx->stream)),
-                           "quantize_mmq_i8 launch");
-            if (st != MI355_STATUS_SUCCESS) return st;
-        }
+        st = fill_act_i8(ctx, tctx, s0, s1, a8, ws, pl);
+        if (st != MI355_STATUS_SUCCESS) return st;
         if (!mmq8_supported(wr, a8)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "mul_mat: operands beyond the int8 kernel");
         MmqSplit sp8{pl.ks, pl.ks > 1 ? reinterpret_cast<float*>(ws + pl.q + pl.d + pl.s + pl.align) : nullptr,
                      ctx->skinny};
@@ -712,6 +752,7 @@ void mi355_context_free(mi355_context* ctx) {
     noalloc_release(ctx);
     mi355_profile_reset(ctx);
     if (ctx->ws) (void)hipFree(ctx->ws);
+    for (void* p : ctx->retired) (void)hipFree(p);
     if (ctx->enc) (void)hipFree(ctx->enc);
     if (ctx->neck) (void)hipFree(ctx->neck);
     delete ctx;
@@ -793,10 +834,10 @@ mi355_status mi355_mul_mat(mi355_context* ctx, const mi355_tensor* s0, const mi3
     if (s0->ne[0] == 0 || s0->ne[1] == 0 || s1->ne[1] == 0 || s1->ne[2] * s1->ne[3] == 0) return MI355_STATUS_SUCCESS;
     if (s0->type == T_F32) return mul_mat_f32(ctx, s0, s1, d, true);
     MmPlan pl = mm_plan(s0, s1, ctx->cus, dst_split_ok(d), mm_route(s0, s1, ctx->mmq_kernel));
-    if (pl.total() > ctx->ws_size) {
-        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(ctx->stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
-            pl = mm_plan_in(ctx, s0, s1, d, ctx->ws_size);  // nothing can be allocated now
+    if (pl.total() <= ctx->ws_size) {
+        (void)ensure_ws(ctx, pl.total());  // large enough: notes a captured use
+    } else {
+        if (capturing(ctx)) pl = mm_plan_in(ctx, s0, s1, d, ctx->ws_size);  // nothing can be allocated now
         const std::string before = ctx->last_error;
         st = ensure_ws(ctx, pl.total());
         if (st != MI355_STATUS_SUCCESS) {  // no memory for the repack: the own route may need less
@@ -865,10 +906,7 @@ mi355_status mi355_mul_mat_block_dots(mi355_context* ctx, const mi355_tensor* s0
             if (st != MI355_STATUS_SUCCESS) return st;
         }
         const ActI8 a8 = act_i8(ws, pl, s0->type, M, K);
-        st = hip_check(ctx, launch_quantize_mmq_i8(view_of(s1), s0->type == T_Q4_1, K, 2 * a8.nst, reinterpret_cast<int8_t*>(ws),
-                                                   reinterpret_cast<uint16_t*>(ws + pl.q),
-                                                   reinterpret_cast<uint16_t*>(const_cast<void*>(a8.s)), ctx->stream),
-                       "quantize_mmq_i8 launch");
+        st = fill_act_i8(ctx, nullptr, s0, s1, a8, ws, pl);
         if (st != MI355_STATUS_SUCCESS) return st;
         return hip_check(ctx, launch_mmq8(wr, a8, MatD{nullptr, 0, 0, 0}, nullptr, MmqSplit{1, nullptr}, ctx->stream,
                                           isums),

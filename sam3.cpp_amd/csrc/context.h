@@ -18,6 +18,8 @@ struct mi355_context {
     hipStream_t stream = nullptr;
     void* ws = nullptr;        // per-call scratch of mul_mat (activation operand, scales)
     size_t ws_size = 0;
+    bool ws_captured = false;  // a captured call uses ws: a larger one replaces it without freeing it
+    std::vector<void*> retired;  // such workspaces, which captured graphs still name
     void* enc = nullptr;       // activation buffers of the image-encoder runner
     size_t enc_size = 0;
     void* neck = nullptr;      // maps and scratch of the SimpleFPN neck
@@ -61,6 +63,11 @@ size_t align_up(size_t x);
 // Grows a device buffer owned by the context to at least bytes (waits for the
 // stream first: earlier kernels may still read the old buffer).
 mi355_status ensure_buffer(mi355_context* ctx, void** buf, size_t* size, size_t bytes);
+
+// The context's workspace of at least bytes, for a call that uses it now: replaced by a larger one, after
+// the stream's work, unless it is large enough.  A workspace that a captured call used is kept until the
+// context is freed; nothing grows under capture.
+mi355_status ensure_ws(mi355_context* ctx, size_t bytes);
 
 // The activation layout a producer pass should write for weights of type t:
 // Q8 quants for Q8_0/Q4_0, Q8 with Q8_1 sums for Q4_1, F16 for F16, F32 otherwise.

@@ -285,6 +285,76 @@ inline int gemm_ksplit(int64_t tiles, int64_t full, int64_t M, int64_t N, int64_
     return bs;
 }
 
+// ---- transformer layers around the products (norm.hip, rope.hip, kvcache.hip, kvattn.hip)
+// Rows of a tensor [ne0][ne1][ne2][ne3]: row r at base + i1 nb[0] + i2 nb[1] + i3 nb[2].
+struct RowSpan {
+    char* base;
+    int64_t nb[3];
+};
+struct RmsArgs {
+    RowSpan x, add, sum, dst;  // add.base, sum.base may be null
+    const float* w;            // [n] or null
+    int64_t rows, ne1, ne2;
+    int n;
+    float eps;
+    bool xf16;                 // x, add and sum; else F32
+    int out;                   // T_F32, T_F16, T_Q8_0, T_Q8_1
+    bool vec;                  // n % 8 == 0 and every row of x, add, sum (and F32 / F16 dst) on 16 bytes
+};
+constexpr int RMS_MAX = 32768;
+hipError_t launch_rms_norm(const RmsArgs& a, hipStream_t st);
+// contiguous ggml rows of type (Q8_0, Q8_1, Q4_0, Q4_1) -> F32 or F16 rows of n
+hipError_t launch_dequantize_rows(const void* src, int type, const RowSpan& dst, bool f16, int64_t n, int64_t rows,
+                                  int64_t ne1, int64_t ne2, hipStream_t st);
+// ggml Q8_0 / Q8_1 rows (row r at src + r * nb1) -> the int8 kernel's operand (ActI8, quants at pitch K)
+hipError_t launch_unpack_q8(const void* src, int64_t nb1, int type, int64_t M, int64_t K, void* q, uint32_t* dl, uint32_t* dh,
+                            void* s, hipStream_t st);
+
+constexpr int ROPE_PAIRS = 128;
+struct RopeArgs {
+    const char* src;
+    char* dst;
+    int64_t s_nb[3], d_nb[3];  // strides of heads, tokens, batches
+    int heads, tokens, batch, ne0, pairs;
+    bool f16, halves, vec;
+    const int32_t* pos;        // [axes][batch][tokens]
+    uint64_t turn[ROPE_PAIRS]; // turns a position, times 2^64
+    uint8_t axis[ROPE_PAIRS];
+};
+hipError_t launch_rope_multi(const RopeArgs& a, hipStream_t st);
+
+struct KvView {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int n_blocks, heads, bt, bt_log2;
+    const int32_t* table;
+    const int32_t* n_kv;
+    int n_seq, max_blocks;
+};
+struct KvRows {                // keys and values [D, n_tok, heads, n_seq]
+    char *k, *v;               // either may be null (reading)
+    int64_t k_nb[3], v_nb[3];
+    int n_tok;
+    bool f16, vec;             // vec: every row on 16 bytes
+    const int32_t* idx;        // write: n_new [n_seq]; read: pos [n_seq][n_tok]; or null
+};
+hipError_t launch_kv_write(const KvView& c, const KvRows& r, int D, hipStream_t st);
+hipError_t launch_kv_read(const KvView& c, const KvRows& r, int D, hipStream_t st);
+
+struct KvAttnArgs {
+    KvView c;
+    const char* q;             // [D, n_q, heads, n_seq]
+    char* dst;                 // [D, heads, n_q, n_seq]
+    int64_t q_nb[3], d_nb[3];  // q: query, head, sequence; dst: head, query, sequence
+    int n_q, heads, group;     // group = heads / c.heads
+    const int32_t* nq;         // [n_seq] or null
+    float scale;
+    int causal, window;
+    bool q16, d16;
+    float* part;
+};
+hipError_t launch_kv_attn(const KvAttnArgs& a, int D, hipStream_t st);
+
 // ---- SAM3 ViT glue (rows of E contiguous floats)
 struct LnArgs {
     const float* x;     // [rows][E], image token order

@@ -258,7 +258,7 @@ mi355_status mi355_model_file_load(mi355_context* ctx, const mi355_model_file* f
     // raw bytes -> pinned staging -> device (dst itself, or the workspace before a conversion)
     const bool same = dst_type == r.type;
     if (!same) {
-        mi355_status st = ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, (size_t)r.nbytes);
+        mi355_status st = ensure_ws(ctx, (size_t)r.nbytes);
         if (st != MI355_STATUS_SUCCESS) return st;
     }
     char* dev = same ? static_cast<char*>(dst) : static_cast<char*>(ctx->ws);
@@ -755,7 +755,7 @@ mi355_status mi355_model_quantize(mi355_context* ctx, const char* in_path, const
             const int64_t chunk_rows = std::max<int64_t>(1, (int64_t)((32u << 20) / in_row));
             const int64_t cr = std::min(rows, chunk_rows);
             const size_t in_dev = (size_t)cr * in_row, dev_off = (in_dev + 255) & ~(size_t)255;
-            mi355_status st = ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, dev_off + (size_t)cr * out_row);
+            mi355_status st = ensure_ws(ctx, dev_off + (size_t)cr * out_row);
             if (st != MI355_STATUS_SUCCESS) return finish(st);
             if (!pinned(hin, hin_cap, in_dev) || !pinned(hout, hout_cap, (size_t)cr * out_row))
                 return finish(fail(ctx, MI355_STATUS_ALLOC_FAILED, "model_quantize: staging allocation failed"));
