@@ -353,7 +353,13 @@ struct KvAttnArgs {
     bool q16, d16;
     float* part;
 };
-hipError_t launch_kv_attn(const KvAttnArgs& a, int D, hipStream_t st);
+struct KvAttnPlan {
+    int nt, tiles;             // 16-row tiles of a workgroup, workgroups over a sequence's rows
+    int splits;                // ranges of the tokens, joined by a second kernel
+    size_t bytes;              // of part
+};
+KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int D, int cus);
+hipError_t launch_kv_attn(const KvAttnArgs& a, const KvAttnPlan& p, int D, hipStream_t st);
 
 // ---- SAM3 ViT glue (rows of E contiguous floats)
 struct LnArgs {

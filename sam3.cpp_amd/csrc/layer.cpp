@@ -192,6 +192,11 @@ mi355_status check_attn(mi355_context* ctx, const mi355_kv_cache* c, const mi355
     return MI355_STATUS_SUCCESS;
 }
 
+KvAttnPlan attn_plan(const mi355_context* ctx, const mi355_kv_cache* c, const mi355_kv_seqs* s, const mi355_tensor* q) {
+    return kv_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, c->head_dim,
+                        ctx->cus);
+}
+
 }  // namespace
 
 extern "C" {
@@ -300,8 +305,10 @@ int mi355_supports_kv_cache_attn(const mi355_kv_cache* cache, const mi355_kv_seq
     return check_attn(nullptr, cache, seqs, q, dst) == MI355_STATUS_SUCCESS;
 }
 
-size_t mi355_kv_cache_attn_workspace_size(const mi355_context*, const mi355_kv_cache*, const mi355_kv_seqs*, const mi355_tensor*) {
-    return 0;
+size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
+                                          const mi355_tensor* q) {
+    if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
+    return attn_plan(ctx, cache, seqs, q).bytes;
 }
 
 mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
@@ -322,11 +329,17 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     a.n_q = (int)q->ne[1]; a.heads = (int)q->ne[2];
     a.group = a.heads / cache->n_head_kv;
     a.nq = n_q;
-    a.scale = scale; a.causal = causal; a.window = window;
+    a.scale = scale; a.causal = causal;
+    a.window = window < 1 << 30 ? window : 1 << 30;
     a.q16 = q->type == T_F16; a.d16 = dst->type == T_F16;
-    a.part = nullptr;
+    if (cache->n_blocks == 0) a.c.max_blocks = 0;  // nothing to attend to
+    if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
+    const KvAttnPlan p = attn_plan(ctx, cache, seqs, q);
+    const mi355_status ws = ensure_ws(ctx, p.bytes);
+    if (ws != MI355_STATUS_SUCCESS) return ws;
+    a.part = static_cast<float*>(ctx->ws);
     Timed tm(ctx, "kv_cache_attn");
-    return hip_check(ctx, tm.done(launch_kv_attn(a, cache->head_dim, ctx->stream)), "kv_cache_attn launch");
+    return hip_check(ctx, tm.done(launch_kv_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache_attn launch");
 }
 
 }  // extern "C"
