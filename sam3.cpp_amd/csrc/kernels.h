@@ -354,7 +354,7 @@ struct KvAttnArgs {
     float* part;
 };
 struct KvAttnPlan {
-    int nt, tiles;             // 16-row tiles of a workgroup, workgroups over a sequence's rows
+    int nt, tiles;             // 16-row tiles of a workgroup (0: the kernel of 128 rows), workgroups over a sequence's rows
     int splits;                // ranges of the tokens, joined by a second kernel
     size_t bytes;              // of part
 };

@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "attn.cuh"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -24,6 +25,7 @@ constexpr float KV_LOG2E = 1.44269504088896340736f;
 constexpr float KV_NONE = -1e30f;    // a reference that nothing has been taken against yet
 constexpr float KV_LIFT = 12.0f;     // probabilities are raised by 2^12 to keep small ones in fp16's normal range
 constexpr float KV_ROOM = 15.0f;     // and their reference moves when one would pass 2^15
+constexpr float KV_LIFT_SUM = 8.0f;  // the same where a lane's sum of 32 of them, and not each, is held below 2^15
 constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
 constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
 }  // namespace
@@ -48,6 +50,32 @@ __device__ __forceinline__ int kv_chunk(const KvRange& r, int splits) {
     return (per + KV_SPAN - 1) / KV_SPAN * KV_SPAN;
 }
 
+// log2 of a block's scale, -inf for 0; the instruction takes no subnormals
+__device__ __forceinline__ float scale_log2(float v) {
+    const bool tiny = v < 7.8886091e-31f;  // 2^-100
+    return __builtin_amdgcn_logf(tiny ? v * 1.1529215e18f : v) - (tiny ? 60.0f : 0.0f);
+}
+
+// What the products need of 16 tokens, which lie in one block: lane i of a wavefront keeps it for the i-th
+// group from a token on, and readlane gives it to the scalar unit when its step comes.  (A load for each
+// step instead is a chain of two latencies in every step.)
+struct KvGroups {
+    int id;           // block, or -1
+    float f, lv, rv;  // key scale times the score's scale; log2 of the value scale; 1 / value scale
+};
+__device__ __forceinline__ int group_block(const KvAttnArgs& a, const int* table, int t) {
+    const int id = table[min(max(t, 0) >> a.c.bt_log2, a.c.max_blocks - 1)];
+    return id >= 0 && id < a.c.n_blocks ? id : -1;
+}
+__device__ __forceinline__ void group_scales(const KvAttnArgs& a, int hk, float sc, KvGroups& x) {
+    const int64_t at = (int64_t)max(x.id, 0) * a.c.heads + hk;
+    const float ks = a.c.k_scale[at], vs = a.c.v_scale[at];
+    x.f = x.id >= 0 ? ks * sc : 0.0f;
+    x.lv = x.id >= 0 ? scale_log2(vs) : 0.0f;
+    x.rv = 1.0f / vs;
+}
+__device__ __forceinline__ float read_lane(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
+
 // four bytes of keys as the halves u - 128 (exact): 0x64uu is the half 1024 + u
 __device__ __forceinline__ void key_halves(uint32_t v, uint32_t* o) {
     const h2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
@@ -61,10 +89,13 @@ __device__ __forceinline__ uint32_t value_halves(uint32_t t0, uint32_t t1, int b
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, mul, off));
 }
 
-// log2 of a block's scale, -inf for 0; the instruction takes no subnormals
-__device__ __forceinline__ float scale_log2(float v) {
-    const bool tiny = v < 7.8886091e-31f;  // 2^-100
-    return __builtin_amdgcn_logf(tiny ? v * 1.1529215e18f : v) - (tiny ? 60.0f : 0.0f);
+// 2^-e and 2^e of a magnitude's exponent e, both normal
+struct Pow2 {
+    float down, up;
+};
+__device__ __forceinline__ Pow2 pow2_of(float top) {
+    const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -126), 126);
+    return {__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23)};
 }
 
 // max and sum over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48)
@@ -146,12 +177,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[m][j]));
             }
-            top = col_max(top);
-            // 2^-e of top's exponent e, and 2^e for the scores
-            const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            const int ec = min(max(e, -126), 126);
-            const float down = __uint_as_float((uint32_t)(127 - ec) << 23);
-            qscale[t] = __uint_as_float((uint32_t)(127 + ec) << 23);
+            const Pow2 z = pow2_of(col_max(top));
+            const float down = z.down;
+            qscale[t] = z.up;
 #pragma unroll
             for (int m = 0; m < KM; ++m)
 #pragma unroll
@@ -182,22 +210,26 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
     const int* table = c.table + (int64_t)s * c.max_blocks;
     const float sc = a.scale * KV_LOG2E;
 
-    for (int t0 = tb + w * KV_STEP; t0 < te; t0 += KV_SPAN) {
-        // the step's two halves of 16 tokens lie in one block each
+    KvGroups gr = {-1, 0.0f, 0.0f, 0.0f};
+    int at = 32;
+    for (int t0 = tb + w * KV_STEP; t0 < te; t0 += KV_SPAN, ++at) {
+        if (at == 32) {  // lane 2 i + u: half u of this wavefront's i-th step from here
+            gr.id = group_block(a, table, t0 + (lane >> 1) * KV_SPAN + 16 * (lane & 1));
+            group_scales(a, hk, sc, gr);
+            at = 0;
+        }
         const uint8_t *kp[2], *vp[2];
         float ks[2], lv[2];
         bool there[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const int tt = t0 + 16 * u, blk = min(tt >> c.bt_log2, c.max_blocks - 1);
-            const int id = table[blk];
-            there[u] = id >= 0 && id < c.n_blocks;
-            const int64_t at = (int64_t)(there[u] ? id : 0) * c.heads + hk;
-            const int64_t off = (at * c.bt + (tt & (c.bt - 1))) * D;
+            const int id = __builtin_amdgcn_readlane(gr.id, 2 * at + u);
+            there[u] = id >= 0;
+            const int64_t off = (((int64_t)max(id, 0) * c.heads + hk) * c.bt + ((t0 + 16 * u) & (c.bt - 1))) * D;
             kp[u] = c.k + off;
             vp[u] = c.v + off;
-            ks[u] = there[u] ? c.k_scale[at] * sc : 0.0f;
-            lv[u] = there[u] ? scale_log2(c.v_scale[at]) : 0.0f;
+            ks[u] = read_lane(gr.f, 2 * at + u);
+            lv[u] = read_lane(gr.lv, 2 * at + u);
         }
         u32x4 kv[2][KC];
         u32x2 kt[2];
@@ -356,6 +388,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
     if (w != 0) return;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+        p_ref[t] += 9.0f;  // the halves were the bytes' values over 512
         const int r = row0 + 16 * t + col, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
         if (r >= rows) continue;
         float f = 1.0f;
@@ -368,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
                 *reinterpret_cast<v4f*>(ml) = v4f{m_ref[t], p_ref[t], l_sum[t], 0.0f};
             }
         } else {
-            f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t] + 9.0f) / l_sum[t];
+            f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t]) / l_sum[t];
             out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
         }
         const bool h16 = splits == 1 && a.d16;
@@ -390,6 +423,337 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
             }
         }
     }
+}
+
+// Many query rows: a workgroup takes 128 rows (as above: queries times the heads of a key head's group) in four
+// wavefronts of 32, and streams the tokens through LDS in tiles of 64, bytes becoming halves once for
+// all four on the way: thread t loads 16 bytes (D = 96: 8) of a row ahead of time and writes 32 after
+// the previous tile's products.  Scores and output as fattn.hip's (v_mfma_f32_32x32x16_f16, S^T = K Q^T, the
+// probabilities' registers as the operand of O^T += V^T P^T, V^T by transposing reads); the tile's scores
+// are computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.  A lane's
+// eight scores (kh, hh) belong to 16 tokens of one block: scales and validity are uniform over them.
+template <int D, bool QS, bool PS>
+__global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles, const int spread) {
+    constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
+    constexpr int UB = D == 96 ? 8 : 16;            // bytes of a staging unit
+    constexpr int UR = D / UB, NU = 16 * UR / 64;   // units of a row, units of a thread
+    __shared__ __attribute__((aligned(16))) _Float16 sK[2][64 * D];
+    __shared__ __attribute__((aligned(16))) _Float16 sV[2][64 * D];
+    const KvView& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // spread: items go to the XCDs in turn with all their row tiles; else row tiles do
+    int item, tile;
+    if (spread) {
+        const int per = 8 * tiles, rb = blockIdx.x % per;
+        item = (int)(blockIdx.x / per) * 8 + (rb & 7);
+        tile = rb >> 3;
+    } else {
+        item = blockIdx.x / tiles;
+        tile = blockIdx.x % tiles;
+    }
+    if (item >= splits * c.heads * c.n_seq) return;
+    tile = tiles - 1 - tile;  // causal: the longest rows first
+    const int sp = item % splits, hk = item / splits % c.heads, s = item / splits / c.heads;
+    const KvRange kr = kv_range(a, s);
+    const int rows = kr.nq * a.group, row0 = tile * 128;
+    if (row0 >= rows) return;
+    const int chunk = kv_chunk(kr, splits);
+    if (sp > 0 && kr.lo + sp * chunk >= kr.hi) return;
+    const int iq_first = row0 / a.group, iq_last = (min(row0 + 128, rows) - 1) / a.group;
+    const int lo_tile = a.window > 0 ? max(kr.pos0 + iq_first - a.window + 1, 0) & ~63 : 0;
+    const int tb = max(kr.lo + sp * chunk, lo_tile);  // (a multiple of 32: blocks are met at 16-token steps)
+    const int te = min(min(kr.lo + sp * chunk + chunk, kr.hi), a.causal ? kr.pos0 + iq_last + 1 : kr.hi);
+
+    // this lane's query row
+    const int r = row0 + 32 * w + lr, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
+    const bool on = r < rows;
+    const int pos = kr.pos0 + iq;
+    const int see_hi = on ? (a.causal ? min(pos + 1, te) : te) : 0, see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    // tokens that every row of the wavefront sees (rows past the last one see what they like)
+    const int iq0 = __builtin_amdgcn_readfirstlane(iq), iq31 = min(__builtin_amdgcn_readlane(iq, 31), iq_last);
+    const int all_hi = a.causal ? min(kr.pos0 + iq0 + 1, te) : te, all_lo = a.window > 0 ? kr.pos0 + iq31 - a.window + 1 : 0;
+    v8h q[NC], ql[QS ? NC : 1];
+    float qscale = a.scale < 0.0f ? -1.0f : 1.0f;
+    {
+        const char* p = a.q + (int64_t)iq * a.q_nb[0] + (int64_t)h * a.q_nb[1] + (int64_t)s * a.q_nb[2];
+        if constexpr (QS) {
+            float top = 0.0f;
+#pragma unroll
+            for (int m = 0; m < NC; ++m)
+                if (on) {
+                    const v4f x0 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g)), x1 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g) + 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(x0[j]), fabsf(x1[j])));
+                }
+            const Pow2 z = pow2_of(xmax32(top));
+            const float down = z.down * qscale;
+            qscale = z.up;
+#pragma unroll
+            for (int m = 0; m < NC; ++m) {
+                v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+                if (on) {
+                    x0 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g)) * down;
+                    x1 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g) + 16) * down;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = j < 4 ? x0[j & 3] : x1[j & 3];
+                    q[m][j] = (_Float16)y;
+                    ql[m][j] = (_Float16)(y - (float)q[m][j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < NC; ++m) {
+                const v8h z = {0, 0, 0, 0, 0, 0, 0, 0};
+                q[m] = on ? *reinterpret_cast<const v8h_a2*>(p + 2 * (16 * m + 8 * g)) : z;
+                if (a.scale < 0.0f) q[m] = -q[m];
+            }
+            qscale = 1.0f;
+        }
+    }
+    const float sc = fabsf(a.scale) * KV_LOG2E;
+
+    const int* table = c.table + (int64_t)s * c.max_blocks;
+    int tile0 = 0;  // the step's tile
+    // groups of the sixteen tiles that the step's tile is of, and of the sixteen after
+    KvGroups cur, nxt;
+    auto group_of = [&](int tile) { return tb + 64 * tile + 16 * lane; };
+    auto staged = [&](int tile) {  // block of this wavefront's 16 rows of a tile of this or the next sixteen
+        const int i = 4 * (tile & 15) + w;
+        return max((tile >> 4) == (tile0 >> 4) ? __builtin_amdgcn_readlane(cur.id, i) : __builtin_amdgcn_readlane(nxt.id, i), 0);
+    };
+    // staging: wavefront w takes rows 16 w .. + 15 of a tile, unit j of a lane bytes UB (u % UR) of row u / UR, u = lane + 64 j
+    typedef uint32_t unit_t __attribute__((ext_vector_type(UB / 4)));
+    unit_t kreg[NU], vreg[NU];
+    auto load_one = [&](const uint8_t* base, unit_t* reg, int tile) {
+        const uint8_t* p = base + (((int64_t)staged(tile) * c.heads + hk) * c.bt + ((tb + 64 * tile + 16 * w) & (c.bt - 1))) * D;
+#pragma unroll
+        for (int j = 0; j < NU; ++j) reg[j] = *reinterpret_cast<const unit_t*>(p + UB * (lane + 64 * j));
+    };
+    auto store_one = [&](_Float16* lds, const unit_t* reg, bool key) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            const int u = ln + 64 * j, row = 16 * w + u / UR;
+#pragma unroll
+            for (int e = 0; e < UB / 8; ++e) {
+                uint32_t f[4];
+                key_halves(reg[j][2 * e], f);
+                key_halves(reg[j][2 * e + 1], f + 2);
+                const int chunk8 = (UB / 8) * (u % UR) + e, slot = chunk8 ^ (key ? kswz<D>(row) : vswz<D>(row));
+                *reinterpret_cast<u32x4*>(&lds[row * D + 8 * slot]) = u32x4{f[0], f[1], f[2], f[3]};
+            }
+        }
+    };
+    v16f O[NDB];
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) O[i][e] = 0.0f;
+    float m_ref = KV_NONE, p_ref = KV_NONE, l_sum = 0.0f, back = 1.0f;  // back = 2^(p_ref - m_ref)
+    // (the LDS addresses follow from one register by a few instructions; kept, they would push the queries out)
+    auto score = [&](const _Float16* lds, v16f* S) {
+        int lrow = lr;
+        asm volatile("" : "+v"(lrow));
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        S[0] = S[1] = z;
+#pragma unroll
+        for (int m = 0; m < NC; ++m)
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                const int row = 32 * kh + lrow;
+                const v8h k8 = *reinterpret_cast<const v8h*>(&lds[row * D + 8 * ((2 * m + g) ^ kswz<D>(row))]);
+                S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q[m], S[kh], 0, 0, 0);
+                if constexpr (QS) S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[m], S[kh], 0, 0, 0);
+            }
+    };
+    uint64_t hide_groups = 0, nan_groups = 0, far_groups = 0;  // (sort_groups)
+    // The token of score i of group j from the lane's first one of the tile.
+    auto token = [](int j, int i) { return 32 * (j >> 1) + 16 * (j & 1) + 8 * (i >> 2) + (i & 3); };
+    // Probabilities of a tile from its scores, at the references as they stand; returns the lane's sum of
+    // them, ls is what they add to l_sum (without the groups of far value scales, whose rv is 0).
+    uint32_t P[2][8], PL[2][PS ? 8 : 1];
+    auto probs = [&](const v16f* S, int tile, float& ls) {
+        float all = 0.0f;
+        ls = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int gi = 4 * (tile & 15) + j, o = 8 * (j & 1);
+            const v16f& x = S[j >> 1];
+            const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0, shift = read_lane(cur.lv, gi) - p_ref;
+            float sum = 0.0f;
+            const h2v ones = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const v2f p = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[o + i], f, shift)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[o + i + 1], f, shift))};
+                const h2v ph = __builtin_convertvector(p, h2v);
+                P[j >> 1][(o + i) >> 1] = __builtin_bit_cast(uint32_t, ph);
+                if constexpr (PS) {
+                    const h2v pl = __builtin_convertvector((v2f{p[0] - (float)ph[0], p[1] - (float)ph[1]}), h2v);
+                    PL[j >> 1][(o + i) >> 1] = __builtin_bit_cast(uint32_t, pl);
+                    sum += p[0] + p[1];
+                } else {  // the sum of what the product takes
+                    sum = __builtin_amdgcn_fdot2(ph, ones, sum, false);
+                }
+            }
+            all += sum;
+            ls = __builtin_fmaf(sum, read_lane(cur.rv, gi), ls);
+        }
+        ls *= back;
+        return all;
+    };
+    auto softmax = [&](const v16f* S, int tile) {
+        float ls;
+        const float all = probs(S, tile, ls);
+        const uint32_t far = (uint32_t)(far_groups >> (4 * (tile & 15))) & 15;
+        if (far || __builtin_amdgcn_ballot_w64(!(all <= 32768.0f))) {
+            // some probability is too large, or may be: the references move to the tile's own largest
+            float topp = -__builtin_inff(), tops = -__builtin_inff();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int gi = 4 * (tile & 15) + j, o = 8 * (j & 1);
+                const v16f& x = S[j >> 1];
+                const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0;
+                const float y = fmaxf(fmaxf(fmaxf(x[o], x[o + 1]), fmaxf(x[o + 2], x[o + 3])), fmaxf(fmaxf(x[o + 4], x[o + 5]), fmaxf(x[o + 6], x[o + 7]))) * f;
+                tops = fmaxf(tops, y);
+                topp = fmaxf(topp, y + read_lane(cur.lv, gi));
+            }
+            const float pn = fmaxf(p_ref, xmax32(topp) - KV_LIFT_SUM), mn = fmaxf(m_ref, xmax32(tops));
+            const float ap = __builtin_amdgcn_exp2f(p_ref - pn), am = __builtin_amdgcn_exp2f(m_ref - mn);
+            p_ref = pn;
+            m_ref = mn;
+            back = __builtin_amdgcn_exp2f(pn - mn);
+            l_sum *= am;
+#pragma unroll
+            for (int b = 0; b < NDB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) O[b][e] *= ap;
+            probs(S, tile, ls);
+            if (far)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int gi = 4 * (tile & 15) + j, o = 8 * (j & 1);
+                    const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0, on = (float)(far >> j & 1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ls = __builtin_fmaf(on, __builtin_amdgcn_exp2f(__builtin_fmaf(S[j >> 1][o + i], f, -m_ref)), ls);
+                }
+        }
+        l_sum += ls;
+    };
+    // What the sixteen tiles of cur have that is out of the ordinary.  Scores of blocks that are not there
+    // are hidden, and so are those that a row does not see, before anything is made of them; where a
+    // block's scales are not finite the others become NaN, and the scales ones.  Value scales of zero or beyond
+    // 2^40 either way add to l_sum on a way of their own.
+    auto sort_groups = [&]() {
+        const bool off = cur.id < 0, bad = !off && !(cur.f <= 1e37f && cur.lv < __builtin_inff() && cur.lv == cur.lv);
+        const bool far = !off && !bad && !(fabsf(cur.lv) <= 40.0f);
+        if (off || bad) cur.f = cur.rv = 1.0f, cur.lv = 0.0f;
+        if (far) cur.rv = 0.0f;
+        cur.f = fmaxf(cur.f, 1e-37f);  // (0 times a hidden score)
+        hide_groups = __builtin_amdgcn_ballot_w64(off);
+        nan_groups = __builtin_amdgcn_ballot_w64(bad);
+        far_groups = __builtin_amdgcn_ballot_w64(far);
+    };
+    auto hide = [&](v16f* S, int tile) {
+        const int t = tb + 64 * tile + 4 * g, shift = 4 * (tile & 15);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t n = hide_groups >> (shift + j) & 1 ? 0u : (uint32_t)max(see_hi - see_lo, 0);
+            const float add = nan_groups >> (shift + j) & 1 ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = S[j >> 1][8 * (j & 1) + i];
+                S[j >> 1][8 * (j & 1) + i] = (uint32_t)(token(j, i) + t - see_lo) < n ? x + add : -__builtin_inff();
+            }
+        }
+    };
+    // V^T fragments by transposing reads (fattn.hip)
+    auto output = [&](const _Float16* lds) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int rw = 4 * g + ((ln & 15) >> 2), qd = ln & 3;
+        int vtoff[NDB];
+#pragma unroll
+        for (int b = 0; b < NDB; ++b) vtoff[b] = rw * 2 * D + 16 * ((4 * b + 2 * ((ln >> 4) & 1) + (qd >> 1)) ^ vswz<D>(rw)) + 8 * (qd & 1);
+#pragma unroll
+        for (int b = 0; b < NDB; ++b)
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const char* vt = reinterpret_cast<const char*>(lds) + vtoff[b] + (32 * kh + 16 * hh) * 2 * D;
+                    const uint2 lo = lds_read_tr16(vt), hi = lds_read_tr16(vt + 8 * 2 * D);
+                    const v8h v8 = __builtin_bit_cast(v8h, (u32x4{lo.x, lo.y, hi.x, hi.y}));
+                    const u32x4 p = {P[kh][4 * hh], P[kh][4 * hh + 1], P[kh][4 * hh + 2], P[kh][4 * hh + 3]};
+                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, __builtin_bit_cast(v8h, p), O[b], 0, 0, 0);
+                    if constexpr (PS) {
+                        const u32x4 e = {PL[kh][4 * hh], PL[kh][4 * hh + 1], PL[kh][4 * hh + 2], PL[kh][4 * hh + 3]};
+                        O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
+                    }
+                }
+    };
+
+    const int nt = te > tb ? (te - tb + 63) / 64 : 0;
+    if (nt > 0) {
+        // Step t: scores, softmax and output of tile t; then the bytes of tile t + 1, loaded a step before, become
+        // halves in the buffers that step t - 1 read, and those of tile t + 2 are asked for.  One barrier a step.
+        cur.id = group_block(a, table, group_of(0));
+        nxt.id = group_block(a, table, group_of(16));
+        group_scales(a, hk, sc, cur);
+        sort_groups();
+        load_one(c.k, kreg, 0);
+        load_one(c.v, vreg, 0);
+        store_one(sK[0], kreg, true);
+        store_one(sV[0], vreg, false);
+        load_one(c.k, kreg, 1);
+        load_one(c.v, vreg, 1);
+        for (int t = 0; t < nt; ++t) {
+            const int t0 = tb + 64 * t, cb = t & 1;
+            lds_barrier();
+            tile0 = t;
+            if ((t & 15) == 0 && t > 0) {
+                cur = nxt;
+                sort_groups();
+                nxt.id = group_block(a, table, group_of(t + 16));
+            }
+            if ((t & 15) == 8) group_scales(a, hk, sc, nxt);
+            v16f S[2];
+            score(sK[cb], S);
+            if (t0 < all_lo || t0 + 64 > all_hi || (((hide_groups | nan_groups) >> (4 * (t & 15))) & 15)) hide(S, t);
+            softmax(S, t);
+            output(sV[cb]);
+            store_one(sK[cb ^ 1], kreg, true);
+            store_one(sV[cb ^ 1], vreg, false);
+            load_one(c.k, kreg, t + 2);
+            load_one(c.v, vreg, t + 2);
+        }
+    }
+
+    if (!on) return;
+    l_sum = xsum32(l_sum);
+    float f = 1.0f;
+    char* out;
+    if (splits > 1) {
+        const int64_t pr = (((int64_t)sp * c.n_seq + s) * a.n_q + iq) * a.heads + h;
+        out = reinterpret_cast<char*>(a.part + pr * D);
+        if (g == 0) *reinterpret_cast<v4f*>(a.part + (int64_t)splits * c.n_seq * a.n_q * a.heads * D + pr * 4) = v4f{m_ref, p_ref, l_sum, 0.0f};
+    } else {
+        f = l_sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref - m_ref) / l_sum;
+        out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
+    }
+    const bool h16 = splits == 1 && a.d16;
+#pragma unroll
+    for (int b = 0; b < NDB; ++b)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            const int e = 32 * b + 8 * i4 + 4 * g;
+            const v4f y = v4f{O[b][4 * i4], O[b][4 * i4 + 1], O[b][4 * i4 + 2], O[b][4 * i4 + 3]} * f;
+            if (h16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y, v4h);
+            else *reinterpret_cast<v4f_a4*>(out + 4 * e) = y;
+        }
 }
 
 // The ranges' joins: thread per four elements of a row
@@ -416,7 +780,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
         l += ml[x * rows * 4 + 2] * __builtin_amdgcn_exp2f(ml[x * rows * 4] - m);
         o = o + *reinterpret_cast<const v4f*>(po + x * rows * D) * __builtin_amdgcn_exp2f(ml[x * rows * 4 + 1] - p);
     }
-    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m + 9.0f) / l;
+    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m) / l;
     o = o * f;
     char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
     if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(o, v4h);
@@ -428,11 +792,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
 KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int D, int cus) {
     KvAttnPlan p;
     const int64_t rows = (int64_t)n_q * (heads / heads_kv);
-    p.nt = rows > 16 ? 2 : 1;
-    p.tiles = (int)((rows + 16 * p.nt - 1) / (16 * p.nt));
+    p.nt = rows > 64 ? 0 : rows > 16 ? 2 : 1;
+    const int rt = p.nt ? 16 * p.nt : 128;
+    p.tiles = (int)((rows + rt - 1) / rt);
     const int64_t wgs = std::max<int64_t>((int64_t)p.tiles * heads_kv * n_seq, 1);
     const int64_t most = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);
-    p.splits = (int)std::max<int64_t>(std::min<int64_t>({(16LL * std::max(cus, 1) + wgs - 1) / wgs, most, 128}), 1);
+    p.splits = (int)std::max<int64_t>(std::min<int64_t>({((p.nt ? 16LL : 4LL) * std::max(cus, 1) + wgs - 1) / wgs, p.nt ? most : (most + 3) / 4, 128}), 1);
     p.bytes = p.splits > 1 ? (size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 : 0;
     return p;
 }
@@ -452,7 +817,18 @@ static hipError_t kv_attn_d(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_
         else if (a.d16) rows_launch<D, NT, true, false>(a, p, st);
         else rows_launch<D, NT, true, true>(a, p, st);
     };
-    if (p.nt == 1) go(std::integral_constant<int, 1>());
+    const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
+    auto tile = [&](auto qs, auto ps) {
+        const int spread = items % 8 == 0 || items >= 64;
+        const unsigned grid = (unsigned)((spread ? (items + 7) / 8 * 8 : items) * p.tiles);
+        kv_attn_tiles_kernel<D, decltype(qs)::value, decltype(ps)::value><<<grid, 256, 0, st>>>(a, p.splits, p.tiles, spread);
+    };
+    if (p.nt == 0) {
+        if (a.q16 && a.d16) tile(std::false_type(), std::false_type());
+        else if (a.q16) tile(std::false_type(), std::true_type());
+        else if (a.d16) tile(std::true_type(), std::false_type());
+        else tile(std::true_type(), std::true_type());
+    } else if (p.nt == 1) go(std::integral_constant<int, 1>());
     else go(std::integral_constant<int, 2>());
     if (p.splits > 1) {
         const int64_t n = (int64_t)a.c.n_seq * a.n_q * a.heads * (D / 4);
