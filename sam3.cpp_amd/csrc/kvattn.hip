@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 // are computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.  A lane's
 // eight scores (kh, hh) belong to 16 tokens of one block: scales and validity are uniform over them.
 template <int D, bool QS, bool PS>
-__global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles, const int spread) {
+__global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
     constexpr int UB = D == 96 ? 8 : 16;            // bytes of a staging unit
     constexpr int UR = D / UB, NU = 16 * UR / 64;   // units of a row, units of a thread
@@ -442,18 +442,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
     const KvView& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // spread: items go to the XCDs in turn with all their row tiles; else row tiles do
-    int item, tile;
-    if (spread) {
-        const int per = 8 * tiles, rb = blockIdx.x % per;
-        item = (int)(blockIdx.x / per) * 8 + (rb & 7);
-        tile = rb >> 3;
-    } else {
-        item = blockIdx.x / tiles;
-        tile = blockIdx.x % tiles;
-    }
-    if (item >= splits * c.heads * c.n_seq) return;
-    tile = tiles - 1 - tile;  // causal: the longest rows first
+    // Eight items (one to an XCD, whose bytes stay in its L2) at a time, and of them the last row tiles
+    // first: causal ones are the longest.
+    const int items = splits * c.heads * c.n_seq, first = blockIdx.x / (8 * tiles) * 8, left = blockIdx.x - first * tiles;
+    const int many = min(8, items - first), item = first + left % many, tile = tiles - 1 - left / many;
     const int sp = item % splits, hk = item / splits % c.heads, s = item / splits / c.heads;
     const KvRange kr = kv_range(a, s);
     const int rows = kr.nq * a.group, row0 = tile * 128;
@@ -532,40 +524,49 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
 #pragma unroll
         for (int j = 0; j < NU; ++j) reg[j] = *reinterpret_cast<const unit_t*>(p + UB * (lane + 64 * j));
     };
-    auto store_one = [&](_Float16* lds, const unit_t* reg, bool key) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
+    constexpr int NW = NU * UB / 8;  // eight elements each
+    // LDS addresses: 16-byte chunk c of row r lies in slot c ^ swizzle(r) of it.  A row's bytes are a power of two
+    // (D = 96: are added afterwards), so that a chunk further on is one exclusive or away.
+    int kst[NU], vst[NU];
 #pragma unroll
-        for (int j = 0; j < NU; ++j) {
-            const int u = ln + 64 * j, row = 16 * w + u / UR;
-#pragma unroll
-            for (int e = 0; e < UB / 8; ++e) {
-                uint32_t f[4];
-                key_halves(reg[j][2 * e], f);
-                key_halves(reg[j][2 * e + 1], f + 2);
-                const int chunk8 = (UB / 8) * (u % UR) + e, slot = chunk8 ^ (key ? kswz<D>(row) : vswz<D>(row));
-                *reinterpret_cast<u32x4*>(&lds[row * D + 8 * slot]) = u32x4{f[0], f[1], f[2], f[3]};
-            }
-        }
+    for (int j = 0; j < NU; ++j) {
+        const int u = lane + 64 * j, row = 16 * w + u / UR, chunk8 = (UB / 8) * (u % UR);
+        kst[j] = row * 2 * D + 16 * (chunk8 ^ kswz<D>(row));
+        vst[j] = row * 2 * D + 16 * (chunk8 ^ vswz<D>(row));
+    }
+    auto store8 = [&](_Float16* lds, const unit_t* reg, const int* st, int i) {
+        const int j = i / (UB / 8), e = i % (UB / 8);
+        uint32_t f[4];
+        key_halves(reg[j][2 * e], f);
+        key_halves(reg[j][2 * e + 1], f + 2);
+        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(lds) + (st[j] ^ (16 * e))) = u32x4{f[0], f[1], f[2], f[3]};
     };
+    auto store_one = [&](_Float16* lds, const unit_t* reg, const int* st) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) store8(lds, reg, st, i);
+    };
+    const int krow = lr * 2 * D, kchunk = 16 * (g ^ kswz<D>(lr));
+    auto key_frag = [&](const _Float16* lds, int pre, int m, int kh) {
+        const int at = D == 96 ? krow + (pre ^ (32 * m)) : pre ^ (32 * m);
+        return *reinterpret_cast<const v8h*>(reinterpret_cast<const char*>(lds) + at + kh * 64 * D);
+    };
+    const int kpre = D == 96 ? kchunk : krow + kchunk;
+    const int vrow = 4 * g + ((lane & 15) >> 2), vpre = vrow * 2 * D + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ vswz<D>(vrow)) + 8 * (lane & 1);
+
     v16f O[NDB];
 #pragma unroll
     for (int i = 0; i < NDB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) O[i][e] = 0.0f;
     float m_ref = KV_NONE, p_ref = KV_NONE, l_sum = 0.0f, back = 1.0f;  // back = 2^(p_ref - m_ref)
-    // (the LDS addresses follow from one register by a few instructions; kept, they would push the queries out)
     auto score = [&](const _Float16* lds, v16f* S) {
-        int lrow = lr;
-        asm volatile("" : "+v"(lrow));
         const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         S[0] = S[1] = z;
 #pragma unroll
         for (int m = 0; m < NC; ++m)
 #pragma unroll
             for (int kh = 0; kh < 2; ++kh) {
-                const int row = 32 * kh + lrow;
-                const v8h k8 = *reinterpret_cast<const v8h*>(&lds[row * D + 8 * ((2 * m + g) ^ kswz<D>(row))]);
+                const v8h k8 = key_frag(lds, kpre, m, kh);
                 S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q[m], S[kh], 0, 0, 0);
                 if constexpr (QS) S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[m], S[kh], 0, 0, 0);
             }
@@ -576,40 +577,65 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
     // Probabilities of a tile from its scores, at the references as they stand; returns the lane's sum of
     // them, ls is what they add to l_sum (without the groups of far value scales, whose rv is 0).
     uint32_t P[2][8], PL[2][PS ? 8 : 1];
-    auto probs = [&](const v16f* S, int tile, float& ls) {
-        float all = 0.0f;
-        ls = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int gi = 4 * (tile & 15) + j, o = 8 * (j & 1);
-            const v16f& x = S[j >> 1];
-            const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0, shift = read_lane(cur.lv, gi) - p_ref;
-            float sum = 0.0f;
-            const h2v ones = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const v2f p = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[o + i], f, shift)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[o + i + 1], f, shift))};
-                const h2v ph = __builtin_convertvector(p, h2v);
-                P[j >> 1][(o + i) >> 1] = __builtin_bit_cast(uint32_t, ph);
-                if constexpr (PS) {
-                    const h2v pl = __builtin_convertvector((v2f{p[0] - (float)ph[0], p[1] - (float)ph[1]}), h2v);
-                    PL[j >> 1][(o + i) >> 1] = __builtin_bit_cast(uint32_t, pl);
-                    sum += p[0] + p[1];
-                } else {  // the sum of what the product takes
-                    sum = __builtin_amdgcn_fdot2(ph, ones, sum, false);
-                }
-            }
-            all += sum;
-            ls = __builtin_fmaf(sum, read_lane(cur.rv, gi), ls);
-        }
-        ls *= back;
-        return all;
+    struct Sums {
+        float s[4];
     };
-    auto softmax = [&](const v16f* S, int tile) {
-        float ls;
-        const float all = probs(S, tile, ls);
+    // pair n of a tile's sixteen pairs of scores
+    auto pair = [&](const v16f* S, int tile, int n, Sums& sums) {
+        const int j = n >> 2, gi = 4 * (tile & 15) + j;
+        const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0, shift = read_lane(cur.lv, gi) - p_ref;
+        const v16f& x = S[n >> 3];
+        const int i = 2 * (n & 7);
+        const v2f p = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], f, shift)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], f, shift))};
+        const h2v ph = __builtin_convertvector(p, h2v), ones = {(_Float16)1.0f, (_Float16)1.0f};
+        P[n >> 3][n & 7] = __builtin_bit_cast(uint32_t, ph);
+        if ((n & 3) == 0) sums.s[j] = 0.0f;
+        if constexpr (PS) {
+            const h2v pl = __builtin_convertvector((v2f{p[0] - (float)ph[0], p[1] - (float)ph[1]}), h2v);
+            PL[n >> 3][n & 7] = __builtin_bit_cast(uint32_t, pl);
+            sums.s[j] += p[0] + p[1];
+        } else {  // the sum of what the product takes
+            sums.s[j] = __builtin_amdgcn_fdot2(ph, ones, sums.s[j], false);
+        }
+    };
+    auto add_up = [&](const Sums& sums, int tile) {
+        float ls = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ls = __builtin_fmaf(sums.s[j], read_lane(cur.rv, 4 * (tile & 15) + j), ls);
+        return ls * back;
+    };
+    // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
+    // a product's fragments are read while the product before multiplies, and pairs go between the products.
+    auto score_softmax = [&](const _Float16* lds, v16f* Sn, const v16f* S, int tile) {
+        int pre = kpre;
+        asm volatile("" : "+v"(pre));  // (the addresses are made here: kept over the loop, they would push the queries out)
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        v8h k8[2], k8n[2];
+        auto frag = [&](int m, v8h* o) {
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) o[kh] = key_frag(lds, pre, m, kh);
+        };
+        frag(0, k8);
+        Sn[0] = Sn[1] = z;
+        Sums sums;
+#pragma unroll
+        for (int m = 0; m < NC; ++m) {
+            if (m + 1 < NC) frag(m + 1, k8n);
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], q[m], Sn[kh], 0, 0, 0);
+                if constexpr (QS) Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], ql[m], Sn[kh], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 16 * m / NC; n < 16 * (m + 1) / NC; ++n) pair(S, tile, n, sums);
+            k8[0] = k8n[0];
+            k8[1] = k8n[1];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const float all = (sums.s[0] + sums.s[1]) + (sums.s[2] + sums.s[3]);
+        float ls = add_up(sums, tile);
         const uint32_t far = (uint32_t)(far_groups >> (4 * (tile & 15))) & 15;
-        if (far || __builtin_amdgcn_ballot_w64(!(all <= 32768.0f))) {
+        if (__builtin_amdgcn_ballot_w64((int)!(all <= 32768.0f) | (int)(far != 0))) {
             // some probability is too large, or may be: the references move to the tile's own largest
             float topp = -__builtin_inff(), tops = -__builtin_inff();
 #pragma unroll
@@ -631,7 +657,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             for (int b = 0; b < NDB; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) O[b][e] *= ap;
-            probs(S, tile, ls);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) pair(S, tile, n, sums);
+            ls = add_up(sums, tile);
             if (far)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -671,47 +699,63 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
         }
     };
     // V^T fragments by transposing reads (fattn.hip)
-    auto output = [&](const _Float16* lds) {
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const int rw = 4 * g + ((ln & 15) >> 2), qd = ln & 3;
-        int vtoff[NDB];
+    // The output of the tile in lds, and the staged bytes of the next ones into their buffers between the products
+    auto output_store = [&](const _Float16* lds, _Float16* vnext, _Float16* knext) {
+        int pre = vpre;
+        asm volatile("" : "+v"(pre));
+        auto frag = [&](int i) {  // product i: 16 tokens i / NDB, output block i % NDB
+            const int b = i % NDB;
+            const char* vt = reinterpret_cast<const char*>(lds) + (D == 96 ? pre + 64 * b : pre ^ (64 * b)) + 16 * (i / NDB) * 2 * D;
+            const uint2 lo = lds_read_tr16(vt), hi = lds_read_tr16(vt + 8 * 2 * D);
+            return __builtin_bit_cast(v8h, (u32x4{lo.x, lo.y, hi.x, hi.y}));
+        };
+        v8h v8[2] = {frag(0), frag(1)}, v8n[2];
+        static_assert(4 * NDB == 4 * NW, "a unit of both to two products");
 #pragma unroll
-        for (int b = 0; b < NDB; ++b) vtoff[b] = rw * 2 * D + 16 * ((4 * b + 2 * ((ln >> 4) & 1) + (qd >> 1)) ^ vswz<D>(rw)) + 8 * (qd & 1);
+        for (int x = 0; x < 2 * NDB; ++x) {
+            if (x + 1 < 2 * NDB) {
+                v8n[0] = frag(2 * x + 2);
+                v8n[1] = frag(2 * x + 3);
+            }
 #pragma unroll
-        for (int b = 0; b < NDB; ++b)
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    const char* vt = reinterpret_cast<const char*>(lds) + vtoff[b] + (32 * kh + 16 * hh) * 2 * D;
-                    const uint2 lo = lds_read_tr16(vt), hi = lds_read_tr16(vt + 8 * 2 * D);
-                    const v8h v8 = __builtin_bit_cast(v8h, (u32x4{lo.x, lo.y, hi.x, hi.y}));
-                    const u32x4 p = {P[kh][4 * hh], P[kh][4 * hh + 1], P[kh][4 * hh + 2], P[kh][4 * hh + 3]};
-                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, __builtin_bit_cast(v8h, p), O[b], 0, 0, 0);
-                    if constexpr (PS) {
-                        const u32x4 e = {PL[kh][4 * hh], PL[kh][4 * hh + 1], PL[kh][4 * hh + 2], PL[kh][4 * hh + 3]};
-                        O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
-                    }
+            for (int y = 0; y < 2; ++y) {
+                const int i = 2 * x + y, kh = i / NDB / 2, hh = i / NDB & 1, b = i % NDB;
+                const u32x4 p = {P[kh][4 * hh], P[kh][4 * hh + 1], P[kh][4 * hh + 2], P[kh][4 * hh + 3]};
+                O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, p), O[b], 0, 0, 0);
+                if constexpr (PS) {
+                    const u32x4 e = {PL[kh][4 * hh], PL[kh][4 * hh + 1], PL[kh][4 * hh + 2], PL[kh][4 * hh + 3]};
+                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
                 }
+            }
+            if (x < NW) store8(vnext, vreg, vst, x);
+            else store8(knext, kreg, kst, x - NW);
+            v8[0] = v8n[0];
+            v8[1] = v8n[1];
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
 
     const int nt = te > tb ? (te - tb + 63) / 64 : 0;
     if (nt > 0) {
-        // Step t: scores, softmax and output of tile t; then the bytes of tile t + 1, loaded a step before, become
-        // halves in the buffers that step t - 1 read, and those of tile t + 2 are asked for.  One barrier a step.
+        // Step t: the scores of tile t + 1 beside the softmax of tile t, and its output; then the bytes of K(t + 2) and
+        // V(t + 1), loaded a step before, become halves in the buffers that step t - 1 read last.  One barrier a step.
         cur.id = group_block(a, table, group_of(0));
         nxt.id = group_block(a, table, group_of(16));
         group_scales(a, hk, sc, cur);
         sort_groups();
+        v16f SA[2], SB[2];
         load_one(c.k, kreg, 0);
+        store_one(sK[0], kreg, kst);
         load_one(c.v, vreg, 0);
-        store_one(sK[0], kreg, true);
-        store_one(sV[0], vreg, false);
+        store_one(sV[0], vreg, vst);
         load_one(c.k, kreg, 1);
+        store_one(sK[1], kreg, kst);
+        load_one(c.k, kreg, 2);
         load_one(c.v, vreg, 1);
-        for (int t = 0; t < nt; ++t) {
-            const int t0 = tb + 64 * t, cb = t & 1;
+        __syncthreads();
+        score(sK[0], SA);
+        auto step = [&](int t, int cb, v16f* Sc, v16f* Sn) {
+            const int t0 = tb + 64 * t;
             lds_barrier();
             tile0 = t;
             if ((t & 15) == 0 && t > 0) {
@@ -720,15 +764,15 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
                 nxt.id = group_block(a, table, group_of(t + 16));
             }
             if ((t & 15) == 8) group_scales(a, hk, sc, nxt);
-            v16f S[2];
-            score(sK[cb], S);
-            if (t0 < all_lo || t0 + 64 > all_hi || (((hide_groups | nan_groups) >> (4 * (t & 15))) & 15)) hide(S, t);
-            softmax(S, t);
-            output(sV[cb]);
-            store_one(sK[cb ^ 1], kreg, true);
-            store_one(sV[cb ^ 1], vreg, false);
-            load_one(c.k, kreg, t + 2);
+            if (t0 < all_lo || t0 + 64 > all_hi || (((hide_groups | nan_groups) >> (4 * (t & 15))) & 15)) hide(Sc, t);
+            score_softmax(sK[cb ^ 1], Sn, Sc, t);
+            output_store(sV[cb], sV[cb ^ 1], sK[cb]);
             load_one(c.v, vreg, t + 2);
+            load_one(c.k, kreg, t + 3);
+        };
+        for (int t = 0; t < nt; t += 2) {
+            step(t, 0, SA, SB);
+            if (t + 1 < nt) step(t + 1, 1, SB, SA);
         }
     }
 
@@ -797,7 +841,17 @@ KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max
     p.tiles = (int)((rows + rt - 1) / rt);
     const int64_t wgs = std::max<int64_t>((int64_t)p.tiles * heads_kv * n_seq, 1);
     const int64_t most = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);
-    p.splits = (int)std::max<int64_t>(std::min<int64_t>({((p.nt ? 16LL : 4LL) * std::max(cus, 1) + wgs - 1) / wgs, p.nt ? most : (most + 3) / 4, 128}), 1);
+    if (p.nt) {
+        p.splits = (int)std::max<int64_t>(std::min<int64_t>({(16LL * std::max(cus, 1) + wgs - 1) / wgs, most, 128}), 1);
+    } else {  // two workgroups of 128 rows to a CU: the ranges whose rounds over the CUs take the least time
+        const int64_t slots = 2LL * std::max(cus, 1);
+        double best = 0.0;
+        p.splits = 1;
+        for (int s = 1; s <= 16 && (s == 1 || most >= 4 * s); ++s) {
+            const double t = (double)((wgs * s + slots - 1) / slots) * ((double)most / s + 2.0) + (s > 1 ? 1.0 + 0.02 * s * (double)wgs / slots : 0.0);
+            if (s == 1 || t < best) best = t, p.splits = s;
+        }
+    }
     p.bytes = p.splits > 1 ? (size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 : 0;
     return p;
 }
@@ -819,9 +873,7 @@ static hipError_t kv_attn_d(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_
     };
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
     auto tile = [&](auto qs, auto ps) {
-        const int spread = items % 8 == 0 || items >= 64;
-        const unsigned grid = (unsigned)((spread ? (items + 7) / 8 * 8 : items) * p.tiles);
-        kv_attn_tiles_kernel<D, decltype(qs)::value, decltype(ps)::value><<<grid, 256, 0, st>>>(a, p.splits, p.tiles, spread);
+        kv_attn_tiles_kernel<D, decltype(qs)::value, decltype(ps)::value><<<(unsigned)(items * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles);
     };
     if (p.nt == 0) {
         if (a.q16 && a.d16) tile(std::false_type(), std::false_type());
