@@ -299,7 +299,6 @@ struct RmsArgs {
     float eps;
     bool xf16;                 // x, add and sum; else F32
     int out;                   // T_F32, T_F16, T_Q8_0, T_Q8_1
-    bool vec;                  // n % 8 == 0 and every row of x, add, sum (and F32 / F16 dst) on 16 bytes
 };
 constexpr int RMS_MAX = 32768;
 hipError_t launch_rms_norm(const RmsArgs& a, hipStream_t st);
@@ -316,7 +315,7 @@ struct RopeArgs {
     char* dst;
     int64_t s_nb[3], d_nb[3];  // strides of heads, tokens, batches
     int heads, tokens, batch, ne0, pairs;
-    bool f16, halves, vec;
+    bool f16, halves;
     const int32_t* pos;        // [axes][batch][tokens]
     uint64_t turn[ROPE_PAIRS]; // turns a position, times 2^64
     uint8_t axis[ROPE_PAIRS];

@@ -86,6 +86,17 @@ bool rope_table(const mi355_rope_params* p, RopeArgs* a) {
         total += s;
     }
     if (total != n || (p->order == MI355_ROPE_INTERLEAVED && p->sections[3] != 0)) return false;
+    // freq_base ^ (-2^k / size) by squaring, of one size or each axis's: a power is a product of at most seven.
+    // 64-bit mantissas and a relative 2^-57 at most leave an int32 position's angle good to 2^-32 of a turn.
+    long double root[4][7];
+    if (a)
+        for (int s = 0; s < (p->restart ? 4 : 1); ++s) {
+            const int size = p->restart ? p->sections[s] : n;
+            if (size == 0) continue;
+            root[s][0] = powl((long double)p->freq_base, -1.0L / (long double)size);
+            for (int k = 1; k < 7; ++k) root[s][k] = root[s][k - 1] * root[s][k - 1];
+        }
+    const long double unit = (long double)p->freq_scale / 6.283185307179586476925286766559L;
     int count[4] = {0, 0, 0, 0}, axis = 0;
     for (int i = 0; i < n; ++i) {
         if (p->order == MI355_ROPE_INTERLEAVED) {
@@ -94,14 +105,14 @@ bool rope_table(const mi355_rope_params* p, RopeArgs* a) {
         } else {
             while (count[axis] == p->sections[axis]) ++axis;  // total == n: an axis with room is left
         }
-        const int e = p->restart ? count[axis] : i, size = p->restart ? p->sections[axis] : n;
+        const int e = p->restart ? count[axis] : i;
         ++count[axis];
         if (!a) continue;
-        // powl and this product are good to 2^-63: int32 positions times it to 2^-32 of a turn
-        const long double f = (long double)p->freq_scale * powl((long double)p->freq_base, -(long double)e / (long double)size) /
-                              6.283185307179586476925286766559L;
-        const long double frac = f - floorl(f);
-        const uint64_t turn = (uint64_t)(frac * 18446744073709551616.0L);
+        long double f = unit;
+        for (int k = 0; k < 7; ++k)
+            if (e >> k & 1) f *= root[p->restart ? axis : 0][k];
+        if (!(f >= 0.0L && f < 1.0L)) f -= floorl(f);
+        const uint64_t turn = f < 1.0L ? (uint64_t)(f * 18446744073709551616.0L) : 0;
         a->turn[i] = p->inverse ? 0 - turn : turn;
         a->axis[i] = (uint8_t)axis;
     }
@@ -119,7 +130,8 @@ mi355_status check_rope(mi355_context* ctx, const mi355_tensor* src, const mi355
     if (!same_ne(src, dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "rope_multi: shape mismatch");
     if (p->n_dims > src->ne[0]) return fail(ctx, MI355_STATUS_INVALID_ARG, "rope_multi: n_dims %d beyond ne0", p->n_dims);
     if (!rows_ok(src) || !rows_ok(dst)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "rope_multi: rows must be contiguous and aligned to their type");
-    if (!rows_fit(src) || src->ne[0] > 65536) return fail(ctx, MI355_STATUS_UNSUPPORTED, "rope_multi: sizes beyond the launch limits");
+    if (!rows_fit(src) || src->ne[0] > 65536 || (double)src->ne[2] * src->ne[3] * ((src->ne[1] + 3) / 4) * (src->ne[0] / 8 + 2) > 2147483000.0)
+        return fail(ctx, MI355_STATUS_UNSUPPORTED, "rope_multi: sizes beyond the launch limits");
     return MI355_STATUS_SUCCESS;
 }
 
@@ -222,8 +234,6 @@ mi355_status mi355_rms_norm(mi355_context* ctx, const mi355_tensor* x, const mi3
     a.eps = eps;
     a.xf16 = x->type == T_F16;
     a.out = dst->type;
-    a.vec = a.n % 8 == 0 && rows_on(x, 16) && (!add || rows_on(add, 16)) && (!sum || rows_on(sum, 16)) &&
-            (!is_float(dst->type) || rows_on(dst, 16)) && (reinterpret_cast<uintptr_t>(w) & 15) == 0;
     Timed tm(ctx, "rms_norm");
     return hip_check(ctx, tm.done(launch_rms_norm(a, ctx->stream)), "rms_norm launch");
 }
@@ -267,7 +277,6 @@ mi355_status mi355_rope_multi(mi355_context* ctx, const mi355_tensor* src, const
     a.pairs = p->n_dims / 2;
     a.f16 = src->type == T_F16;
     a.halves = p->pairs == MI355_ROPE_HALVES;
-    a.vec = rows_on(src, 16) && rows_on(dst, 16);
     a.pos = pos;
     Timed tm(ctx, "rope_multi");
     return hip_check(ctx, tm.done(launch_rope_multi(a, ctx->stream)), "rope_multi launch");
