@@ -334,7 +334,7 @@ struct KvRows {                // keys and values [D, n_tok, heads, n_seq]
     char *k, *v;               // either may be null (reading)
     int64_t k_nb[3], v_nb[3];
     int n_tok;
-    bool f16, vec;             // vec: every row on 16 bytes
+    bool f16;
     const int32_t* idx;        // write: n_new [n_seq]; read: pos [n_seq][n_tok]; or null
 };
 hipError_t launch_kv_write(const KvView& c, const KvRows& r, int D, hipStream_t st);

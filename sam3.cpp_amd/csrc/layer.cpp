@@ -167,7 +167,6 @@ mi355_status kv_rows(mi355_context* ctx, const char* op, const mi355_kv_cache* c
                      const mi355_tensor* v, const int32_t* idx, KvRows* r) {
     const mi355_tensor* one = k ? k : v;
     r->k = r->v = nullptr;
-    r->vec = true;
     for (const mi355_tensor* t : {k, v}) {
         if (!t) continue;
         if (!has_data(t)) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: null data pointer", op);
@@ -177,7 +176,6 @@ mi355_status kv_rows(mi355_context* ctx, const char* op, const mi355_kv_cache* c
             return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: k and v must be [head_dim, n_tokens, n_head_kv, n_seq]", op);
         if (!rows_ok(t)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: rows must be contiguous and aligned to their type", op);
         if (!rows_fit(t)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: sizes beyond the launch limits", op);
-        if (!rows_on(t, 16)) r->vec = false;
     }
     if (reinterpret_cast<uintptr_t>(idx) & 3) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: counts and positions must be 4-byte aligned", op);
     if (k) { r->k = static_cast<char*>(k->data); strides(k, r->k_nb); }
