@@ -111,6 +111,21 @@ mi355_status ensure_ws(mi355_context* ctx, size_t bytes) {
     return ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, bytes);
 }
 
+mi355_status ensure_arrived(mi355_context* ctx) {
+    if (ctx->arrived) return MI355_STATUS_SUCCESS;
+    if (capturing(ctx)) return fail(ctx, MI355_STATUS_ALLOC_FAILED, "a captured call needs workspace that the context does not have (mi355_reserve_workspace)");
+    void* p = nullptr;
+    hipError_t e = hipMalloc(&p, KV_ARRIVALS * 4);
+    if (e != hipSuccess) return fail(ctx, MI355_STATUS_ALLOC_FAILED, "hipMalloc(%d): %s", KV_ARRIVALS * 4, hipGetErrorString(e));
+    e = hipMemsetAsync(p, 0, KV_ARRIVALS * 4, ctx->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(p);
+        return hip_check(ctx, e, "hipMemsetAsync");
+    }
+    ctx->arrived = p;
+    return MI355_STATUS_SUCCESS;
+}
+
 }  // namespace mi355
 
 namespace {
@@ -751,6 +766,7 @@ void mi355_context_free(mi355_context* ctx) {
     (void)hipStreamSynchronize(ctx->stream);
     noalloc_release(ctx);
     mi355_profile_reset(ctx);
+    if (ctx->arrived) (void)hipFree(ctx->arrived);
     if (ctx->ws) (void)hipFree(ctx->ws);
     for (void* p : ctx->retired) (void)hipFree(p);
     if (ctx->enc) (void)hipFree(ctx->enc);
@@ -767,7 +783,8 @@ mi355_status mi355_synchronize(mi355_context* ctx) {
 mi355_status mi355_reserve_workspace(mi355_context* ctx, size_t bytes) {
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "reserve_workspace: null context");
     (void)hipSetDevice(ctx->device);
-    return ensure_ws(ctx, bytes);
+    const mi355_status st = bytes ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
+    return st != MI355_STATUS_SUCCESS ? st : ensure_ws(ctx, bytes);
 }
 
 size_t mi355_mul_mat_workspace_size(const mi355_tensor* s0, const mi355_tensor* s1) {

@@ -20,6 +20,7 @@ struct mi355_context {
     size_t ws_size = 0;
     bool ws_captured = false;  // a captured call uses ws: a larger one replaces it without freeing it
     std::vector<void*> retired;  // such workspaces, which captured graphs still name
+    void* arrived = nullptr;   // the cache attention's counters (KV_ARRIVALS), zero between its launches
     void* enc = nullptr;       // activation buffers of the image-encoder runner
     size_t enc_size = 0;
     void* neck = nullptr;      // maps and scratch of the SimpleFPN neck
@@ -68,6 +69,8 @@ mi355_status ensure_buffer(mi355_context* ctx, void** buf, size_t* size, size_t 
 // the stream's work, unless it is large enough.  A workspace that a captured call used is kept until the
 // context is freed; nothing grows under capture.
 mi355_status ensure_ws(mi355_context* ctx, size_t bytes);
+// The cache attention's counters, zeroed on the stream when they are made (not under capture).
+mi355_status ensure_arrived(mi355_context* ctx);
 
 // The activation layout a producer pass should write for weights of type t:
 // Q8 quants for Q8_0/Q4_0, Q8 with Q8_1 sums for Q4_1, F16 for F16, F32 otherwise.

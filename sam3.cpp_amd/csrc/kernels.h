@@ -351,7 +351,9 @@ struct KvAttnArgs {
     int causal, window;
     bool q16, d16;
     float* part;
+    uint32_t* arrived;         // [KV_ARRIVALS], zero between launches: ranges done of a sequence, key head and row tile
 };
+constexpr int KV_ARRIVALS = 8192;
 struct KvAttnPlan {
     int nt, tiles;             // 16-row tiles of a workgroup (0: the kernel of 128 rows), workgroups over a sequence's rows
     int splits;                // ranges of the tokens, joined by a second kernel

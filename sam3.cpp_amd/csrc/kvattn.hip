@@ -108,6 +108,61 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + lane_swap_f<32>(v);
 }
 
+// Four elements from e on of a row's output, joined from its n ranges' partial sums in the ranges' order and written.
+// ONE: another workgroup of this launch wrote them, through the caches; loads that bypass them read them.
+template <int D, bool ONE>
+__device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int n, int s, int iq, int h, int e) {
+    const int64_t rows = (int64_t)a.c.n_seq * a.n_q * a.heads, pr = ((int64_t)s * a.n_q + iq) * a.heads + h;
+    const float* ml = a.part + (int64_t)splits * rows * D + pr * 4;
+    const float* po = a.part + pr * D + e;
+    auto get = [](const float* p) -> v4f {
+        if constexpr (ONE) {
+            const uint64_t* q = reinterpret_cast<const uint64_t*>(p);
+            const uint64_t lo = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const uint64_t hi = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const v2f x = __builtin_bit_cast(v2f, lo), y = __builtin_bit_cast(v2f, hi);
+            return v4f{x[0], x[1], y[0], y[1]};
+        } else {
+            return *reinterpret_cast<const v4f*>(p);
+        }
+    };
+    constexpr int B = 8;  // ranges whose loads are on their way together
+    float m = KV_NONE, p = KV_NONE, l = 0.0f;
+    v4f o = {0, 0, 0, 0};
+    for (int x0 = 0; x0 < n; x0 += B) {
+        v4f z[B], y[B];
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            z[x] = v4f{KV_NONE, KV_NONE, 0, 0};
+            y[x] = v4f{0, 0, 0, 0};
+            if (x0 + x < n) {
+                z[x] = get(ml + (x0 + x) * rows * 4);
+                y[x] = get(po + (x0 + x) * rows * D);
+            }
+        }
+        float mn = m, pn = p;
+#pragma unroll
+        for (int x = 0; x < B; ++x) mn = fmaxf(mn, z[x][0]), pn = fmaxf(pn, z[x][1]);
+        l *= __builtin_amdgcn_exp2f(m - mn);
+        o = o * __builtin_amdgcn_exp2f(p - pn);
+        m = mn;
+        p = pn;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            l += z[x][2] * __builtin_amdgcn_exp2f(z[x][0] - m);
+            o = o + y[x] * __builtin_amdgcn_exp2f(z[x][1] - p);
+        }
+    }
+    o = o * (l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m) / l);
+    char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
+    if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(o, v4h);
+    else *reinterpret_cast<v4f_a4*>(out + 4 * e) = o;
+}
+// A store past the caches of the workgroup's XCD, for a workgroup on another one
+__device__ __forceinline__ void put_through(float* p, v2f v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // Few query rows over many tokens.  A row is one query and head of the group that shares a key head: row
 // r of a sequence and key head is query r / group, head r % group.  A workgroup takes 16 NT rows and
 // one range of the tokens, its four wavefronts every fourth step of 32 tokens; nothing passes through
@@ -144,7 +199,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
     const int last = min(row0 + 16 * NT, rows) - 1;
     const int hi_tile = a.causal ? min(kr.pos0 + last / a.group + 1, kr.hi) : kr.hi;
     const int te = min(min(tb + chunk, kr.hi), hi_tile);
-    if (splits > 1 && sp > 0 && tb >= kr.hi) return;  // no such range (the first always answers)
+    if (sp > 0 && tb >= kr.hi) return;  // no such range (the first always answers)
+    const int ranges = max((kr.hi - kr.lo + chunk - 1) / chunk, 1);
 
     // queries
     v8h q[NT][KM], ql[QS ? NT : 1][KM];
@@ -210,41 +266,52 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
     const int* table = c.table + (int64_t)s * c.max_blocks;
     const float sc = a.scale * KV_LOG2E;
 
+    // A step's two halves of 16 tokens: where their bytes are, and their scales.  The keys of a step are asked for
+    // when the step before has multiplied its own, its values when it begins, so that something is always on its way.
+    struct Step {
+        const uint8_t* vp[2];
+        float ks[2], lv[2];
+        bool there[2];
+    };
     KvGroups gr = {-1, 0.0f, 0.0f, 0.0f};
     int at = 32;
-    for (int t0 = tb + w * KV_STEP; t0 < te; t0 += KV_SPAN, ++at) {
+    u32x4 kv[2][KC];
+    u32x2 kt[2];
+    auto ask = [&](int t0) {
+        Step x;
         if (at == 32) {  // lane 2 i + u: half u of this wavefront's i-th step from here
             gr.id = group_block(a, table, t0 + (lane >> 1) * KV_SPAN + 16 * (lane & 1));
             group_scales(a, hk, sc, gr);
             at = 0;
         }
-        const uint8_t *kp[2], *vp[2];
-        float ks[2], lv[2];
-        bool there[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int id = __builtin_amdgcn_readlane(gr.id, 2 * at + u);
-            there[u] = id >= 0;
             const int64_t off = (((int64_t)max(id, 0) * c.heads + hk) * c.bt + ((t0 + 16 * u) & (c.bt - 1))) * D;
-            kp[u] = c.k + off;
-            vp[u] = c.v + off;
-            ks[u] = read_lane(gr.f, 2 * at + u);
-            lv[u] = read_lane(gr.lv, 2 * at + u);
+            const uint8_t* kp = c.k + off;
+            x.vp[u] = c.v + off;
+            x.there[u] = id >= 0;
+            x.ks[u] = read_lane(gr.f, 2 * at + u);
+            x.lv[u] = read_lane(gr.lv, 2 * at + u);
+#pragma unroll
+            for (int y = 0; y < KC; ++y) kv[u][y] = *reinterpret_cast<const u32x4*>(kp + col * D + 64 * y + 16 * g);
+            if (TAIL) kt[u] = *reinterpret_cast<const u32x2*>(kp + col * D + 64 + 8 * g);
         }
-        u32x4 kv[2][KC];
-        u32x2 kt[2];
+        ++at;
+        return x;
+    };
+    Step next{};
+    if (tb + w * KV_STEP < te) next = ask(tb + w * KV_STEP);
+    for (int t0 = tb + w * KV_STEP; t0 < te; t0 += KV_SPAN) {
+        const Step x0 = next;
+        const float (&ks)[2] = x0.ks, (&lv)[2] = x0.lv;
+        const bool (&there)[2] = x0.there;
         uint32_t vv[2][4][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int x = 0; x < KC; ++x) kv[u][x] = *reinterpret_cast<const u32x4*>(kp[u] + col * D + 64 * x + 16 * g);
-            if (TAIL) kt[u] = *reinterpret_cast<const u32x2*>(kp[u] + col * D + 64 + 8 * g);
-        }
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint8_t* row = vp[u] + (4 * g + i) * D;
+                const uint8_t* row = x0.vp[u] + (4 * g + i) * D;
                 if constexpr (D == 128) {
                     const u32x2 x = *reinterpret_cast<const u32x2*>(row + 8 * col);
                     vv[u][i][0] = x[0];
@@ -274,6 +341,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
                     if (QS) S[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[t][m], S[t][u], 0, 0, 0);
                 }
             }
+
+        if (t0 + KV_SPAN < te) next = ask(t0 + KV_SPAN);
 
         // probabilities
         uint32_t P[NT][4], PL[PS ? NT : 1][4];
@@ -385,43 +454,70 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
         }
         __syncthreads();
     }
-    if (w != 0) return;
+    if (w == 0) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        p_ref[t] += 9.0f;  // the halves were the bytes' values over 512
-        const int r = row0 + 16 * t + col, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
-        if (r >= rows) continue;
-        float f = 1.0f;
-        char* out;
-        if (splits > 1) {
-            const int64_t pr = (((int64_t)sp * c.n_seq + s) * a.n_q + iq) * a.heads + h;
-            out = reinterpret_cast<char*>(a.part + pr * D);
-            if (g == 0) {
-                float* ml = a.part + (int64_t)splits * c.n_seq * a.n_q * a.heads * D + pr * 4;
-                *reinterpret_cast<v4f*>(ml) = v4f{m_ref[t], p_ref[t], l_sum[t], 0.0f};
-            }
-        } else {
-            f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t]) / l_sum[t];
-            out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
-        }
-        const bool h16 = splits == 1 && a.d16;
+        for (int t = 0; t < NT; ++t) {
+            const int r = row0 + 16 * t + col, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
+            if (r >= rows) continue;
+            p_ref[t] += 9.0f;  // the halves were the bytes' values over 512
+            if (ranges > 1) {
+                const int64_t pr = (((int64_t)sp * c.n_seq + s) * a.n_q + iq) * a.heads + h;
+                float* out = a.part + pr * D;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int ar = 4 * g + i;
-            v4f y[2];
+                for (int i = 0; i < 4; ++i) {
+                    const int ar = 4 * g + i;
 #pragma unroll
-            for (int b = 0; b < 8; ++b) y[b >> 2][b & 3] = b < NB ? O[t][b < NB ? b : 0][i] * f : 0.0f;
-            const int e = (D == 128 ? 8 : 4) * ar;
-            if (h16) {
-                *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y[0], v4h);
-                if (D == 128) *reinterpret_cast<v4h_a2*>(out + 2 * e + 8) = __builtin_convertvector(y[1], v4h);
-                if (TAIL) *reinterpret_cast<h2v_a2*>(out + 2 * (64 + 2 * ar)) = __builtin_convertvector((v2f{y[1][0], y[1][1]}), h2v);
+                    for (int b = 0; b < NB; b += 2) {
+                        const int e = D == 128 ? 8 * ar + b : b < 4 ? 4 * ar + b : 64 + 2 * ar;
+                        put_through(out + e, v2f{O[t][b][i], O[t][b + 1][i]});
+                    }
+                }
+                if (g == 0) {
+                    float* ml = a.part + (int64_t)splits * c.n_seq * a.n_q * a.heads * D + pr * 4;
+                    put_through(ml, v2f{m_ref[t], p_ref[t]});
+                    put_through(ml + 2, v2f{l_sum[t], 0.0f});
+                }
             } else {
-                *reinterpret_cast<v4f_a4*>(out + 4 * e) = y[0];
-                if (D == 128) *reinterpret_cast<v4f_a4*>(out + 4 * e + 16) = y[1];
-                if (TAIL) *reinterpret_cast<v2f_a4*>(out + 4 * (64 + 2 * ar)) = v2f{y[1][0], y[1][1]};
+                const float f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t]) / l_sum[t];
+                char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int ar = 4 * g + i;
+                    v4f y[2];
+#pragma unroll
+                    for (int b = 0; b < 8; ++b) y[b >> 2][b & 3] = b < NB ? O[t][b < NB ? b : 0][i] * f : 0.0f;
+                    const int e = (D == 128 ? 8 : 4) * ar;
+                    if (a.d16) {
+                        *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y[0], v4h);
+                        if (D == 128) *reinterpret_cast<v4h_a2*>(out + 2 * e + 8) = __builtin_convertvector(y[1], v4h);
+                        if (TAIL) *reinterpret_cast<h2v_a2*>(out + 2 * (64 + 2 * ar)) = __builtin_convertvector((v2f{y[1][0], y[1][1]}), h2v);
+                    } else {
+                        *reinterpret_cast<v4f_a4*>(out + 4 * e) = y[0];
+                        if (D == 128) *reinterpret_cast<v4f_a4*>(out + 4 * e + 16) = y[1];
+                        if (TAIL) *reinterpret_cast<v2f_a4*>(out + 4 * (64 + 2 * ar)) = v2f{y[1][0], y[1][1]};
+                    }
+                }
             }
         }
+    }
+    if (ranges == 1) return;
+    // The workgroup that comes last joins the ranges.  What the others wrote is in memory before they count
+    // themselves, and the counter goes back to zero for the next launch.
+    __shared__ int join;
+    if (w == 0) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (lane == 0) {
+            uint32_t* n = a.arrived + ((int64_t)s * c.heads + hk) * tiles + tile;
+            join = __hip_atomic_fetch_add(n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)ranges - 1;
+            if (join) __hip_atomic_store(n, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    __syncthreads();
+    if (!join) return;
+    asm volatile("" ::: "memory");
+    for (int i = threadIdx.x; i < 16 * NT * (D / 4); i += 256) {
+        const int r = row0 + i / (D / 4), iq = r / a.group, h = hk * a.group + (r - iq * a.group);
+        if (r < rows) join_ranges<D, true>(a, splits, ranges, s, iq, h, 4 * (i % (D / 4)));
     }
 }
 
@@ -800,35 +896,17 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
         }
 }
 
-// The ranges' joins: thread per four elements of a row
+// The joins of kv_attn_tiles_kernel's ranges: thread per four elements of a row
 template <int D>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, const int splits) {
     constexpr int C4 = D / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, rows = (int64_t)a.c.n_seq * a.n_q * a.heads;
-    const int64_t pr = i / C4;
-    if (pr >= rows) return;
-    const int e = (int)(i - pr * C4) * 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pr = i / C4;
+    if (pr >= (int64_t)a.c.n_seq * a.n_q * a.heads) return;
     const int h = (int)(pr % a.heads), iq = (int)(pr / a.heads % a.n_q), s = (int)(pr / a.heads / a.n_q);
     const KvRange kr = kv_range(a, s);
     if (iq >= kr.nq) return;
-    const int chunk = kv_chunk(kr, splits), n = max((kr.hi - kr.lo + chunk - 1) / chunk, 1);
-    const float* ml = a.part + (int64_t)splits * rows * D + pr * 4;
-    const float* po = a.part + pr * D + e;
-    float m = KV_NONE, p = KV_NONE, l = 0.0f;
-    v4f o = {0, 0, 0, 0};
-    for (int x = 0; x < n; ++x) {
-        m = fmaxf(m, ml[x * rows * 4]);
-        p = fmaxf(p, ml[x * rows * 4 + 1]);
-    }
-    for (int x = 0; x < n; ++x) {
-        l += ml[x * rows * 4 + 2] * __builtin_amdgcn_exp2f(ml[x * rows * 4] - m);
-        o = o + *reinterpret_cast<const v4f*>(po + x * rows * D) * __builtin_amdgcn_exp2f(ml[x * rows * 4 + 1] - p);
-    }
-    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m) / l;
-    o = o * f;
-    char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
-    if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(o, v4h);
-    else *reinterpret_cast<v4f_a4*>(out + 4 * e) = o;
+    const int chunk = kv_chunk(kr, splits);
+    join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), s, iq, h, (int)(i - pr * C4) * 4);
 }
 
 // Row tiles and ranges of the kernel above for n_q queries: enough workgroups to fill the CUs several times
@@ -842,7 +920,8 @@ KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max
     const int64_t wgs = std::max<int64_t>((int64_t)p.tiles * heads_kv * n_seq, 1);
     const int64_t most = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);
     if (p.nt) {
-        p.splits = (int)std::max<int64_t>(std::min<int64_t>({(16LL * std::max(cus, 1) + wgs - 1) / wgs, most, 128}), 1);
+        p.splits = (int)std::max<int64_t>(std::min<int64_t>({(4LL * std::max(cus, 1) + wgs - 1) / wgs, most, 128}), 1);
+        if (wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
     } else {  // two workgroups of 128 rows to a CU: the ranges whose rounds over the CUs take the least time
         const int64_t slots = 2LL * std::max(cus, 1);
         double best = 0.0;
@@ -882,7 +961,7 @@ static hipError_t kv_attn_d(const KvAttnArgs& a, const KvAttnPlan& p, hipStream_
         else tile(std::true_type(), std::true_type());
     } else if (p.nt == 1) go(std::integral_constant<int, 1>());
     else go(std::integral_constant<int, 2>());
-    if (p.splits > 1) {
+    if (p.nt == 0 && p.splits > 1) {
         const int64_t n = (int64_t)a.c.n_seq * a.n_q * a.heads * (D / 4);
         kv_attn_join_kernel<D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a, p.splits);
     }
@@ -893,7 +972,7 @@ hipError_t launch_kv_attn(const KvAttnArgs& a, const KvAttnPlan& p, int D, hipSt
     const int64_t rows = (int64_t)a.n_q * a.heads * a.c.n_seq;
     if (rows <= 0) return hipSuccess;
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
-    if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || rows * (D / 4) > (int64_t)INT32_MAX * 256 || (p.splits > 1 && !a.part))
+    if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || rows * (D / 4) > (int64_t)INT32_MAX * 256 || (p.splits > 1 && (!a.part || (p.nt && !a.arrived))))
         return hipErrorInvalidValue;
     switch (D) {
         case 64: return kv_attn_d<64>(a, p, st);

@@ -342,9 +342,11 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     if (cache->n_blocks == 0) a.c.max_blocks = 0;  // nothing to attend to
     if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
     const KvAttnPlan p = attn_plan(ctx, cache, seqs, q);
-    const mi355_status ws = ensure_ws(ctx, p.bytes);
+    mi355_status ws = p.nt && p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
+    if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes);
     if (ws != MI355_STATUS_SUCCESS) return ws;
     a.part = static_cast<float*>(ctx->ws);
+    a.arrived = static_cast<uint32_t*>(ctx->arrived);
     Timed tm(ctx, "kv_cache_attn");
     return hip_check(ctx, tm.done(launch_kv_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache_attn launch");
 }
