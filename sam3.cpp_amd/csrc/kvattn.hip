@@ -909,28 +909,52 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
     join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), s, iq, h, (int)(i - pr * C4) * 4);
 }
 
-// Row tiles and ranges of the kernel above for n_q queries: enough workgroups to fill the CUs several times
-// over, of at least one step each.
+// The kernel, its row tiles and the ranges of the tokens for n_q queries.
+// Up to 16 rows (decoding) the bytes bound it: four workgroups to a CU in all, but no more ranges than twice the root of
+// the 128-token steps, since one workgroup joins them (28 heads over 19328 tokens: 128 ranges 26 us, 25 of them 17).
+// Beyond, the kernels of 32 and 128 rows are compared at their best number of ranges by the rounds of workgroups
+// over the CUs times a step's time with one and with two workgroups on a CU (tens of nanoseconds): the wide one has
+// 1.7 times the throughput, the narrow one four times the workgroups.
 KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int D, int cus) {
+    const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
+    const int64_t steps = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);  // of 128 tokens
+    cus = std::max(cus, 1);
+    int64_t root = 8;  // (as many as one round of a join's loads)
+    while (root < 128 && root * root < 4 * steps) ++root;
     KvAttnPlan p;
-    const int64_t rows = (int64_t)n_q * (heads / heads_kv);
-    p.nt = rows > 64 ? 0 : rows > 16 ? 2 : 1;
-    const int rt = p.nt ? 16 * p.nt : 128;
-    p.tiles = (int)((rows + rt - 1) / rt);
-    const int64_t wgs = std::max<int64_t>((int64_t)p.tiles * heads_kv * n_seq, 1);
-    const int64_t most = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);
-    if (p.nt) {
-        p.splits = (int)std::max<int64_t>(std::min<int64_t>({(4LL * std::max(cus, 1) + wgs - 1) / wgs, most, 128}), 1);
-        if (wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
-    } else {  // two workgroups of 128 rows to a CU: the ranges whose rounds over the CUs take the least time
-        const int64_t slots = 2LL * std::max(cus, 1);
-        double best = 0.0;
+    if (rows <= 16) {
+        p.nt = 1;
+        p.tiles = 1;
         p.splits = 1;
-        for (int s = 1; s <= 16 && (s == 1 || most >= 4 * s); ++s) {
-            const double t = (double)((wgs * s + slots - 1) / slots) * ((double)most / s + 2.0) + (s > 1 ? 1.0 + 0.02 * s * (double)wgs / slots : 0.0);
+        double best = 0.0;
+        const int64_t most = std::min<int64_t>({(4LL * cus + items - 1) / items, steps, root});
+        for (int s = 1; s <= most; ++s) {
+            const int64_t per = (steps + s - 1) / s;
+            const double load = (double)(items * s) / cus;
+            const double t = (per + 1) * 50.0 * std::max(1.0, 0.7 * load) + (s == 1 ? 0.0 : 130.0 + 10.0 * std::max(s - 8, 0) + 100.0 * load);
             if (s == 1 || t < best) best = t, p.splits = s;
         }
+    } else {
+        double best = 0.0;
+        for (int nt : {2, 0}) {
+            if (nt == 0 && rows <= 64) break;
+            const int64_t wgs = items * ((rows + (nt ? 31 : 127)) / (nt ? 32 : 128));
+            for (int s = 1; s <= std::min<int64_t>(steps, nt ? root : 32); ++s) {
+                const int64_t n = wgs * s, rounds = (n + 2 * cus - 1) / (2 * cus), per = (steps + s - 1) / s;
+                const double step = nt ? (n <= cus ? 90.0 : 230.0) : (n <= cus ? 260.0 : 600.0);
+                const double join = s == 1 ? 0.0 : nt ? 100.0 + 12.0 * s : 450.0 + s * (double)(rows * items * D) / 10000.0;
+                const double t = rounds * (per + 1) * step + join;
+                if ((nt == 2 && s == 1) || t < best) {
+                    best = t;
+                    p.nt = nt;
+                    p.splits = s;
+                }
+            }
+        }
+        const int rt = p.nt ? 16 * p.nt : 128;
+        p.tiles = (int)((rows + rt - 1) / rt);
     }
+    if (p.nt && items * p.tiles > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
     p.bytes = p.splits > 1 ? (size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 : 0;
     return p;
 }
