@@ -366,7 +366,7 @@ mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache
 int mi355_supports_kv_cache_attn(const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                                  const mi355_tensor* dst);
 size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache* cache,
-                                          const mi355_kv_seqs* seqs, const mi355_tensor* q);
+                                          const mi355_kv_seqs* seqs, const mi355_tensor* q, int32_t window);
 mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
                                  const mi355_tensor* q, const int32_t* n_q, float scale, int causal, int32_t window,
                                  const mi355_tensor* dst);

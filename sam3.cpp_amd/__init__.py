@@ -180,7 +180,7 @@ def lib():
         "mi355_kv_cache_write": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, T, P]),
         "mi355_kv_cache_read": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), P, T, T]),
         "mi355_supports_kv_cache_attn": (I, [C.POINTER(KvCache), C.POINTER(KvSeqs), T, T]),
-        "mi355_kv_cache_attn_workspace_size": (SZ, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T]),
+        "mi355_kv_cache_attn_workspace_size": (SZ, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, C.c_int32]),
         "mi355_kv_cache_attn": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, P, F, I, C.c_int32, T]),
         "mi355_vit_workspace_size": (SZ, [C.POINTER(VitHparams)]),
         "mi355_vit_prefix": (I, [P, C.POINTER(VitHparams), P, T, P, P, P, P]),
@@ -487,8 +487,8 @@ class Context:
                       window: int = 0):
         self._check(self.L.mi355_kv_cache_attn(self.h, cache, seqs, q, n_q or None, scale, 1 if causal else 0, window, dst))
 
-    def kv_cache_attn_workspace_size(self, cache: KvCache, seqs: KvSeqs, q: Tensor) -> int:
-        return int(self.L.mi355_kv_cache_attn_workspace_size(self.h, cache, seqs, q))
+    def kv_cache_attn_workspace_size(self, cache: KvCache, seqs: KvSeqs, q: Tensor, window: int = 0) -> int:
+        return int(self.L.mi355_kv_cache_attn_workspace_size(self.h, cache, seqs, q, window))
 
     def reserve_workspace(self, size: int):
         self._check(self.L.mi355_reserve_workspace(self.h, size))

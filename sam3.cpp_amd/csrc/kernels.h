@@ -359,7 +359,7 @@ struct KvAttnPlan {
     int splits;                // ranges of the tokens, joined by a second kernel
     size_t bytes;              // of part
 };
-KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int D, int cus);
+KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);
 hipError_t launch_kv_attn(const KvAttnArgs& a, const KvAttnPlan& p, int D, hipStream_t st);
 
 // ---- SAM3 ViT glue (rows of E contiguous floats)

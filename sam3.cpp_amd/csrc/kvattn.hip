@@ -28,6 +28,7 @@ constexpr float KV_ROOM = 15.0f;     // and their reference moves when one would
 constexpr float KV_LIFT_SUM = 8.0f;  // the same where a lane's sum of 32 of them, and not each, is held below 2^15
 constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
 constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
+constexpr int KV_RANGES = 64;        // ranges of a row that one workgroup joins, at most
 }  // namespace
 
 // The tokens that a sequence's queries can see, and its queries.
@@ -108,23 +109,25 @@ __device__ __forceinline__ float col_sum(float v) {
     return v + lane_swap_f<32>(v);
 }
 
-// Four elements from e on of a row's output, joined from its n ranges' partial sums in the ranges' order and written.
-// ONE: another workgroup of this launch wrote them, through the caches; loads that bypass them read them.
+// A store past the caches of the workgroup's XCD, for a workgroup on another one, and a load of such
+__device__ __forceinline__ v2f get_through(const float* p) {
+    return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void put_through(float* p, v2f v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Four elements from e on of row pr (sequence, query, head in that order), joined from the row's n ranges in the ranges'
+// order and written.  ONE: other workgroups of this launch wrote the partial sums.
 template <int D, bool ONE>
-__device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int n, int s, int iq, int h, int e) {
-    const int64_t rows = (int64_t)a.c.n_seq * a.n_q * a.heads, pr = ((int64_t)s * a.n_q + iq) * a.heads + h;
+__device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int n, int64_t pr, int e) {
+    const int64_t rows = (int64_t)a.c.n_seq * a.n_q * a.heads;
     const float* ml = a.part + (int64_t)splits * rows * D + pr * 4;
     const float* po = a.part + pr * D + e;
-    auto get = [](const float* p) -> v4f {
-        if constexpr (ONE) {
-            const uint64_t* q = reinterpret_cast<const uint64_t*>(p);
-            const uint64_t lo = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const uint64_t hi = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const v2f x = __builtin_bit_cast(v2f, lo), y = __builtin_bit_cast(v2f, hi);
-            return v4f{x[0], x[1], y[0], y[1]};
-        } else {
-            return *reinterpret_cast<const v4f*>(p);
-        }
+    auto get = [](const float* q) {
+        if constexpr (!ONE) return *reinterpret_cast<const v4f*>(q);
+        const v2f lo = get_through(q), hi = get_through(q + 2);
+        return v4f{lo[0], lo[1], hi[0], hi[1]};
     };
     constexpr int B = 8;  // ranges whose loads are on their way together
     float m = KV_NONE, p = KV_NONE, l = 0.0f;
@@ -154,15 +157,11 @@ __device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int
         }
     }
     o = o * (l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m) / l);
-    char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
+    const int64_t h = pr % a.heads, iq = pr / a.heads % a.n_q, s = pr / a.heads / a.n_q;
+    char* out = a.dst + h * a.d_nb[0] + iq * a.d_nb[1] + s * a.d_nb[2];
     if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(o, v4h);
     else *reinterpret_cast<v4f_a4*>(out + 4 * e) = o;
 }
-// A store past the caches of the workgroup's XCD, for a workgroup on another one
-__device__ __forceinline__ void put_through(float* p, v2f v) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 // Few query rows over many tokens.  A row is one query and head of the group that shares a key head: row
 // r of a sequence and key head is query r / group, head r % group.  A workgroup takes 16 NT rows and
 // one range of the tokens, its four wavefronts every fourth step of 32 tokens; nothing passes through
@@ -454,70 +453,155 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
         }
         __syncthreads();
     }
-    if (w == 0) {
+    if (ranges == 1) {
+        if (w != 0) return;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int r = row0 + 16 * t + col, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
             if (r >= rows) continue;
-            p_ref[t] += 9.0f;  // the halves were the bytes' values over 512
-            if (ranges > 1) {
-                const int64_t pr = (((int64_t)sp * c.n_seq + s) * a.n_q + iq) * a.heads + h;
-                float* out = a.part + pr * D;
+            // (2^9: the halves were the bytes' values over 512)
+            const float f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t] + 9.0f) / l_sum[t];
+            char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ar = 4 * g + i;
+            for (int i = 0; i < 4; ++i) {
+                const int ar = 4 * g + i;
+                v4f y[2];
 #pragma unroll
-                    for (int b = 0; b < NB; b += 2) {
-                        const int e = D == 128 ? 8 * ar + b : b < 4 ? 4 * ar + b : 64 + 2 * ar;
-                        put_through(out + e, v2f{O[t][b][i], O[t][b + 1][i]});
-                    }
-                }
-                if (g == 0) {
-                    float* ml = a.part + (int64_t)splits * c.n_seq * a.n_q * a.heads * D + pr * 4;
-                    put_through(ml, v2f{m_ref[t], p_ref[t]});
-                    put_through(ml + 2, v2f{l_sum[t], 0.0f});
-                }
-            } else {
-                const float f = l_sum[t] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p_ref[t] - m_ref[t]) / l_sum[t];
-                char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int ar = 4 * g + i;
-                    v4f y[2];
-#pragma unroll
-                    for (int b = 0; b < 8; ++b) y[b >> 2][b & 3] = b < NB ? O[t][b < NB ? b : 0][i] * f : 0.0f;
-                    const int e = (D == 128 ? 8 : 4) * ar;
-                    if (a.d16) {
-                        *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y[0], v4h);
-                        if (D == 128) *reinterpret_cast<v4h_a2*>(out + 2 * e + 8) = __builtin_convertvector(y[1], v4h);
-                        if (TAIL) *reinterpret_cast<h2v_a2*>(out + 2 * (64 + 2 * ar)) = __builtin_convertvector((v2f{y[1][0], y[1][1]}), h2v);
-                    } else {
-                        *reinterpret_cast<v4f_a4*>(out + 4 * e) = y[0];
-                        if (D == 128) *reinterpret_cast<v4f_a4*>(out + 4 * e + 16) = y[1];
-                        if (TAIL) *reinterpret_cast<v2f_a4*>(out + 4 * (64 + 2 * ar)) = v2f{y[1][0], y[1][1]};
-                    }
+                for (int b = 0; b < 8; ++b) y[b >> 2][b & 3] = b < NB ? O[t][b < NB ? b : 0][i] * f : 0.0f;
+                const int e = (D == 128 ? 8 : 4) * ar;
+                if (a.d16) {
+                    *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y[0], v4h);
+                    if (D == 128) *reinterpret_cast<v4h_a2*>(out + 2 * e + 8) = __builtin_convertvector(y[1], v4h);
+                    if (TAIL) *reinterpret_cast<h2v_a2*>(out + 2 * (64 + 2 * ar)) = __builtin_convertvector((v2f{y[1][0], y[1][1]}), h2v);
+                } else {
+                    *reinterpret_cast<v4f_a4*>(out + 4 * e) = y[0];
+                    if (D == 128) *reinterpret_cast<v4f_a4*>(out + 4 * e + 16) = y[1];
+                    if (TAIL) *reinterpret_cast<v2f_a4*>(out + 4 * (64 + 2 * ar)) = v2f{y[1][0], y[1][1]};
                 }
             }
         }
+        return;
     }
-    if (ranges == 1) return;
+    // One of several ranges: its sums go to memory past the caches, rows whole.
+    auto partial_row = [&](int r) {  // row r of the tile: its number among all
+        const int iq = (row0 + r) / a.group;
+        return row0 + r < rows ? ((int64_t)s * a.n_q + iq) * a.heads + hk * a.group + (row0 + r - iq * a.group) : (int64_t)-1;
+    };
+    if (w == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) so[0][t][b][lane] = O[t][b];
+            const int64_t pr = partial_row(16 * t + col);
+            if (g == 0 && pr >= 0) {
+                const int64_t all = (int64_t)c.n_seq * a.n_q * a.heads;
+                float* ml = a.part + (int64_t)splits * all * D + (sp * all + pr) * 4;
+                put_through(ml, v2f{m_ref[t], p_ref[t] + 9.0f});
+                put_through(ml + 2, v2f{l_sum[t], 0.0f});
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * NT * (D / 2); i += 256) {
+        const int r = i / (D / 2), e = 2 * (i % (D / 2));
+        const int64_t pr = partial_row(r);
+        if (pr < 0) break;
+        const int ar = D == 128 ? e >> 3 : e < 64 ? e >> 2 : (e - 64) >> 1, b = D == 128 ? e & 7 : e < 64 ? e & 3 : 4;
+        const v4f* o = &so[0][r >> 4][b][(r & 15) + 16 * (ar >> 2)];
+        put_through(a.part + ((int64_t)sp * c.n_seq * a.n_q * a.heads + pr) * D + e, v2f{o[0][ar & 3], o[64][ar & 3]});
+    }
     // The workgroup that comes last joins the ranges.  What the others wrote is in memory before they count
     // themselves, and the counter goes back to zero for the next launch.
     __shared__ int join;
-    if (w == 0) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (lane == 0) {
-            uint32_t* n = a.arrived + ((int64_t)s * c.heads + hk) * tiles + tile;
-            join = __hip_atomic_fetch_add(n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)ranges - 1;
-            if (join) __hip_atomic_store(n, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t* n = a.arrived + ((int64_t)s * c.heads + hk) * tiles + tile;
+        join = __hip_atomic_fetch_add(n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)ranges - 1;
+        if (join) __hip_atomic_store(n, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
     if (!join) return;
     asm volatile("" ::: "memory");
-    for (int i = threadIdx.x; i < 16 * NT * (D / 4); i += 256) {
-        const int r = row0 + i / (D / 4), iq = r / a.group, h = hk * a.group + (r - iq * a.group);
-        if (r < rows) join_ranges<D, true>(a, splits, ranges, s, iq, h, 4 * (i % (D / 4)));
+    if constexpr (NT == 1) {  // (few elements: one round of loads more would cost more than the weights' reuse saves)
+        for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+            const int64_t pr = partial_row(i / (D / 4));
+            if (pr >= 0) join_ranges<D, true>(a, splits, ranges, pr, 4 * (i % (D / 4)));
+        }
+        return;
+    }
+    // First each row's weights of its ranges, lanes L to a row, then the rows' elements.
+    constexpr int L = 256 / (16 * NT), MAXN = KV_RANGES;
+    __shared__ float weight[16 * NT][MAXN];
+    const int64_t all = (int64_t)c.n_seq * a.n_q * a.heads;
+    {
+        const int r = threadIdx.x / L, x0 = threadIdx.x % L;
+        const int64_t pr = partial_row(r);
+        const float* ml = a.part + (int64_t)splits * all * D + max(pr, (int64_t)0) * 4;
+        v2f mp[MAXN / L];
+        float l[MAXN / L], m = KV_NONE, p = KV_NONE, sum = 0.0f;
+#pragma unroll
+        for (int x = 0; x < MAXN / L; ++x) {
+            mp[x] = v2f{KV_NONE, KV_NONE};
+            l[x] = 0.0f;
+            if (pr >= 0 && x0 + L * x < ranges) {
+                mp[x] = get_through(ml + (x0 + L * x) * all * 4);
+                l[x] = get_through(ml + (x0 + L * x) * all * 4 + 2)[0];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < MAXN / L; ++x) m = fmaxf(m, mp[x][0]), p = fmaxf(p, mp[x][1]);
+        m = group_max<L>(m);
+        p = group_max<L>(p);
+        // (the lanes' sums meet in a fixed order)
+#pragma unroll
+        for (int x = 0; x < MAXN / L; ++x) sum += l[x] * __builtin_amdgcn_exp2f(mp[x][0] - m);
+        sum = group_sum<L>(sum);
+        const float f = sum == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(p - m) / sum;
+#pragma unroll
+        for (int x = 0; x < MAXN / L; ++x)
+            if (x0 + L * x < ranges) weight[r][x0 + L * x] = __builtin_amdgcn_exp2f(mp[x][1] - p) * f;
+    }
+    __syncthreads();
+    constexpr int K = NT * D / 64, B = 4;  // pieces of a thread, ranges whose loads are on their way together
+    int64_t place[K];
+    int row[K];
+    v4f o[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int i = threadIdx.x + 256 * k;
+        row[k] = i / (D / 4);
+        const int64_t pr = i < 16 * NT * (D / 4) ? partial_row(row[k]) : -1;
+        place[k] = pr < 0 ? -1 : pr * D + 4 * (i % (D / 4));
+        o[k] = v4f{0, 0, 0, 0};
+    }
+    for (int x0 = 0; x0 < ranges; x0 += B) {
+        v2f y[K][B][2];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int x = 0; x < B; ++x) {
+                y[k][x][0] = y[k][x][1] = v2f{0, 0};
+                if (place[k] >= 0 && x0 + x < ranges) {
+                    y[k][x][0] = get_through(a.part + (x0 + x) * all * D + place[k]);
+                    y[k][x][1] = get_through(a.part + (x0 + x) * all * D + place[k] + 2);
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int x = 0; x < B; ++x) {
+                const float f = place[k] >= 0 && x0 + x < ranges ? weight[row[k]][x0 + x] : 0.0f;
+                o[k] = o[k] + v4f{y[k][x][0][0], y[k][x][0][1], y[k][x][1][0], y[k][x][1][1]} * f;
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (place[k] < 0) continue;
+        const int r = row0 + row[k], iq = r / a.group, h = hk * a.group + (r - iq * a.group), e = 4 * ((threadIdx.x + 256 * k) % (D / 4));
+        char* out = a.dst + (int64_t)h * a.d_nb[0] + (int64_t)iq * a.d_nb[1] + (int64_t)s * a.d_nb[2];
+        if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(o[k], v4h);
+        else *reinterpret_cast<v4f_a4*>(out + 4 * e) = o[k];
     }
 }
 
@@ -531,6 +615,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 template <int D, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
+    constexpr bool AHEAD = !((QS && D > 64) || (PS && D > 96));  // scores a tile ahead; else the second halves have their registers
     constexpr int UB = D == 96 ? 8 : 16;            // bytes of a staging unit
     constexpr int UR = D / UB, NU = 16 * UR / 64;   // units of a row, units of a thread
     __shared__ __attribute__((aligned(16))) _Float16 sK[2][64 * D];
@@ -700,34 +785,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
         for (int j = 0; j < 4; ++j) ls = __builtin_fmaf(sums.s[j], read_lane(cur.rv, 4 * (tile & 15) + j), ls);
         return ls * back;
     };
-    // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
-    // a product's fragments are read while the product before multiplies, and pairs go between the products.
-    auto score_softmax = [&](const _Float16* lds, v16f* Sn, const v16f* S, int tile) {
-        int pre = kpre;
-        asm volatile("" : "+v"(pre));  // (the addresses are made here: kept over the loop, they would push the queries out)
-        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        v8h k8[2], k8n[2];
-        auto frag = [&](int m, v8h* o) {
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) o[kh] = key_frag(lds, pre, m, kh);
-        };
-        frag(0, k8);
-        Sn[0] = Sn[1] = z;
-        Sums sums;
-#pragma unroll
-        for (int m = 0; m < NC; ++m) {
-            if (m + 1 < NC) frag(m + 1, k8n);
-#pragma unroll
-            for (int kh = 0; kh < 2; ++kh) {
-                Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], q[m], Sn[kh], 0, 0, 0);
-                if constexpr (QS) Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], ql[m], Sn[kh], 0, 0, 0);
-            }
-#pragma unroll
-            for (int n = 16 * m / NC; n < 16 * (m + 1) / NC; ++n) pair(S, tile, n, sums);
-            k8[0] = k8n[0];
-            k8[1] = k8n[1];
-            __builtin_amdgcn_sched_barrier(0);
-        }
+    // What is left when a tile's pairs are done: the sums, and the references where they have to move.
+    auto settle = [&](const v16f* S, int tile, Sums& sums) {
         const float all = (sums.s[0] + sums.s[1]) + (sums.s[2] + sums.s[3]);
         float ls = add_up(sums, tile);
         const uint32_t far = (uint32_t)(far_groups >> (4 * (tile & 15))) & 15;
@@ -766,6 +825,36 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
                 }
         }
         l_sum += ls;
+    };
+    // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
+    // a product's fragments are read while the product before multiplies, and pairs go between the products.
+    auto score_softmax = [&](const _Float16* lds, v16f* Sn, const v16f* S, int tile) {
+        int pre = kpre;
+        asm volatile("" : "+v"(pre));  // (the addresses are made here: kept over the loop, they would push the queries out)
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        v8h k8[2], k8n[2];
+        auto frag = [&](int m, v8h* o) {
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) o[kh] = key_frag(lds, pre, m, kh);
+        };
+        frag(0, k8);
+        Sn[0] = Sn[1] = z;
+        Sums sums;
+#pragma unroll
+        for (int m = 0; m < NC; ++m) {
+            if (m + 1 < NC) frag(m + 1, k8n);
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], q[m], Sn[kh], 0, 0, 0);
+                if constexpr (QS) Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], ql[m], Sn[kh], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 16 * m / NC; n < 16 * (m + 1) / NC; ++n) pair(S, tile, n, sums);
+            k8[0] = k8n[0];
+            k8[1] = k8n[1];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        settle(S, tile, sums);
     };
     // What the sixteen tiles of cur have that is out of the ordinary.  Scores of blocks that are not there
     // are hidden, and so are those that a row does not see, before anything is made of them; where a
@@ -833,8 +922,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
 
     const int nt = te > tb ? (te - tb + 63) / 64 : 0;
     if (nt > 0) {
-        // Step t: the scores of tile t + 1 beside the softmax of tile t, and its output; then the bytes of K(t + 2) and
-        // V(t + 1), loaded a step before, become halves in the buffers that step t - 1 read last.  One barrier a step.
+        // Step t: the scores of tile t + 1 beside the softmax of tile t (AHEAD; else its own before it), and its
+        // output; then the bytes of K(t + 2) (t + 1) and V(t + 1), loaded a step before, become halves in the buffers
+        // that step t - 1 read last.  One barrier a step.
         cur.id = group_block(a, table, group_of(0));
         nxt.id = group_block(a, table, group_of(16));
         group_scales(a, hk, sc, cur);
@@ -845,11 +935,13 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
         load_one(c.v, vreg, 0);
         store_one(sV[0], vreg, vst);
         load_one(c.k, kreg, 1);
-        store_one(sK[1], kreg, kst);
-        load_one(c.k, kreg, 2);
+        if constexpr (AHEAD) {
+            store_one(sK[1], kreg, kst);
+            load_one(c.k, kreg, 2);
+        }
         load_one(c.v, vreg, 1);
         __syncthreads();
-        score(sK[0], SA);
+        if constexpr (AHEAD) score(sK[0], SA);
         auto step = [&](int t, int cb, v16f* Sc, v16f* Sn) {
             const int t0 = tb + 64 * t;
             lds_barrier();
@@ -860,15 +952,23 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
                 nxt.id = group_block(a, table, group_of(t + 16));
             }
             if ((t & 15) == 8) group_scales(a, hk, sc, nxt);
+            if constexpr (!AHEAD) score(sK[cb], Sc);
             if (t0 < all_lo || t0 + 64 > all_hi || (((hide_groups | nan_groups) >> (4 * (t & 15))) & 15)) hide(Sc, t);
-            score_softmax(sK[cb ^ 1], Sn, Sc, t);
-            output_store(sV[cb], sV[cb ^ 1], sK[cb]);
+            if constexpr (AHEAD) {
+                score_softmax(sK[cb ^ 1], Sn, Sc, t);
+            } else {
+                Sums sums;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) pair(Sc, t, n, sums);
+                settle(Sc, t, sums);
+            }
+            output_store(sV[cb], sV[cb ^ 1], sK[AHEAD ? cb : cb ^ 1]);
             load_one(c.v, vreg, t + 2);
-            load_one(c.k, kreg, t + 3);
+            load_one(c.k, kreg, t + (AHEAD ? 3 : 2));
         };
         for (int t = 0; t < nt; t += 2) {
-            step(t, 0, SA, SB);
-            if (t + 1 < nt) step(t + 1, 1, SB, SA);
+            step(t, 0, SA, AHEAD ? SB : SA);
+            if (t + 1 < nt) step(t + 1, 1, AHEAD ? SB : SA, SA);
         }
     }
 
@@ -902,25 +1002,25 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
     constexpr int C4 = D / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pr = i / C4;
     if (pr >= (int64_t)a.c.n_seq * a.n_q * a.heads) return;
-    const int h = (int)(pr % a.heads), iq = (int)(pr / a.heads % a.n_q), s = (int)(pr / a.heads / a.n_q);
-    const KvRange kr = kv_range(a, s);
-    if (iq >= kr.nq) return;
+    const KvRange kr = kv_range(a, (int)(pr / a.heads / a.n_q));
+    if (pr / a.heads % a.n_q >= kr.nq) return;
     const int chunk = kv_chunk(kr, splits);
-    join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), s, iq, h, (int)(i - pr * C4) * 4);
+    join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), pr, (int)(i - pr * C4) * 4);
 }
 
 // The kernel, its row tiles and the ranges of the tokens for n_q queries.
 // Up to 16 rows (decoding) the bytes bound it: four workgroups to a CU in all, but no more ranges than twice the root of
 // the 128-token steps, since one workgroup joins them (28 heads over 19328 tokens: 128 ranges 26 us, 25 of them 17).
 // Beyond, the kernels of 32 and 128 rows are compared at their best number of ranges by the rounds of workgroups
-// over the CUs times a step's time with one and with two workgroups on a CU (tens of nanoseconds): the wide one has
-// 1.7 times the throughput, the narrow one four times the workgroups.
-KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int D, int cus) {
+// over the CUs times a step's time (tens of nanoseconds, heads of 128) with one and with two workgroups on a CU: the
+// wide one has 1.7 times the throughput (F32 queries: 1.25), the narrow one four times the workgroups.
+KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus) {
+    if (window > 0) max_tokens = std::min<int64_t>(max_tokens, (int64_t)window + n_q + KV_STEP);  // (kv_range)
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
     const int64_t steps = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);  // of 128 tokens
     cus = std::max(cus, 1);
     int64_t root = 8;  // (as many as one round of a join's loads)
-    while (root < 128 && root * root < 4 * steps) ++root;
+    while (root < KV_RANGES && root * root < 4 * steps) ++root;
     KvAttnPlan p;
     if (rows <= 16) {
         p.nt = 1;
@@ -941,9 +1041,10 @@ KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max
             const int64_t wgs = items * ((rows + (nt ? 31 : 127)) / (nt ? 32 : 128));
             for (int s = 1; s <= std::min<int64_t>(steps, nt ? root : 32); ++s) {
                 const int64_t n = wgs * s, rounds = (n + 2 * cus - 1) / (2 * cus), per = (steps + s - 1) / s;
-                const double step = nt ? (n <= cus ? 90.0 : 230.0) : (n <= cus ? 260.0 : 600.0);
-                const double join = s == 1 ? 0.0 : nt ? 100.0 + 12.0 * s : 450.0 + s * (double)(rows * items * D) / 10000.0;
-                const double t = rounds * (per + 1) * step + join;
+                const double step = nt ? (n <= cus ? (q16 ? 155.0 : 185.0) : (q16 ? 165.0 : 200.0))
+                                       : (n <= cus ? (q16 ? 275.0 : 375.0) : (q16 ? 385.0 : 610.0));
+                const double join = s == 1 ? 0.0 : nt ? 480.0 + 50.0 * s : 450.0 + s * (double)(rows * items * D) / 10000.0;
+                const double t = rounds * (per * step + 250.0) + join;
                 if ((nt == 2 && s == 1) || t < best) {
                     best = t;
                     p.nt = nt;

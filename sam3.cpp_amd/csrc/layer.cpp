@@ -202,9 +202,10 @@ mi355_status check_attn(mi355_context* ctx, const mi355_kv_cache* c, const mi355
     return MI355_STATUS_SUCCESS;
 }
 
-KvAttnPlan attn_plan(const mi355_context* ctx, const mi355_kv_cache* c, const mi355_kv_seqs* s, const mi355_tensor* q) {
-    return kv_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, c->head_dim,
-                        ctx->cus);
+KvAttnPlan attn_plan(const mi355_context* ctx, const mi355_kv_cache* c, const mi355_kv_seqs* s, const mi355_tensor* q,
+                     int window) {
+    return kv_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, window, c->head_dim,
+                        q->type == T_F16, ctx->cus);
 }
 
 }  // namespace
@@ -313,9 +314,9 @@ int mi355_supports_kv_cache_attn(const mi355_kv_cache* cache, const mi355_kv_seq
 }
 
 size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
-                                          const mi355_tensor* q) {
+                                          const mi355_tensor* q, int32_t window) {
     if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
-    return attn_plan(ctx, cache, seqs, q).bytes;
+    return attn_plan(ctx, cache, seqs, q, window).bytes;
 }
 
 mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
@@ -341,7 +342,7 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     a.q16 = q->type == T_F16; a.d16 = dst->type == T_F16;
     if (cache->n_blocks == 0) a.c.max_blocks = 0;  // nothing to attend to
     if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
-    const KvAttnPlan p = attn_plan(ctx, cache, seqs, q);
+    const KvAttnPlan p = attn_plan(ctx, cache, seqs, q, a.window);
     mi355_status ws = p.nt && p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
     if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes);
     if (ws != MI355_STATUS_SUCCESS) return ws;
