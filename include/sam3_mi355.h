@@ -330,7 +330,8 @@ typedef struct mi355_kv_seqs {
 /* Writes the last n_new[s] tokens of every sequence s (device int32; NULL: all
  * n_tokens): row i of k and v [head_dim, n_tokens, n_head_kv, n_seq] (F32 or
  * F16, the same type, rows contiguous, any other strides) becomes token
- * n_kv[s] - n_new[s] + i; rows from n_new[s] on are not read.  Per block and
+ * n_kv[s] - n_new[s] + i (none before token 0); rows from n_new[s] on are not
+ * read.  Per block and
  * head, with top the largest magnitude among its new elements:
  *   scale = top / 127, or max(scale, top / 127) where the block keeps tokens
  *           before the first new one;
@@ -354,7 +355,8 @@ mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache
  * h / (n_head / n_head_kv)).  Sequence s has n_q[s] queries (device int32; NULL: all
  * n_q); rows of dst from n_q[s] on are left as they are.  Query i stands at position
  * p = n_kv[s] - n_q[s] + i and attends to tokens t < n_kv[s], with causal t <= p,
- * and with window > 0 t > p - window; a query that attends to nothing gives zeros.
+ * and with window > 0 t > p - window; a query that attends to nothing gives zeros,
+ * one that sees a token of a block whose scales are not both finite gives NaN.
  * Scores, softmax and outputs accumulate in fp32.  An F16 q enters the matrix
  * products as it is and an F32 q as two halves (22 bits); the probabilities enter
  * as F16 for an F16 dst and as two halves for an F32 dst; the cache's bytes

@@ -783,7 +783,7 @@ mi355_status mi355_synchronize(mi355_context* ctx) {
 mi355_status mi355_reserve_workspace(mi355_context* ctx, size_t bytes) {
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "reserve_workspace: null context");
     (void)hipSetDevice(ctx->device);
-    const mi355_status st = bytes ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
+    const mi355_status st = bytes && !capturing(ctx) ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
     return st != MI355_STATUS_SUCCESS ? st : ensure_ws(ctx, bytes);
 }
 

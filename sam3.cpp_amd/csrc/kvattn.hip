@@ -71,7 +71,8 @@ __device__ __forceinline__ int group_block(const KvAttnArgs& a, const int* table
 __device__ __forceinline__ void group_scales(const KvAttnArgs& a, int hk, float sc, KvGroups& x) {
     const int64_t at = (int64_t)max(x.id, 0) * a.c.heads + hk;
     const float ks = a.c.k_scale[at], vs = a.c.v_scale[at];
-    x.f = x.id >= 0 ? ks * sc : 0.0f;
+    const bool finite = fabsf(ks) < __builtin_inff() && fabsf(vs) < __builtin_inff();
+    x.f = x.id < 0 ? 0.0f : finite ? ks * sc : __builtin_nanf("");  // (a score that is seen is then NaN)
     x.lv = x.id >= 0 ? scale_log2(vs) : 0.0f;
     x.rv = 1.0f / vs;
 }

@@ -87,16 +87,23 @@ bool rope_table(const mi355_rope_params* p, RopeArgs* a) {
     }
     if (total != n || (p->order == MI355_ROPE_INTERLEAVED && p->sections[3] != 0)) return false;
     // freq_base ^ (-2^k / size) by squaring, of one size or each axis's: a power is a product of at most seven.
-    // 64-bit mantissas and a relative 2^-57 at most leave an int32 position's angle good to 2^-32 of a turn.
+    // 64-bit mantissas and a relative 2^-57 at most leave an int32 position's angle good to 2^-32 of a turn; the
+    // products below one are made in 64-bit fixed point (eight truncations: 2^-61 of a turn, 2^-30 at such a position),
+    // a tenth of the time of the floating ones.
     long double root[4][7];
+    uint64_t fixed[4][7];
+    const long double unit = (long double)p->freq_scale / 6.283185307179586476925286766559L, two64 = 18446744073709551616.0L;
+    bool below = unit >= 0.0L && unit < 1.0L;
     if (a)
         for (int s = 0; s < (p->restart ? 4 : 1); ++s) {
             const int size = p->restart ? p->sections[s] : n;
             if (size == 0) continue;
             root[s][0] = powl((long double)p->freq_base, -1.0L / (long double)size);
             for (int k = 1; k < 7; ++k) root[s][k] = root[s][k - 1] * root[s][k - 1];
+            below = below && root[s][0] < 1.0L;
+            for (int k = 0; below && k < 7; ++k) fixed[s][k] = (uint64_t)(root[s][k] * two64);
         }
-    const long double unit = (long double)p->freq_scale / 6.283185307179586476925286766559L;
+    const uint64_t unit64 = below ? (uint64_t)(unit * two64) : 0;
     int count[4] = {0, 0, 0, 0}, axis = 0;
     for (int i = 0; i < n; ++i) {
         if (p->order == MI355_ROPE_INTERLEAVED) {
@@ -108,11 +115,18 @@ bool rope_table(const mi355_rope_params* p, RopeArgs* a) {
         const int e = p->restart ? count[axis] : i;
         ++count[axis];
         if (!a) continue;
-        long double f = unit;
-        for (int k = 0; k < 7; ++k)
-            if (e >> k & 1) f *= root[p->restart ? axis : 0][k];
-        if (!(f >= 0.0L && f < 1.0L)) f -= floorl(f);
-        const uint64_t turn = f < 1.0L ? (uint64_t)(f * 18446744073709551616.0L) : 0;
+        const int s = p->restart ? axis : 0;
+        uint64_t turn = unit64;
+        if (below) {
+            for (int k = 0, b = e; b; ++k, b >>= 1)
+                if (b & 1) turn = (uint64_t)(((unsigned __int128)turn * fixed[s][k]) >> 64);
+        } else {
+            long double f = unit;
+            for (int k = 0; k < 7; ++k)
+                if (e >> k & 1) f *= root[s][k];
+            f -= floorl(f);
+            turn = f < 1.0L ? (uint64_t)(f * two64) : 0;
+        }
         a->turn[i] = p->inverse ? 0 - turn : turn;
         a->axis[i] = (uint8_t)axis;
     }
@@ -148,7 +162,7 @@ mi355_status check_cache(mi355_context* ctx, const char* op, const mi355_kv_cach
         ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) | reinterpret_cast<uintptr_t>(s->table) |
           reinterpret_cast<uintptr_t>(s->n_kv)) & 3))
         return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: the cache must be 16-byte aligned, scales, table and lengths 4-byte", op);
-    if (c->n_head_kv > 65535 || s->n_seq > 65535 || (int64_t)s->max_blocks * c->block_tokens > INT_MAX - 4096)
+    if (c->n_head_kv > 65535 || s->n_seq > 65535 || (int64_t)s->max_blocks * c->block_tokens > 1 << 30)
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: sizes beyond the launch limits", op);
     return MI355_STATUS_SUCCESS;
 }

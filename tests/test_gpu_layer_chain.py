@@ -1,12 +1,10 @@
 """A layer's operators in a run, as a decoder over quantized weights uses them: a prompt, then token by token,
 eagerly and as a replayed graph, each stage against float64 of what the stage before left."""
-import math
-
 import pytest
 import torch
 
 import layer_refs as R
-from layer_refs import F64, H, U, tensor
+from layer_refs import F64, U, tensor
 
 pytestmark = pytest.mark.gpu
 E, NH, KV, D, BT, S, PER = 256, 4, 2, 64, 16, 3, 6
@@ -175,6 +173,42 @@ def test_layer_as_a_graph(mi):
         ctx.close()
 
 
+def test_capture_needs_its_workspace(mi):
+    """A captured call whose ranges need workspace that the context lacks is refused, with the way out, and the capture goes
+    on; after mi355_reserve_workspace it is taken, and replays survive the workspace's replacement."""
+    stream = torch.cuda.Stream()
+    ctx = mi.Context(0, stream.cuda_stream)
+    try:
+        with torch.cuda.stream(stream):
+            d = R.Cache(1, 200, 1, 64, 64, seed=8).fill([12800]).on_gpu(mi)
+            q, out, mark = torch.randn((1, 4, 1, 64), device="cuda"), torch.zeros((1, 1, 4, 64), device="cuda"), torch.zeros(8, device="cuda")
+            need = ctx.kv_cache_attn_workspace_size(d["cache"], d["seqs"], tensor(mi, q))
+            assert need > 0
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                mark.add_(1)
+                with pytest.raises(mi.Mi355Error, match="mi355_reserve_workspace"):
+                    ctx.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, q), tensor(mi, out), 0.125)
+            graph.replay()
+            stream.synchronize()
+            assert (mark == 1).all() and not out.any()
+            ctx.reserve_workspace(need)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                ctx.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, q), tensor(mi, out), 0.125)
+            eager = torch.zeros_like(out)
+            ctx.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, q), tensor(mi, eager), 0.125)
+            for i in range(4):
+                out.zero_()
+                graph.replay()
+                stream.synchronize()
+                assert eager.any() and torch.equal(out, eager), i
+                ctx.reserve_workspace(need + (i << 22))
+    finally:
+        ctx.close()
+
+
 def test_two_contexts_at_once(mi):
     """Two streams with a context each, launched together."""
     streams = [torch.cuda.Stream() for _ in range(2)]
@@ -198,4 +232,3 @@ def test_two_contexts_at_once(mi):
     finally:
         for x in ctxs:
             x.close()
-    assert math.isfinite(H)

@@ -238,6 +238,23 @@ def test_rope_multi(mi, ctx, case, dtype):
         assert torch.equal(dst, same) and torch.equal(dst, wide[..., :D]) and (wide[..., D:] == 9).all()
 
 
+@pytest.mark.parametrize("base,scale", [(10000.0, 10.0), (10000.0, -0.5), (1.0, 0.3), (0.25, 1.0), (5e5, 0.0)])
+def test_rope_multi_other_frequencies(mi, ctx, base, scale):
+    """Turns of one and more a position, backwards, the same for every pair, growing with the pair, and none."""
+    x = rnd(33, 1, 9, 2, 64)
+    pos = torch.arange(-4, 5, dtype=torch.int32, device="cuda").reshape(1, 1, 9) * 1000003
+    out = torch.empty_like(x)
+    ctx.rope_multi(tensor(mi, x), pos.data_ptr(), mi.rope_params(64, [32], base, pairs=1, freq_scale=scale), tensor(mi, out))
+    ctx.synchronize()
+    # the float32 parameters as they are, and float64's own rounding of far angles
+    f32 = lambda v: float(torch.tensor(v, dtype=F32))  # noqa: E731
+    ang = R.angles(pos, [32], 64, f32(base), scale=f32(scale))
+    both = x.abs().to(F64)
+    both = both + both.roll(32, -1)
+    far = torch.cat([ang, ang], -1).abs()[:, :, None] * 2.0 ** -51
+    assert ((out.to(F64) - R.rope(x, ang, True)).abs() <= (6 * U + far) * both).all()
+
+
 def test_rope_multi_is_the_image_encoders(mi, ctx):
     """Two axes with restart turn as the encoder's own table pass does (adjacent pairs, x first), to the table's rounding."""
     side, NH, hd = 6, 2, 64
@@ -484,6 +501,65 @@ def test_attn_odd_caches(mi, ctx, nq):
     for qt, ot in ((F16, F32), (F32, F32)):
         q = (torch.randn((4, nq, 4, D), generator=torch.Generator().manual_seed(8)) * 3).to(qt)
         check_attn(mi, ctx, c, q, [nq] * 4, 0.5, nq > 1, 0, ot)
+
+
+@pytest.mark.parametrize("nq", [16, 60, 300])
+@pytest.mark.parametrize("qt,ot", TYPES[:2], ids=["hh", "ff"])
+def test_attn_hides_what_is_not_finite(mi, ctx, nq, qt, ot):
+    """A block spoilt by a NaN or an infinity reaches only the queries that see its tokens: none of those before it
+    (causal), behind it (window) or of the other key head."""
+    D, bt, n = 64, 16, 310
+    for window, (ks, vs) in ((0, (math.nan, 1.0)), (40, (math.inf, math.nan)), (40, (1.0, math.inf))):
+        c = R.Cache(1, 20, 2, bt, D, seed=11).fill([n])
+        q = torch.randn((1, nq, 4, D), generator=torch.Generator().manual_seed(12)).to(qt)
+        block = 18  # tokens 288 .. 303
+        want, tol = c.attn(q, [nq], 0.125, True, window, qt == F32, ot == F32)
+        i = int(c.table[0, block])
+        c.ks[i, 1], c.vs[i, 1] = ks, vs
+        d = c.on_gpu(mi)
+        out = torch.full((1, nq, 4, D), 7.0, dtype=ot, device="cuda")
+        qd = q.cuda()
+        ctx.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, qd.transpose(1, 2)), tensor(mi, out), 0.125, causal=True, window=window)
+        ctx.synchronize()
+        p = n - nq + torch.arange(nq)
+        sees = p >= block * bt
+        if window:
+            sees &= p - window < block * bt + bt - 1
+        got = out.cpu().to(F64)
+        assert got[0, sees, 2:].isnan().any(-1).all() or not math.isnan(ks * vs)
+        ok = torch.ones((nq, 4), dtype=torch.bool)
+        ok[sees, 2:] = False
+        assert ((got - want).abs() <= tol)[0, ok].all()
+
+
+def test_far_blocks(mi, ctx):
+    """A cache of more than 4 GiB: blocks at its end are written, read and attended to."""
+    D, bt, heads = 128, 64, 8
+    n = (1 << 32) // (bt * heads * D) + 700
+    k, v = (torch.empty((n, heads, bt, D), dtype=torch.uint8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty((n, heads), device="cuda") for _ in range(2))
+    table = torch.tensor([[n - 1, 3, n - 2], [n - 600, n - 3, 0]], dtype=torch.int32, device="cuda")
+    n_kv = torch.tensor([150, 190], dtype=torch.int32, device="cuda")
+    cache, seqs = mi.kv_cache(k, v, ks, vs), mi.kv_seqs(table, n_kv)
+    x = rnd(50, 2, heads, 190, D)
+    new = n_kv.clone()
+    ctx.kv_cache_write(cache, seqs, tensor(mi, x), tensor(mi, -x), n_new=new.data_ptr())
+    kb, vb = torch.zeros_like(x), torch.zeros_like(x)
+    ctx.kv_cache_read(cache, seqs, tensor(mi, kb), tensor(mi, vb))
+    small = R.Cache(2, 3, heads, bt, D, extra=0)
+    small.table = torch.arange(6, dtype=torch.int32).reshape(2, 3)
+    small.n_kv = n_kv.cpu()
+    small.write(x.cpu(), -x.cpu(), [150, 190])
+    for nq in (1, 100):
+        q = rnd(51, 2, nq, heads, D)
+        out = torch.empty((2, nq, heads, D), device="cuda")
+        ctx.kv_cache_attn(cache, seqs, tensor(mi, q.transpose(1, 2)), tensor(mi, out), 0.09)
+        ctx.synchronize()
+        want, tol = small.attn(q.cpu(), [nq, nq], 0.09, True, 0, True, True)
+        assert ((out.cpu().to(F64) - want).abs() <= tol).all()
+    for s, m in enumerate((150, 190)):
+        assert torch.equal(kb[s, :, :m].cpu().to(F64), small.values(s, "k")[0].float().to(F64)) and torch.equal(vb[s, :, :m], -kb[s, :, :m])
+        assert not kb[s, :, m:].any()
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
