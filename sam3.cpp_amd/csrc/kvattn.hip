@@ -179,6 +179,10 @@ __device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int
 // that factor passes 2^90 (scales far below the others', and zero) the sum is taken of 2^(s - m) itself.
 // QS: an F32 q enters as two halves of 11 bits, scaled by a power of two that brings the row's largest
 // magnitude to about one.  PS: for an F32 output the probabilities enter as two halves too.
+//
+// With many conversations the cache's bytes bound it: 32 of 16384 tokens, 32 heads of 128 over 8 key heads, 815 MB in
+// 152.5 us (5.3 TB/s).  With few tokens the chain of latencies does: table, block, scales, then the last workgroup's
+// join (777 tokens, 16 heads of 64 over 2: 7.0 us).
 template <int D, int NT, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int KC = D / 64, KM = D / 32, NB = D / 16;  // key chunks of 64, score products, output blocks
@@ -613,6 +617,13 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 // probabilities' registers as the operand of O^T += V^T P^T, V^T by transposing reads); the tile's scores
 // are computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.  A lane's
 // eight scores (kh, hh) belong to 16 tokens of one block: scales and validity are uniform over them.
+//
+// Bounded by the VALU's work of a score (scale, exponential, sum, conversion: about 10 cycles of a SIMD for each score of
+// 64 lanes) and the LDS reads beside the matrix products: at 4096 causal F16 queries twice, 32 heads of 128 over 8 key
+// heads, 388 us or 814 TFLOP/s, the matrix pipe is busy 36 % of the time, the VALU 55 %, the LDS 52 % (bank conflicts
+// 9 %).  F32 queries and probabilities as two halves cost three more products of four: 5184 queries over 15552 tokens,
+// 8 heads of 64, 353 us for 165 GFLOP as the formula counts them.  Eight items at a time: 388 us; sixteen or thirty-two
+// 466, one 482, the shortest row tiles first 497.
 template <int D, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
@@ -838,6 +849,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
 #pragma unroll
             for (int kh = 0; kh < 2; ++kh) o[kh] = key_frag(lds, pre, m, kh);
         };
+        // With F32 queries' two products to a fragment a wavefront here goes before the other one of its SIMD, which
+        // then has its output's reads and stores beside them (5184 queries over 15552 tokens 353 us, 371 without); with
+        // one product it does not pay (4096 F16 queries twice 394 us, 388 without).
+        if constexpr (QS) __builtin_amdgcn_s_setprio(1);
         frag(0, k8);
         Sn[0] = Sn[1] = z;
         Sums sums;
@@ -855,6 +870,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             k8[1] = k8n[1];
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (QS) __builtin_amdgcn_s_setprio(0);
         settle(S, tile, sums);
     };
     // What the sixteen tiles of cur have that is out of the ordinary.  Scores of blocks that are not there
@@ -1010,8 +1026,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
 }
 
 // The kernel, its row tiles and the ranges of the tokens for n_q queries.
-// Up to 16 rows (decoding) the bytes bound it: four workgroups to a CU in all, but no more ranges than twice the root of
-// the 128-token steps, since one workgroup joins them (28 heads over 19328 tokens: 128 ranges 26 us, 25 of them 17).
+// Up to 16 rows (decoding) the number of ranges is the cheapest of: steps of 128 tokens of a range at 0.5 us, or 0.35 us
+// for each workgroup of a CU where there are more than that; and, from two ranges on, the join's 1.3 us (more past the
+// eight ranges of one round of its loads) and 1 us for each workgroup of a CU, which all write partial sums.  Four
+// workgroups to a CU at most, and no more ranges than twice the root of the steps, since one workgroup joins them.
+// 32 conversations of 16384 tokens, 8 key heads: two ranges 153 us, four 164, sixteen 189; one of 19328 tokens with 28
+// heads: 16 us, and 26 with 128 ranges.
 // Beyond, the kernels of 32 and 128 rows are compared at their best number of ranges by the rounds of workgroups
 // over the CUs times a step's time (tens of nanoseconds, heads of 128) with one and with two workgroups on a CU: the
 // wide one has 1.7 times the throughput (F32 queries: 1.25), the narrow one four times the workgroups.
