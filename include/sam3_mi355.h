@@ -142,7 +142,7 @@ mi355_status mi355_tensor_memset(mi355_context* ctx, const mi355_tensor* t, uint
  * src1: F32 (any strides) or, with F16 src0, F16.  dst: F32, nb[0] = 4.
  * src1 may also hold the rows already quantized (mi355_rms_norm,
  * mi355_quantize_rows): Q8_0 with Q8_0 / Q4_0 weights, Q8_1 with Q4_1 ones, in
- * 2-D products; the same bits as with the F32 rows they were made of.
+ * 2-D products; the same bits as with the finite F32 rows they were made of.
  * Q8_0/Q4_0 quantize src1 to Q8_0 and Q4_1 to Q8_1 (x86 variant) exactly as
  * ggml-cpu's from_float, then combine exact int32 block dots in fp32.  F16
  * converts src1 to F16 (round to nearest even) and accumulates in fp32. */
@@ -253,7 +253,8 @@ mi355_status mi355_flash_attn_ext(mi355_context* ctx, const mi355_tensor* q, con
  * pass over the rows: h = x + add (add NULL: h = x), sum = h (sum NULL: not
  * kept), dst = h / sqrt(mean(h^2) + eps) * w (w device F32 [ne0], NULL: no
  * weight).  x, add and sum: F32 or F16, the same type and ne; dst: F32, F16,
- * Q8_0 or Q8_1 (the x86 from_float, as MUL_MAT quantizes src1), the same ne.
+ * Q8_0 or Q8_1 (the x86 from_float, bit for bit mi355_quantize_rows of the F32
+ * dst; a row with a NaN has NaN scales), the same ne.
  * Rows of ne0 <= 32768 contiguous elements, any row strides; ne0 % 32 == 0 for
  * Q8_0 and Q8_1.  h and every later step are fp32 as ggml's nodes are (the sum
  * of squares in double); sum and F16 outputs round once, and the norm is
@@ -304,7 +305,7 @@ mi355_status mi355_rope_multi(mi355_context* ctx, const mi355_tensor* src, const
  * head_dim bytes at k + ((b * n_head_kv + h) * block_tokens) * head_dim (v alike),
  * with one F32 scale at k_scale[b * n_head_kv + h]: byte u stands for
  * (u - 128) * scale.  All device memory of the caller's, of any initial content;
- * k and v 16-byte aligned. */
+ * k and v 16-byte aligned.  Scales are not negative. */
 typedef struct mi355_kv_cache {
     uint8_t* k;
     uint8_t* v;
@@ -339,8 +340,8 @@ typedef struct mi355_kv_seqs {
  *           (scale 0: 128); kept tokens whose scale grew are rounded anew from
  *           the values they stood for.
  * A NaN or infinity makes its block's scale NaN or infinite and the block's
- * values with it, until it is written from its first row again.  A block may be
- * written through one sequence only in one call. */
+ * values with it, until it is written from its first row again.  Among the blocks
+ * that one call writes, of all sequences, each may stand once. */
 mi355_status mi355_kv_cache_write(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
                                   const mi355_tensor* k, const mi355_tensor* v, const int32_t* n_new);
 /* Reads tokens back as (byte - 128) * scale in fp32, F16 rounded once: row i of
@@ -360,7 +361,7 @@ mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache
  * Scores, softmax and outputs accumulate in fp32.  An F16 q enters the matrix
  * products as it is and an F32 q as two halves (22 bits); the probabilities enter
  * as F16 for an F16 dst and as two halves for an F32 dst; the cache's bytes
- * are exact in F16.
+ * are exact in F16.  dst overlaps nothing that the call reads.
  * mi355_kv_cache_attn_workspace_size: bytes of the context's workspace that these
  * sizes need (0: none); a call grows it on demand, except under stream capture,
  * where it has to be there (mi355_reserve_workspace).  Graphs captured from one context

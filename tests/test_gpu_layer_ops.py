@@ -123,6 +123,31 @@ def test_rms_norm_special_values(mi, ctx):
     assert torch.allclose(y[4], torch.ones(64, device="cuda"), rtol=1e-6) and not y[5].any()
 
 
+@pytest.mark.parametrize("q8", ["Q8_0", "Q8_1"])
+def test_rms_norm_special_values_in_eight_bits(mi, ctx, q8):
+    """Rows with NaN and infinities become the blocks that the quantizer makes of the F32 norm: scales of NaN, not 0."""
+    ty = getattr(mi, q8)
+    x = rnd(11, 6, 96)
+    x[1, 3] = math.nan
+    x[2, 5] = math.inf
+    x[3] = math.nan
+    w = torch.ones(96, device="cuda")
+    w[40], w[70] = math.nan, -math.inf
+    bytes_ = 3 * (34 if q8 == "Q8_0" else 36)
+    for weights in (None, w):
+        y = torch.empty_like(x)
+        got, want = (torch.full((6, bytes_), 0x55, dtype=torch.uint8, device="cuda") for _ in range(2))
+        ctx.rms_norm(tensor(mi, x), tensor(mi, y), 1e-5, w=0 if weights is None else weights.data_ptr())
+        ctx.rms_norm(tensor(mi, x), mi.from_torch(got, ty, [96, 6], [bytes_ // 3, bytes_, 6 * bytes_, 6 * bytes_]), 1e-5, w=0 if weights is None else weights.data_ptr())
+        ctx.quantize_rows(ty, mi.ACT_X86, tensor(mi, y), want.data_ptr())
+        ctx.synchronize()
+        assert torch.equal(got, want)
+        back = torch.zeros_like(x)
+        ctx.dequantize_rows(ty, got.data_ptr(), tensor(mi, back))
+        ctx.synchronize()
+        assert back[1].isnan().all() and back[3].isnan().all()
+
+
 @pytest.mark.parametrize("n", [32, 4736])
 def test_dequantize_rows(mi, ctx, orc, n):
     import numpy as np
