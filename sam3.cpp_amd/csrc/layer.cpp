@@ -150,7 +150,8 @@ mi355_status check_rope(mi355_context* ctx, const mi355_tensor* src, const mi355
 }
 
 mi355_status check_cache(mi355_context* ctx, const char* op, const mi355_kv_cache* c, const mi355_kv_seqs* s) {
-    if (!c || !s || !c->k || !c->v || !c->k_scale || !c->v_scale || (!s->table && s->n_seq && s->max_blocks) || (!s->n_kv && s->n_seq))
+    if (!c || !s || (c->n_blocks && (!c->k || !c->v || !c->k_scale || !c->v_scale)) || (!s->table && s->n_seq && s->max_blocks) ||
+        (!s->n_kv && s->n_seq))
         return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: null argument", op);
     if (c->n_blocks < 0 || c->n_head_kv < 1 || s->n_seq < 0 || s->max_blocks < 0)
         return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: negative cache or sequence sizes, or no heads", op);

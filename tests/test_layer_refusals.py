@@ -148,6 +148,14 @@ def test_kv_cache_description(mi, op):
         refused(mi, call(cache(mi), seqs(mi, **kw)), st, text)
 
 
+def test_kv_cache_of_no_blocks(mi):
+    """A cache without blocks needs no memory, whatever the table says."""
+    L = mi.lib()
+    c, s = cache(mi, n_blocks=0, k=None, v=None, k_scale=None, v_scale=None), seqs(mi)
+    assert L.mi355_supports_kv_cache_attn(c, s, t(mi, F16, [64, 5, 4, 3]), t(mi, F16, [64, 4, 5, 3]))
+    refused(mi, L.mi355_kv_cache_write(None, c, s, t(mi, F16, [64, 5, 2, 3]), t(mi, F16, [64, 5, 2, 3]), None), INVALID, "null context")
+
+
 def test_kv_cache_rows(mi):
     L, c, s = mi.lib(), cache(mi), seqs(mi)
     kv = t(mi, F16, [64, 5, 2, 3])
