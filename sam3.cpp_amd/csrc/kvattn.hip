@@ -618,11 +618,11 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 // are computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.  A lane's
 // eight scores (kh, hh) belong to 16 tokens of one block: scales and validity are uniform over them.
 //
-// Bounded by the VALU's work of a score (scale, exponential, sum, conversion: about 10 cycles of a SIMD for each score of
-// 64 lanes) and the LDS reads beside the matrix products: at 4096 causal F16 queries twice, 32 heads of 128 over 8 key
-// heads, 388 us or 814 TFLOP/s, the matrix pipe is busy 36 % of the time, the VALU 55 %, the LDS 52 % (bank conflicts
-// 9 %).  F32 queries and probabilities as two halves cost three more products of four: 5184 queries over 15552 tokens,
-// 8 heads of 64, 353 us for 165 GFLOP as the formula counts them.  Eight items at a time: 388 us; sixteen or thirty-two
+// Bounded by the VALU's work of a score (scale, exponential, sum, the bytes' conversion) and the matrix products, which
+// two wavefronts of a SIMD overlap in part, at a clock that they pull down to 2.0 GHz: at 4096 causal F16 queries twice, 32 heads
+// of 128 over 8 key heads, 388 us or 814 TFLOP/s, the matrix pipe is busy 40 % of the time, the VALU 50 %, the LDS 41 %
+// (10 % bank conflicts).  F32 queries and probabilities as two halves cost twice the products: 5184 queries over 15552
+// tokens, 8 heads of 64, 353 us for 165 GFLOP as the formula counts them (matrix pipe 45 %, VALU 64 %).  Eight items at a time: 388 us; sixteen or thirty-two
 // 466, one 482, the shortest row tiles first 497.
 template <int D, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles) {
