@@ -118,9 +118,10 @@ mi355_status ensure_arrived(mi355_context* ctx) {
     hipError_t e = hipMalloc(&p, KV_ARRIVALS * 4);
     if (e != hipSuccess) return fail(ctx, MI355_STATUS_ALLOC_FAILED, "hipMalloc(%d): %s", KV_ARRIVALS * 4, hipGetErrorString(e));
     e = hipMemsetAsync(p, 0, KV_ARRIVALS * 4, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);  // (a graph may be replayed on another stream)
     if (e != hipSuccess) {
         (void)hipFree(p);
-        return hip_check(ctx, e, "hipMemsetAsync");
+        return hip_check(ctx, e, "zeroing the counters");
     }
     ctx->arrived = p;
     return MI355_STATUS_SUCCESS;

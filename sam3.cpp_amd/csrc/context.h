@@ -69,7 +69,7 @@ mi355_status ensure_buffer(mi355_context* ctx, void** buf, size_t* size, size_t 
 // the stream's work, unless it is large enough.  A workspace that a captured call used is kept until the
 // context is freed; nothing grows under capture.
 mi355_status ensure_ws(mi355_context* ctx, size_t bytes);
-// The cache attention's counters, zeroed on the stream when they are made (not under capture).
+// The cache attention's counters, zeroed when they are made (not under capture), after the stream's work.
 mi355_status ensure_arrived(mi355_context* ctx);
 
 // The activation layout a producer pass should write for weights of type t:

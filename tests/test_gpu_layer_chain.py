@@ -209,6 +209,41 @@ def test_capture_needs_its_workspace(mi):
         ctx.close()
 
 
+def test_graph_on_another_stream(mi):
+    """A graph captured behind work that is still on its context's stream, and replayed at once on another one: what the
+    reservation made is there."""
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    ctx, plain = mi.Context(0, stream.cuda_stream), mi.Context(0)
+    try:
+        d = R.Cache(1, 200, 1, 64, 64, seed=8).fill([12800]).on_gpu(mi)
+        q, out, eager = torch.randn((1, 4, 1, 64), device="cuda"), torch.zeros((1, 1, 4, 64), device="cuda"), torch.zeros((1, 1, 4, 64), device="cuda")
+        busy = torch.randn((4096, 4096), device="cuda")
+        plain.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, q), tensor(mi, eager), 0.125)
+        plain.synchronize()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            work = busy @ busy  # (warms the product up)
+            stream.synchronize()
+            for _ in range(20):
+                work = busy @ work
+            ctx.reserve_workspace(ctx.kv_cache_attn_workspace_size(d["cache"], d["seqs"], tensor(mi, q)))
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            ctx.kv_cache_attn(d["cache"], d["seqs"], tensor(mi, q), tensor(mi, out), 0.125)
+            graph.capture_end()
+        with torch.cuda.stream(other):
+            for i in range(4):
+                graph.replay()
+                other.synchronize()
+                assert eager.any() and torch.equal(out, eager), i
+                out.zero_()
+                other.synchronize()
+        stream.synchronize()
+    finally:
+        ctx.close()
+        plain.close()
+
+
 def test_two_contexts_at_once(mi):
     """Two streams with a context each, launched together."""
     streams = [torch.cuda.Stream() for _ in range(2)]
