@@ -1032,9 +1032,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(const KvAttnArgs a, c
 // workgroups to a CU at most, and no more ranges than twice the root of the steps, since one workgroup joins them.
 // 32 conversations of 16384 tokens, 8 key heads: two ranges 153 us, four 164, sixteen 189; one of 19328 tokens with 28
 // heads: 16 us, and 26 with 128 ranges.
-// Beyond, the kernels of 32 and 128 rows are compared at their best number of ranges by the rounds of workgroups
+// Beyond, the kernels of 16, 32 and 128 rows are compared at their best number of ranges by the rounds of workgroups
 // over the CUs times a step's time (tens of nanoseconds, heads of 128) with one and with two workgroups on a CU: the
-// wide one has 1.7 times the throughput (F32 queries: 1.25), the narrow one four times the workgroups.
+// widest has the throughput of many rows, the narrowest the shortest steps and joins where the CUs are not full
+// (63 F32 rows of two sequences of 2424 tokens: 13.9 us with 16 rows to a workgroup, 19.8 with 32, 20.4 with 128; 80
+// rows of 32 sequences and heads of 3000 tokens: 24.5, 27.3 and 23.0).  An item's row tiles of 16 or 32 share an XCD, so
+// that fewer than eight items leave XCDs idle (3160 rows of four key heads: 29.6 us with 32 rows, 15.5 with 128).
 KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus) {
     if (window > 0) max_tokens = std::min<int64_t>(max_tokens, (int64_t)window + n_q + KV_STEP);  // (kv_range)
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
@@ -1056,17 +1059,22 @@ KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max
             if (s == 1 || t < best) best = t, p.splits = s;
         }
     } else {
-        double best = 0.0;
-        for (int nt : {2, 0}) {
+        double best = 1e300;
+        for (int nt : {1, 2, 0}) {
             if (nt == 0 && rows <= 64) break;
-            const int64_t wgs = items * ((rows + (nt ? 31 : 127)) / (nt ? 32 : 128));
+            const int64_t row = nt ? 16 * nt : 128, wgs = (rows + row - 1) / row;
             for (int s = 1; s <= std::min<int64_t>(steps, nt ? root : 32); ++s) {
-                const int64_t n = wgs * s, rounds = (n + 2 * cus - 1) / (2 * cus), per = (steps + s - 1) / s;
-                const double step = nt ? (n <= cus ? (q16 ? 155.0 : 185.0) : (q16 ? 165.0 : 200.0))
-                                       : (n <= cus ? (q16 ? 275.0 : 375.0) : (q16 ? 385.0 : 610.0));
-                const double join = s == 1 ? 0.0 : nt ? 480.0 + 50.0 * s : 450.0 + s * (double)(rows * items * D) / 10000.0;
-                const double t = rounds * (per * step + 250.0) + join;
-                if ((nt == 2 && s == 1) || t < best) {
+                const int64_t n = wgs * (nt ? (items * s + 7) / 8 * 8 : items * s), rounds = (n + 2 * cus - 1) / (2 * cus), per = (steps + s - 1) / s;
+                const bool alone = n <= cus;
+                const double step = nt == 1   ? (alone ? (q16 ? 100.0 : 115.0) : (q16 ? 140.0 : 170.0))
+                                    : nt == 2 ? (alone ? (q16 ? 155.0 : 185.0) : (q16 ? 165.0 : 200.0))
+                                              : (alone ? (q16 ? 275.0 : 375.0) : (q16 ? 385.0 : 610.0));
+                const double join = s == 1    ? 0.0
+                                    : nt == 1 ? 340.0 + 30.0 * s
+                                    : nt == 2 ? 480.0 + 50.0 * s
+                                              : 650.0 + s * (double)(rows * items * D) / 10000.0;
+                const double t = rounds * (per * step + (nt == 1 ? 180.0 : 250.0)) + join;
+                if (t < best) {
                     best = t;
                     p.nt = nt;
                     p.splits = s;
