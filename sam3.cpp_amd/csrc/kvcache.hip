@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const KvView c, const KvR
 }
 
 // Thread per eight elements of a row; blockIdx.y: keys or values.  Bound by memory (15552 tokens of 8 heads of 64 to halves,
-// 48 MB, in 11.6 us).
+// 48 MB, in 11.2 us).
 template <bool F16>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, const KvRows r, const int D8, const int64_t total) {
     const bool val = r.k ? blockIdx.y == 1 : true;
@@ -158,9 +158,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvView c, const KvRo
     const uint32_t hs = row / (uint32_t)r.n_tok;
     const int t = (int)(row - hs * r.n_tok), s = (int)(hs / (uint32_t)c.heads), h = (int)(hs - (uint32_t)s * c.heads);
     const int p = r.idx ? r.idx[(int64_t)s * r.n_tok + t] : t;
-    if (p < 0 || p >= kv_len(c, s)) return;
-    const int b = p >> c.bt_log2, id = c.table[(int64_t)s * c.max_blocks + b];
-    if (id < 0 || id >= c.n_blocks) return;
+    const int id = c.table[(int64_t)s * c.max_blocks + min(max(p, 0) >> c.bt_log2, c.max_blocks - 1)];  // (on its way beside the length)
+    if (p < 0 || p >= kv_len(c, s) || id < 0 || id >= c.n_blocks) return;
     const int64_t at = (int64_t)id * c.heads + h;
     const u32x2 u = reinterpret_cast<const u32x2*>(val ? c.v : c.k)[(at * c.bt + (p & (c.bt - 1))) * D8 + e];
     const float scale = (val ? c.v_scale : c.k_scale)[at];
