@@ -23,9 +23,16 @@ typedef v4h v4h_a2 __attribute__((aligned(2)));
 typedef h2v h2v_a2 __attribute__((aligned(2)));
 constexpr float KV_LOG2E = 1.44269504088896340736f;
 constexpr float KV_NONE = -1e30f;    // a reference that nothing has been taken against yet
+constexpr float KV_NO_P = -2e30f;    // the probabilities' own: below it, so that rows that see nothing are not taken for thin ones
 constexpr float KV_LIFT = 12.0f;     // probabilities are raised by 2^12 to keep small ones in fp16's normal range
 constexpr float KV_ROOM = 15.0f;     // and their reference moves when one would pass 2^15
 constexpr float KV_LIFT_SUM = 8.0f;  // the same where a lane's sum of 32 of them, and not each, is held below 2^15
+// A probability that a product takes as a half is 2^-b of its softmax weight (the largest weight one), b the negative lift
+// where the blocks' value scales are alike, and more by the binades that a block's scale lies below the others'.  The sum
+// of the rounded halves has the products' own roundings, which then cancel; but a half's step of 2^-24 is 2^(b - 24) of a
+// weight, so that from b on the unrounded probabilities are summed.  Steps of 2^-32 and 2^-29 of the largest weight are
+// left, which a million tokens of such weights may lose once each.
+constexpr float KV_THIN = -8.0f, KV_THIN_SUM = -5.0f;
 constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
 constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
 constexpr int KV_RANGES = 64;        // ranges of a row that one workgroup joins, at most
@@ -176,7 +183,8 @@ __device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int
 //           permutation.
 // A block's value scale is part of the exponent of its probabilities, P = 2^(s + log2(v_scale) - M), and
 // comes out of the sum again with one factor for a block, l += 2^(M - m - log2(v_scale)) sum P; where
-// that factor passes 2^90 (scales far below the others', and zero) the sum is taken of 2^(s - m) itself.
+// that factor passes 2^90 (scales far below the others', and zero) the sum is taken of 2^(s - m) itself, and for an
+// F16 output from 2^-8 on of P before its rounding (KV_THIN).
 // QS: an F32 q enters as two halves of 11 bits, scaled by a power of two that brings the row's largest
 // magnitude to about one.  PS: for an F32 output the probabilities enter as two halves too.
 //
@@ -262,7 +270,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
     v4f O[NT][NB];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        m_ref[t] = p_ref[t] = KV_NONE;
+        m_ref[t] = KV_NONE;
+        p_ref[t] = KV_NO_P;
         l_sum[t] = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) O[t][b] = v4f{0, 0, 0, 0};
@@ -389,9 +398,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
                     const h2v e1 = __builtin_convertvector((v2f{p[2] - (float)h1[0], p[3] - (float)h1[1]}), h2v);
                     PL[t][2 * u] = __builtin_bit_cast(uint32_t, e0);
                     PL[t][2 * u + 1] = __builtin_bit_cast(uint32_t, e1);
-                } else {  // the sum of what the product takes
+                } else {  // the sum of what the product takes (KV_THIN)
                     const h2v ones = {(_Float16)1.0f, (_Float16)1.0f};
                     sum = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, 0.0f, false), false);
+                    if (__builtin_amdgcn_ballot_w64(back > KV_THIN)) sum = back > KV_THIN ? (p[0] + p[1]) + (p[2] + p[3]) : sum;
                 }
                 if (__builtin_amdgcn_ballot_w64(back > 90.0f)) {
                     float d = 0.0f;
@@ -765,6 +775,11 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             }
     };
     uint64_t hide_groups = 0, nan_groups = 0, far_groups = 0;  // (sort_groups)
+    // Whether a group with 1 / value scale rv is thin against some row's references (KV_THIN_SUM), and whether one of these
+    // sixteen tiles' groups is, which have at most top_rv.
+    auto is_thin = [&](float rv) { return __builtin_amdgcn_ballot_w64(m_ref > KV_NONE && rv * back > __builtin_exp2f(KV_THIN_SUM)) != 0; };
+    float top_rv = 0.0f;
+    bool thin = false;
     // The token of score i of group j from the lane's first one of the tile.
     auto token = [](int j, int i) { return 32 * (j >> 1) + 16 * (j & 1) + 8 * (i >> 2) + (i & 3); };
     // Probabilities of a tile from its scores, at the references as they stand; returns the lane's sum of
@@ -787,7 +802,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             const h2v pl = __builtin_convertvector((v2f{p[0] - (float)ph[0], p[1] - (float)ph[1]}), h2v);
             PL[n >> 3][n & 7] = __builtin_bit_cast(uint32_t, pl);
             sums.s[j] += p[0] + p[1];
-        } else {  // the sum of what the product takes
+        } else {  // the sum of what the product takes (KV_THIN)
             sums.s[j] = __builtin_amdgcn_fdot2(ph, ones, sums.s[j], false);
         }
     };
@@ -819,6 +834,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             p_ref = pn;
             m_ref = mn;
             back = __builtin_amdgcn_exp2f(pn - mn);
+            if constexpr (!PS) thin = is_thin(top_rv);
             l_sum *= am;
 #pragma unroll
             for (int b = 0; b < NDB; ++b)
@@ -836,6 +852,19 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
                     for (int i = 0; i < 8; ++i) ls = __builtin_fmaf(on, __builtin_amdgcn_exp2f(__builtin_fmaf(S[j >> 1][o + i], f, -m_ref)), ls);
                 }
         }
+        if constexpr (!PS)
+            if (thin)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int gi = 4 * (tile & 15) + j, o = 8 * (j & 1);
+                    const float rv = read_lane(cur.rv, gi);
+                    if (!is_thin(rv)) continue;
+                    const float f0 = read_lane(cur.f, gi), f = QS ? fmaxf(f0 * qscale, 1e-37f) : f0, shift = read_lane(cur.lv, gi) - p_ref;
+                    float sum = -sums.s[j];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(S[j >> 1][o + i], f, shift));
+                    ls = __builtin_fmaf(sum * rv, back, ls);
+                }
         l_sum += ls;
     };
     // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
@@ -882,6 +911,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
         const bool far = !off && !bad && !(fabsf(cur.lv) <= 40.0f);
         if (off || bad) cur.f = cur.rv = 1.0f, cur.lv = 0.0f;
         if (far) cur.rv = 0.0f;
+        if constexpr (!PS) {
+            top_rv = group_max<64>(off ? 0.0f : cur.rv);
+            thin = is_thin(top_rv);
+        }
         cur.f = fmaxf(cur.f, 1e-37f);  // (0 times a hidden score)
         hide_groups = __builtin_amdgcn_ballot_w64(off);
         nan_groups = __builtin_amdgcn_ballot_w64(bad);

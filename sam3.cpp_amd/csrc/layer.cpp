@@ -363,7 +363,7 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     if (ws != MI355_STATUS_SUCCESS) return ws;
     a.part = static_cast<float*>(ctx->ws);
     a.arrived = static_cast<uint32_t*>(ctx->arrived);
-    Timed tm(ctx, "kv_cache_attn");
+    Timed tm(ctx, p.nt == 0 ? "kv_cache_attn_128" : p.nt == 2 ? "kv_cache_attn_32" : "kv_cache_attn_16");  // by the rows of a workgroup
     return hip_check(ctx, tm.done(launch_kv_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache_attn launch");
 }
 
