@@ -907,7 +907,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
     // block's scales are not finite the others become NaN, and the scales ones.  Value scales of zero or beyond
     // 2^40 either way add to l_sum on a way of their own.
     auto sort_groups = [&]() {
-        const bool off = cur.id < 0, bad = !off && !(cur.f <= 1e37f && cur.lv < __builtin_inff() && cur.lv == cur.lv);
+        const bool off = cur.id < 0, bad = !off && !(cur.f < __builtin_inff() && cur.lv < __builtin_inff() && cur.lv == cur.lv);
         const bool far = !off && !bad && !(fabsf(cur.lv) <= 40.0f);
         if (off || bad) cur.f = cur.rv = 1.0f, cur.lv = 0.0f;
         if (far) cur.rv = 0.0f;
@@ -915,7 +915,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs 
             top_rv = group_max<64>(off ? 0.0f : cur.rv);
             thin = is_thin(top_rv);
         }
-        cur.f = fmaxf(cur.f, 1e-37f);  // (0 times a hidden score)
+        if constexpr (!QS) cur.f = fmaxf(cur.f, 1e-37f);  // (0 times a hidden score; an F32 q's own factor comes first)
         hide_groups = __builtin_amdgcn_ballot_w64(off);
         nan_groups = __builtin_amdgcn_ballot_w64(bad);
         far_groups = __builtin_amdgcn_ballot_w64(far);

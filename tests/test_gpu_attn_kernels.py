@@ -36,7 +36,8 @@ def exact(c, q, n_q, scale, causal, window, dtype):
     """(out, tolerance) [seqs, n_q, heads, D] in float64, rows past n_q NaN.
 
     Off by at most, with w the exact weights, W = sum w |v| and o the output:
-      E = |scale| (sum |q k| (D + 3) U, for an F32 q with its two halves' 2^-22, + 2^-25 sum |k|, their range) in a score;
+      E = |scale| (sum |q k| (D + 3) U, for an F32 q with its two halves' 2^-22, + 2^-25 max |q| sum |k|, their range once the
+        row's largest is between one and two) in a score;
       A = 2 U (|score| log2(e) + |log2 of the value scale| + 16) in exp2's argument, the reference and the lift in it: both
         move a weight's numerator and its part of the sum, 2 (E + A) W together;
       a weight enters its product as a half (F32 dst: as two): H relative, in the sum as well where that is of the halves,
@@ -75,7 +76,7 @@ def exact(c, q, n_q, scale, causal, window, dtype):
             w = torch.nan_to_num(torch.softmax(sc.masked_fill(~seen, -math.inf), -1))
             o = w @ vv
             W = w @ vv.abs()
-            E = mag * ((D + 3) * U + (2.0 ** -22 if q32 else 0)) + (2.0 ** -25 * abs(scale) * kk.abs().sum(-1) if q32 else 0)
+            E = mag * ((D + 3) * U + (2.0 ** -22 if q32 else 0)) + (2.0 ** -25 * abs(scale) * qq.abs().amax(-1, keepdim=True) * kk.abs().sum(-1) if q32 else 0)
             A = 2 * U * (sc.abs() * 1.4427 + torch.where(sv > 0, torch.log2(sv.clamp(min=1e-300)).abs(), 0.0) + 16)
             EA = torch.where(seen, E + A, 0.0).amax(-1, keepdim=True)
             top = (w * sv).amax(-1, keepdim=True)
@@ -124,3 +125,18 @@ def test_weights_do_not_depend_on_the_values_size(mi, ctx, kernel, qt, ot):
                         c.vs[i] *= ratio
             c.vs[:] = torch.where(c.vs < 1e-37, torch.where(c.vs.isnan(), c.vs, 0.0), c.vs)
             check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot)
+
+
+@pytest.mark.parametrize("kernel", KERNELS, ids=NAMES)
+@pytest.mark.parametrize("ot", [F32, F16], ids=["ff", "fh"])
+def test_scales_at_the_ends_of_fp32(mi, ctx, kernel, ot):
+    """Large queries at a scale of zero and over a cache of small keys, small ones over large keys: the scores are what
+    their product says."""
+    for D, bt in ((64, 16), (96, 32), (128, 64)):
+        c, q, n_q = call(kernel, D, bt, F32, (0.97, 0.66, 0.83), seed=19)
+        check(mi, ctx, c, q * 2.0 ** 119, n_q, 0.0, kernel, ot)
+        keys = c.ks.clone()
+        c.ks = keys * 2.0 ** -119
+        check(mi, ctx, c, q * 2.0 ** 119, n_q, D ** -0.5, kernel, ot)
+        c.ks = keys * 2.0 ** 119
+        check(mi, ctx, c, q * 2.0 ** -132, n_q, 2.0 ** 10, kernel, ot)
