@@ -140,3 +140,119 @@ def test_scales_at_the_ends_of_fp32(mi, ctx, kernel, ot):
         check(mi, ctx, c, q * 2.0 ** 119, n_q, D ** -0.5, kernel, ot)
         c.ks = keys * 2.0 ** 119
         check(mi, ctx, c, q * 2.0 ** -132, n_q, 2.0 ** 10, kernel, ot)
+
+
+WINDOWS = {(16, False): (1, 100), (16, True): (900,), (32, False): (1, 100), (32, True): (500, 700), (128, False): (1, 100), (128, True): (100, 300)}
+SIZES = ((64, 16), (96, 32), (128, 64), (64, 128), (128, 16))
+KERNEL = pytest.mark.parametrize("kernel", KERNELS, ids=NAMES)
+TYPE = pytest.mark.parametrize("qt,ot", TYPES, ids=IDS)
+
+
+@KERNEL
+@TYPE
+@pytest.mark.parametrize("D,bt", SIZES)
+def test_causal_lengths(mi, ctx, kernel, D, bt, qt, ot):
+    """Lengths at and off tiles' ends, of one token, of none, below the queries' number (the first see nothing); counts
+    of all, a part and none of the queries."""
+    for lens, part in (((1.0, 0.93, 0.5), (1, 1, 1)), ((0.999, 0.31, 0.7), (1, 0.5, 1)), ((0.07, 0.011, 0.002), (1, 1, 1)), ((0.004, 0, 0.4), (1, 1, 0)),
+                       ((0.6, 0.21, 0.1), (0.17, 0.9, 1))):
+        c, q, n_q = call(kernel, D, bt, qt, lens, seed=3)
+        check(mi, ctx, c, q, [math.ceil(n * p) for n, p in zip(n_q, part)], D ** -0.5, kernel, ot)
+
+
+@KERNEL
+@TYPE
+@pytest.mark.parametrize("D,bt", SIZES)
+def test_masks_and_scales(mi, ctx, kernel, D, bt, qt, ot):
+    """Every token seen, windows with and without the causal limit, negative scales and none, scores far apart."""
+    c, q, n_q = call(kernel, D, bt, qt, (0.97, 0.66, 0.13), seed=5)
+    check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot, causal=False)
+    for window in WINDOWS[kernel]:
+        check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot, causal=True, window=window)
+        check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot, causal=False, window=window)
+    for scale in (-0.2, 0.0, 2.0):
+        check(mi, ctx, c, q, n_q, scale, kernel, ot)
+
+
+@KERNEL
+@TYPE
+@pytest.mark.parametrize("D,bt", SIZES)
+def test_blocks_that_are_not_there(mi, ctx, kernel, D, bt, qt, ot):
+    """The first, some between, the last, all of a sequence's: left out.  Key scales of zero, value scales of zero, and
+    scales that span twelve binades."""
+    c, q, n_q = call(kernel, D, bt, qt, (0.97, 0.66, 0.83), seed=7)
+    last = (int(c.n_kv[0]) - 1) // bt
+    c.table[0, 0], c.table[0, min(3, last)], c.table[0, last] = -1, c.k.shape[0], -2 ** 31
+    if c.table.shape[0] > 1:
+        c.table[1, :] = -1
+    ids = c.table[0].tolist()
+    for b, i in enumerate(ids):
+        if 0 <= i < c.k.shape[0]:
+            c.vs[i] = c.vs[i] * 2.0 ** (b % 13 - 6) if b % 5 else torch.zeros(c.heads)
+            if b % 7 == 1:
+                c.ks[i] = 0.0
+    c.vs[:] = torch.where(c.vs == 0, 0.0, c.vs)
+    check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot)
+    check(mi, ctx, c, q, n_q, D ** -0.5, kernel, ot, causal=False)
+
+
+@KERNEL
+@TYPE
+@pytest.mark.parametrize("ks,vs", [(math.nan, 1.0), (1.0, math.nan), (math.inf, 1.0), (1.0, math.inf), (math.inf, math.inf)])
+def test_scales_that_are_not_finite(mi, ctx, kernel, ks, vs, qt, ot):
+    """Queries that see a token of such a block get NaN in every element, all others what they get without the block."""
+    for D, bt in ((64, 16), (96, 32), (128, 64)):
+        for window in (0, WINDOWS[kernel][-1]):
+            c, q, n_q = call(kernel, D, bt, qt, (0.97, 0.8, 0.6), seed=11)
+            S, NQ, NH, _ = q.shape
+            want, tol = exact(c, q, n_q, D ** -0.5, True, window, ot)
+            head, block = c.heads - 1, int(c.n_kv[0]) // bt - (1 if bt == 64 else 2)
+            i = int(c.table[0, block])
+            c.ks[i, head], c.vs[i, head] = ks, vs
+            d = c.on_gpu(mi)
+            dst = torch.full((S, NQ, NH, D), 77.0, dtype=ot, device="cuda")
+            attend(mi, ctx, d, q.cuda(), dst, D ** -0.5, kernel, window=window)
+            n = int(c.n_kv[0])
+            p = n - NQ + torch.arange(NQ)
+            sees = p >= block * bt
+            if window:
+                sees &= p - window < min(block * bt + bt, n) - 1
+            hit = torch.zeros((S, NQ, NH), dtype=torch.bool)
+            hit[0, :, head * (NH // c.heads):] = sees[:, None]
+            got = dst.to(F64).cpu()
+            assert hit.any() and got[hit].isnan().all()
+            assert ((got - want.cpu()).abs() <= tol.cpu())[~hit].all()
+
+
+@KERNEL
+@TYPE
+def test_orders_and_pitches(mi, ctx, kernel, qt, ot):
+    """Queries in a product's rows and outputs at odd pitches and offsets: the bits of plain ones; what lies beside stays."""
+    for D, bt in ((64, 16), (96, 32), (128, 64)):
+        c, q, n_q = call(kernel, D, bt, qt, (0.97, 0.66, 0.83), seed=13)
+        S, NQ, NH, _ = q.shape
+        d = c.on_gpu(mi)
+        want = torch.empty((S, NQ, NH, D), dtype=ot, device="cuda")
+        attend(mi, ctx, d, q.cuda(), want, 0.11, kernel)
+        for off in (0, 1, 2):
+            wide = torch.zeros((NQ, S, NH, D + 5), dtype=qt, device="cuda")
+            qd = wide.transpose(0, 1)[..., off:off + D]
+            qd.copy_(q)
+            out = torch.full((NH, S, NQ, D + 7), 5.0, dtype=ot, device="cuda")
+            view = out.permute(1, 2, 0, 3)[..., off:off + D]
+            attend(mi, ctx, d, qd, view, 0.11, kernel)
+            assert torch.equal(view, want)
+            view.fill_(5)
+            assert (out == 5).all()
+
+
+@KERNEL
+def test_repeated_calls_have_the_same_bits(mi, ctx, kernel):
+    c, q, n_q = call(kernel, 128, 16, F16, (1.0, 0.9, 0.8), seed=17)
+    d, qd = c.on_gpu(mi), q.cuda()
+    first = None
+    for i in range(20):
+        dst = torch.full(q.shape, float(i), dtype=F16, device="cuda")
+        attend(mi, ctx, d, qd, dst, 0.1, kernel)
+        first = dst if first is None else first
+        assert torch.equal(dst, first)
