@@ -215,7 +215,7 @@ static void rms_launch(const RmsArgs& a, hipStream_t st) {
     else if (c <= 2048 && !few) rms_go<256, 8, XF16>(a, st);
     else if (c <= 2048) rms_go<1024, 2, XF16>(a, st);
     else if (c <= 4096) rms_go<1024, 4, XF16>(a, st);
-    else rms_go<1024, 8, XF16>(a, st);
+    else if constexpr (!XF16) rms_go<1024, 8, XF16>(a, st);  // (RMS_MAX halves are 4096 pieces)
 }
 
 hipError_t launch_rms_norm(const RmsArgs& a, hipStream_t st) {
