@@ -93,13 +93,13 @@ static bool capturing(const mi355_context* ctx) {
     return ctx->stream && hipStreamIsCapturing(ctx->stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone;
 }
 
-mi355_status ensure_ws(mi355_context* ctx, size_t bytes) {
+mi355_status ensure_ws(mi355_context* ctx, size_t bytes, bool captured_alloc) {
     const bool cap = bytes > 0 && (bytes > ctx->ws_size || !ctx->ws_captured) && capturing(ctx);
     if (bytes <= ctx->ws_size) {
         ctx->ws_captured = ctx->ws_captured || cap;
         return MI355_STATUS_SUCCESS;
     }
-    if (cap)
+    if (cap && (ctx->ws || !captured_alloc))
         return fail(ctx, MI355_STATUS_ALLOC_FAILED, "a captured call needs %zu bytes of workspace, the context has %zu (mi355_reserve_workspace)",
                     bytes, ctx->ws_size);
     if (ctx->ws_captured) {
@@ -108,7 +108,9 @@ mi355_status ensure_ws(mi355_context* ctx, size_t bytes) {
         ctx->ws_size = 0;
         ctx->ws_captured = false;
     }
-    return ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, bytes);
+    const mi355_status st = ensure_buffer(ctx, &ctx->ws, &ctx->ws_size, bytes);
+    ctx->ws_captured = cap && st == MI355_STATUS_SUCCESS;
+    return st;
 }
 
 mi355_status ensure_arrived(mi355_context* ctx) {

@@ -67,8 +67,9 @@ mi355_status ensure_buffer(mi355_context* ctx, void** buf, size_t* size, size_t 
 
 // The context's workspace of at least bytes, for a call that uses it now: replaced by a larger one, after
 // the stream's work, unless it is large enough.  A workspace that a captured call used is kept until the
-// context is freed; nothing grows under capture.
-mi355_status ensure_ws(mi355_context* ctx, size_t bytes);
+// context is freed; nothing grows under capture, but a context without one can make its first there
+// (captured_alloc, and where the capture's mode allows an allocation).
+mi355_status ensure_ws(mi355_context* ctx, size_t bytes, bool captured_alloc = true);
 // The cache attention's counters, zeroed when they are made (not under capture), after the stream's work.
 mi355_status ensure_arrived(mi355_context* ctx);
 

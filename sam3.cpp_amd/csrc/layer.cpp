@@ -359,7 +359,7 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
     const KvAttnPlan p = attn_plan(ctx, cache, seqs, q, a.window);
     mi355_status ws = p.nt && p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
-    if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes);
+    if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes, false);
     if (ws != MI355_STATUS_SUCCESS) return ws;
     a.part = static_cast<float*>(ctx->ws);
     a.arrived = static_cast<uint32_t*>(ctx->arrived);
