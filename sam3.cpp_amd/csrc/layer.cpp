@@ -12,9 +12,8 @@ namespace {
 bool is_float(int t) { return t == T_F32 || t == T_F16; }
 
 // an empty tensor needs no data
-bool has_data(const mi355_tensor* t) {
-    return t->data || t->ne[0] == 0 || t->ne[1] == 0 || t->ne[2] == 0 || t->ne[3] == 0;
-}
+bool empty(const mi355_tensor* t) { return t->ne[0] == 0 || t->ne[1] == 0 || t->ne[2] == 0 || t->ne[3] == 0; }
+bool has_data(const mi355_tensor* t) { return t->data || empty(t); }
 // every row of t starts on `bytes`
 bool rows_on(const mi355_tensor* t, uintptr_t bytes) {
     return ((reinterpret_cast<uintptr_t>(t->data) | (uintptr_t)t->nb[1] | (uintptr_t)t->nb[2] | (uintptr_t)t->nb[3]) &
@@ -253,7 +252,7 @@ mi355_status mi355_rms_norm(mi355_context* ctx, const mi355_tensor* x, const mi3
 }
 
 mi355_status mi355_dequantize_rows(mi355_context* ctx, int type, const void* src, const mi355_tensor* dst) {
-    if (!dst || !has_data(dst) || (!src && dst->data)) return fail(ctx, MI355_STATUS_INVALID_ARG, "dequantize_rows: null argument");
+    if (!dst || !has_data(dst) || (!src && !empty(dst))) return fail(ctx, MI355_STATUS_INVALID_ARG, "dequantize_rows: null argument");
     if (!dims_ok(dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "dequantize_rows: negative ne/nb or not the ggml layout");
     if (!(type == T_Q8_0 || type == T_Q8_1 || type == T_Q4_0 || type == T_Q4_1))
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "dequantize_rows: type %d not supported", type);
@@ -280,7 +279,7 @@ mi355_status mi355_rope_multi(mi355_context* ctx, const mi355_tensor* src, const
     RopeArgs a;
     const mi355_status st = check_rope(ctx, src, p, dst, &a);
     if (st != MI355_STATUS_SUCCESS) return st;
-    if ((!pos && src->data) || (reinterpret_cast<uintptr_t>(pos) & 3)) return fail(ctx, MI355_STATUS_INVALID_ARG, "rope_multi: pos null or not 4-byte aligned");
+    if ((!pos && !empty(src)) || (reinterpret_cast<uintptr_t>(pos) & 3)) return fail(ctx, MI355_STATUS_INVALID_ARG, "rope_multi: pos null or not 4-byte aligned");
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "rope_multi: null context");
     (void)hipSetDevice(ctx->device);
     a.src = static_cast<const char*>(src->data);

@@ -235,3 +235,14 @@ def test_python_descriptors(mi):
         mi.kv_seqs(torch.zeros((4, 7), dtype=torch.int64), torch.zeros(4, dtype=torch.int32))
     with pytest.raises(ValueError):
         mi.kv_seqs(torch.zeros((4, 7), dtype=torch.int32), torch.zeros(3, dtype=torch.int32))
+
+
+def test_empty_tensors_need_no_other_operand(mi):
+    """No rows and no tokens: neither source nor positions are asked for, whatever the tensor's own pointer is."""
+    for ptr in (None, 0x10000):
+        for ne in ([64, 0], [64, 3, 0, 2], [0, 3]):
+            refused(mi, mi.lib().mi355_dequantize_rows(None, Q8_0, None, t(mi, F32, ne, ptr=ptr)), INVALID, "null context")
+        for ne in ([64, 0, 5, 1], [64, 2, 0, 1], [64, 2, 5, 0]):
+            x = t(mi, F16, ne, ptr=ptr)
+            refused(mi, rope(mi, x, mi.rope_params(64, [32]), x, pos=None), INVALID, "null context")
+    refused(mi, rope(mi, t(mi, F16, [64, 2, 5, 1]), mi.rope_params(64, [32]), t(mi, F16, [64, 2, 5, 1]), pos=None), INVALID, "pos null")
