@@ -142,7 +142,8 @@ mi355_status mi355_tensor_memset(mi355_context* ctx, const mi355_tensor* t, uint
  * src1: F32 (any strides) or, with F16 src0, F16.  dst: F32, nb[0] = 4.
  * src1 may also hold the rows already quantized (mi355_rms_norm,
  * mi355_quantize_rows): Q8_0 with Q8_0 / Q4_0 weights, Q8_1 with Q4_1 ones, in
- * 2-D products; the same bits as with the finite F32 rows they were made of.
+ * 2-D products; the same bits as with the finite F32 rows they were made of,
+ * always by the int8 kernel (up to about 64 rows F32 rows have faster ways).
  * Q8_0/Q4_0 quantize src1 to Q8_0 and Q4_1 to Q8_1 (x86 variant) exactly as
  * ggml-cpu's from_float, then combine exact int32 block dots in fp32.  F16
  * converts src1 to F16 (round to nearest even) and accumulates in fp32. */
@@ -282,8 +283,10 @@ mi355_status mi355_dequantize_rows(mi355_context* ctx, int type, const void* src
  * sections: pairs of each axis, n_dims / 2 in all; MI355_ROPE_CONSECUTIVE: the
  * first sections[0] pairs have axis 0, and so on; MI355_ROPE_INTERLEAVED (three
  * axes): pair i has axis i % 3 = a for a = 1, 2 while i < 3 sections[a], and axis 0
- * otherwise.  Angles are taken modulo a turn in 64-bit fixed point, so far
- * positions lose nothing.  inverse 1 turns back (the gradient). */
+ * otherwise.  Angles are taken modulo a turn in 64-bit fixed point: at the ends of
+ * int32 a position's is good to 2^-30 of a turn (freq_scale up to 2 pi and
+ * freq_base away from one), below fp32's own step.  inverse 1 turns back (the
+ * gradient). */
 typedef enum { MI355_ROPE_ADJACENT = 0, MI355_ROPE_HALVES = 1 } mi355_rope_pairs; /* (2i, 2i+1); (i, i + n_dims/2) */
 typedef enum { MI355_ROPE_CONSECUTIVE = 0, MI355_ROPE_INTERLEAVED = 1 } mi355_rope_order;
 typedef struct mi355_rope_params {
@@ -360,7 +363,9 @@ mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache
  * one that sees a token of a block whose scales are not both finite gives NaN.
  * Scores, softmax and outputs accumulate in fp32.  An F16 q enters the matrix
  * products as it is and an F32 q as two halves (22 bits); the probabilities enter
- * as F16 for an F16 dst and as two halves for an F32 dst; the cache's bytes
+ * as F16 for an F16 dst and as two halves for an F32 dst, each times its block's
+ * value scale; the fp32 sum of an F16 dst is of these halves, and of the unrounded
+ * probabilities where a block's scale is far below others'.  The cache's bytes
  * are exact in F16.  dst overlaps nothing that the call reads.
  * mi355_kv_cache_attn_workspace_size: bytes of the context's workspace that these
  * sizes need (0: none); a call grows it on demand, except under stream capture,

@@ -170,8 +170,8 @@ struct MmPlan {
     size_t total() const { return q + d + s + align + part; }
 };
 
-// The int8-MFMA kernel takes plain 2-D GEMMs with block-quantized weights.
 bool q8_rows(const mi355_tensor* s1) { return s1->type == T_Q8_0 || s1->type == T_Q8_1; }  // src1 quantized already
+// The int8-MFMA kernel takes plain 2-D GEMMs with block-quantized weights.
 bool mm_i8_eligible(const mi355_tensor* s0, const mi355_tensor* s1) {
     return (s0->type == T_Q8_0 || s0->type == T_Q4_0 || s0->type == T_Q4_1) && s0->ne[2] == 1 && s0->ne[3] == 1 &&
            s1->ne[2] == 1 && s1->ne[3] == 1 && s0->ne[0] % 32 == 0;
@@ -202,7 +202,7 @@ int device_cus(int device) {
 // kernel: the MI355_MMQ_* route when the operands are eligible for it
 MmPlan mm_plan(const mi355_tensor* s0, const mi355_tensor* s1, int cus, bool split = true, int kernel = 0) {
     const bool prep = s0->layout == MI355_LAYOUT_INT8;
-    const bool i8 = prep || kernel != MI355_MMQ_F16 || q8_rows(s1);  // (8-bit rows are the int8 operand already)
+    const bool i8 = prep || kernel != MI355_MMQ_F16 || q8_rows(s1);  // (8-bit rows have the int8 kernel only)
     MmPlan pl;
     if (s0->type == T_F32) return pl;
     const int64_t K = s1->ne[0], M = s1->ne[1], Z = s1->ne[2] * s1->ne[3];

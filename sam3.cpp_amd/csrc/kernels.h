@@ -356,7 +356,7 @@ struct KvAttnArgs {
 constexpr int KV_ARRIVALS = 8192;
 struct KvAttnPlan {
     int nt, tiles;             // 16-row tiles of a workgroup (0: the kernel of 128 rows), workgroups over a sequence's rows
-    int splits;                // ranges of the tokens, joined by a second kernel
+    int splits;                // ranges of the tokens, joined by a row tile's last workgroup (128 rows: by a second kernel)
     size_t bytes;              // of part
 };
 KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);

@@ -189,8 +189,8 @@ __device__ __forceinline__ void join_ranges(const KvAttnArgs& a, int splits, int
 // magnitude to about one.  PS: for an F32 output the probabilities enter as two halves too.
 //
 // With many conversations the cache's bytes bound it: 32 of 16384 tokens, 32 heads of 128 over 8 key heads, 815 MB in
-// 152.5 us (5.3 TB/s).  With few tokens the chain of latencies does: table, block, scales, then the last workgroup's
-// join (777 tokens, 16 heads of 64 over 2: 7.0 us).
+// 153 us (5.3 TB/s).  With few tokens the chain of latencies does: table, block, scales, then the last workgroup's
+// join (777 tokens, 16 heads of 64 over 2: 7.2 us).
 template <int D, int NT, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int KC = D / 64, KM = D / 32, NB = D / 16;  // key chunks of 64, score products, output blocks
@@ -630,10 +630,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_rows_kernel(const KvAttnArgs a
 //
 // Bounded by the VALU's work of a score (scale, exponential, sum, the bytes' conversion) and the matrix products, which
 // two wavefronts of a SIMD overlap in part, at a clock that they pull down to 2.0 GHz: at 4096 causal F16 queries twice, 32 heads
-// of 128 over 8 key heads, 388 us or 814 TFLOP/s, the matrix pipe is busy 40 % of the time, the VALU 50 %, the LDS 41 %
-// (10 % bank conflicts).  F32 queries and probabilities as two halves cost twice the products: 5184 queries over 15552
-// tokens, 8 heads of 64, 353 us for 165 GFLOP as the formula counts them (matrix pipe 45 %, VALU 64 %).  Eight items at a time: 388 us; sixteen or thirty-two
-// 466, one 482, the shortest row tiles first 497.
+// of 128 over 8 key heads, 355 us or 890 TFLOP/s (320 to 430 from one run to another), the matrix pipe is busy 40 % of the
+// time, the VALU 50 %, the LDS 40 % (10 % bank conflicts).  F32 queries and probabilities as two halves cost twice the
+// products: 5184 queries over 15552 tokens, 8 heads of 64, 346 us for 165 GFLOP as the formula counts them (matrix pipe 45 %,
+// VALU 63 %).  Eight items at a time 388 us; beside it sixteen or thirty-two 466, one 482, the shortest row tiles first 497.
 template <int D, bool QS, bool PS>
 __global__ __launch_bounds__(256, 2) void kv_attn_tiles_kernel(const KvAttnArgs a, const int splits, const int tiles) {
     constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks

@@ -86,9 +86,9 @@ bool rope_table(const mi355_rope_params* p, RopeArgs* a) {
     }
     if (total != n || (p->order == MI355_ROPE_INTERLEAVED && p->sections[3] != 0)) return false;
     // freq_base ^ (-2^k / size) by squaring, of one size or each axis's: a power is a product of at most seven.
-    // 64-bit mantissas and a relative 2^-57 at most leave an int32 position's angle good to 2^-32 of a turn; the
-    // products below one are made in 64-bit fixed point (eight truncations: 2^-61 of a turn, 2^-30 at such a position),
-    // a tenth of the time of the floating ones.
+    // The 64-bit mantissas' error doubles with every squaring and is a relative e 2^-63 at pair e, which bases far from one
+    // make small beside what follows; the products below one are made in 64-bit fixed point (eight truncations: 2^-61 of a
+    // turn, 2^-30 at the ends of int32's positions), a tenth of the time of the floating ones.
     long double root[4][7];
     uint64_t fixed[4][7];
     const long double unit = (long double)p->freq_scale / 6.283185307179586476925286766559L, two64 = 18446744073709551616.0L;

@@ -81,8 +81,10 @@ __device__ __forceinline__ void st_some(char* row, int i, int n, const float (&v
 // v < V: 16 bytes a load.  A wavefront's rows follow one another at the grid's stride, so that the weights are
 // read once; what bounds the pass is memory, each operand moving once (8191 rows of 4736 halves with residual: 310 MB in
 // 62.7 us, which is past the copy rate since a part is still in the last-level cache; 5184 rows of 1024 floats to Q8_0:
-// 19.5 us with the read-back's launch for 80 MB), and for single tokens the launch (4096 floats: 7.4 us with the
-// read-back's).
+// 19.6 us with the read-back's launch for 80 MB), and for single tokens the launch (4096 floats: 6.6 to 8.4 us with the
+// read-back's).  Rows beyond 8192 floats or 16384 halves want more registers than 1024 threads have, and spill (140 to 656
+// bytes a lane): 512 rows of 32768 floats with residual 133 us, of halves 72, where their bytes take 57 and 29; 2048 of
+// 16384 floats 112 for 114.
 template <int T, int V, bool XF16>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(const RmsArgs a) {
 #pragma clang fp contract(off)

@@ -1,8 +1,9 @@
 // Rotary positions over several axes: pair i of a head turns by pos[axis(i)] * f(i).
 //
 // f is held as a fraction of a turn in 64-bit fixed point (turn = f / (2 pi) * 2^64), so
-// pos * turn modulo 2^64 is the angle modulo a turn, exact to 2^-33 turns for every int32
-// position; what is left within an eighth of a turn is a fp32 angle for two Taylor series.
+// pos * turn modulo 2^64 is the angle modulo a turn; turn itself is good to 2^-61 (rope_table), so
+// the angle to 2^-30 of a turn at the ends of int32.  What is left within an eighth of a turn is a
+// fp32 angle for two Taylor series.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -88,7 +89,7 @@ __device__ __forceinline__ void rope_st1(char* p, int i, float v) {
 // A thread turns four neighbouring pairs of a token in H heads, `across` heads apart, with one set of angles; its
 // neighbours take the head's other pairs, then the next heads.  Pieces after the pairs copy eight elements each.  Bound
 // by memory, every element moving once in 16-byte (halves of an F16 head: 8) accesses: 4 x 5184 tokens of 16 heads of 64
-// floats, 170 MB, in 35.5 us (4.8 TB/s); 32 single tokens of 40 heads of 128 halves are a launch, 4.3 us.
+// floats, 170 MB, in 35.5 us (4.8 TB/s); 32 single tokens of 40 heads of 128 halves are a launch, 5.0 us.
 template <bool F16, bool HALVES, int H>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs a, const int pieces, const int across, const int items) {
     const int i = blockIdx.x * 256 + threadIdx.x;
