@@ -256,3 +256,62 @@ def test_repeated_calls_have_the_same_bits(mi, ctx, kernel):
         attend(mi, ctx, d, qd, dst, 0.1, kernel)
         first = dst if first is None else first
         assert torch.equal(dst, first)
+
+
+def test_blocks_beyond_4_gib(mi, ctx):
+    """Each kernel follows blocks that lie past 32 bits of offset in the cache as it follows near ones."""
+    D, bt = 128, 64
+    n = (1 << 32) // (bt * D) + 700
+    k, v = (torch.empty(n * bt * D, dtype=torch.uint8, device="cuda") for _ in range(2))
+    for kernel in KERNELS:
+        c, q, n_q = call(kernel, D, bt, F16, (1.0, 0.77, 0.6), seed=23)
+        near = c.on_gpu(mi)
+        kv, blocks = c.heads, n // c.heads
+        kf, vf = (x[:blocks * kv * bt * D].reshape(blocks, kv, bt, D) for x in (k, v))
+        ks, vs = (torch.full((blocks, kv), math.nan, device="cuda") for _ in range(2))
+        ids = near["table"].long().flatten()
+        far = torch.arange(ids.numel(), device="cuda")
+        far[1::2] = blocks - 1 - far[1::2]  # every second block at the far end
+        kf[far], vf[far], ks[far], vs[far] = near["k"][ids], near["v"][ids], near["ks"][ids], near["vs"][ids]
+        table = far.to(torch.int32).reshape(c.table.shape)
+        there = dict(cache=mi.kv_cache(kf, vf, ks, vs), seqs=mi.kv_seqs(table, near["n_kv"]))
+        want, got = (torch.full(q.shape, x, dtype=F16, device="cuda") for x in (1.0, 2.0))
+        attend(mi, ctx, near, q.cuda(), want, 0.09, kernel)
+        attend(mi, ctx, there, q.cuda(), got, 0.09, kernel)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("kernel", KERNELS, ids=NAMES)
+def test_captured_and_replayed(mi, kernel):
+    """Two graphs of one context over caches of their own, replayed in turn between its eager calls, also after a larger
+    workspace has taken the place of theirs: the eager bits every time."""
+    stream = torch.cuda.Stream()
+    ctx = mi.Context(0, stream.cuda_stream)
+    try:
+        with torch.cuda.stream(stream):
+            sets = []
+            for seed in (29, 31):
+                c, q, _ = call(kernel, 64, 16, F16, (1.0, 0.9, 0.7), seed=seed)
+                d, qd = c.on_gpu(mi), q.cuda()
+                want, out = (torch.zeros(q.shape, dtype=F16, device="cuda") for _ in range(2))
+                sets.append((d, qd, want, out))
+            args = lambda x, o: (x[0]["cache"], x[0]["seqs"], tensor(mi, x[1].transpose(1, 2)), tensor(mi, o), 0.125)  # noqa: E731
+            ctx.reserve_workspace(max(ctx.kv_cache_attn_workspace_size(*args(x, x[3])[:3]) for x in sets))
+            graphs = []
+            for x in sets:
+                stream.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=stream):
+                    ctx.kv_cache_attn(*args(x, x[3]))
+                graphs.append(graph)
+                ctx.kv_cache_attn(*args(x, x[2]))
+            for i in range(5):
+                for x, graph in zip(sets, graphs):
+                    x[3].fill_(i)
+                    graph.replay()
+                    ctx.kv_cache_attn(*args(sets[i & 1], sets[i & 1][2]))
+                    stream.synchronize()
+                    assert x[2].any() and torch.equal(x[3], x[2]), i
+                ctx.reserve_workspace(1 << (20 + i))
+    finally:
+        ctx.close()
