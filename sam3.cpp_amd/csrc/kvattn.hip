@@ -30,8 +30,10 @@ constexpr float KV_LIFT_SUM = 8.0f;  // the same where a lane's sum of 32 of the
 // A probability that a product takes as a half is 2^-b of its softmax weight (the largest weight one), b the negative lift
 // where the blocks' value scales are alike, and more by the binades that a block's scale lies below the others'.  The sum
 // of the rounded halves has the products' own roundings, which then cancel; but a half's step of 2^-24 is 2^(b - 24) of a
-// weight, so that from b on the unrounded probabilities are summed.  Steps of 2^-32 and 2^-29 of the largest weight are
-// left, which a million tokens of such weights may lose once each.
+// weight, so that from these b on the unrounded probabilities are summed.  Steps of 2^-32 and 2^-29 of the largest weight are
+// left, which a million tokens of such weights may lose once each.  Every second block's values 2^-10 of the others': 2 x
+// 4096 queries over 5120 tokens 504 us, 459 where all are alike (those groups' exponentials a second time); single tokens
+// of 32 sequences over 16384 186 us either way.
 constexpr float KV_THIN = -8.0f, KV_THIN_SUM = -5.0f;
 constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
 constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
