@@ -379,6 +379,90 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
                                  const mi355_tensor* q, const int32_t* n_q, float scale, int causal, int32_t window,
                                  const mi355_tensor* dst);
 
+/* ggml_rms_norm and ggml_mul of every head of the queries and of the keys, and
+ * ggml_rope_multi of both, in one pass:
+ *   dst = turned(x / sqrt(mean over ne0 of x^2 + eps) * w)
+ * q [ne0, n_head, n_tokens, batch] and k [ne0, n_head_kv, n_tokens, batch] (either
+ * may be NULL, with its output), F32 or F16, both the same type; q_dst and k_dst of the
+ * same ne, F32 or F16, both the same type; rows of ne0 <= 256 contiguous elements, any
+ * other strides, so that q and k may be parts of one product's rows.  q_w, k_w:
+ * device F32 [ne0] or NULL.  pos and p as mi355_rope_multi's; elements past n_dims are
+ * normed and not turned.  Every step is fp32, F16 outputs round once.  An output may be
+ * its source, as the same tensor; any other overlap is not allowed. */
+int mi355_supports_qk_norm_rope(const mi355_tensor* q, const mi355_tensor* k, const mi355_rope_params* p,
+                                const mi355_tensor* q_dst, const mi355_tensor* k_dst);
+mi355_status mi355_qk_norm_rope(mi355_context* ctx, const mi355_tensor* q, const mi355_tensor* k, const float* q_w,
+                                const float* k_w, float eps, const int32_t* pos, const mi355_rope_params* p,
+                                const mi355_tensor* q_dst, const mi355_tensor* k_dst);
+
+/* A cache of keys and values in 4 bits, in blocks as mi355_kv_cache's, with an fp16
+ * scale d for each 32 elements of a token and head: nibble u stands for (u - 8) d.
+ * Row t of block b, head h is head_dim / 2 bytes at k + ((b * n_head_kv + h) *
+ * block_tokens + t) * head_dim / 2 (v alike): 32-bit words of eight elements, element
+ * 2 i in nibble i (bits 4 i on) and element 2 i + 1 in nibble i + 4.  Scales, with
+ * G = head_dim / 32: k_scale[((b * n_head_kv + h) * block_tokens + t) * G + group] and
+ * v_scale[((b * n_head_kv + h) * G + group) * block_tokens + t].  A scale has eight
+ * significant bits and a magnitude up to 8160, so that every value is an fp16 number, or
+ * is NaN, and then all scales of that token and head are.  All device memory of the
+ * caller's, of any initial content where no sequence has tokens; k and v 16-byte aligned, scales 8-byte. */
+typedef struct mi355_kv_cache4 {
+    uint8_t* k;
+    uint8_t* v;
+    uint16_t* k_scale;
+    uint16_t* v_scale;
+    int32_t n_blocks;
+    int32_t n_head_kv;
+    int32_t block_tokens; /* 16, 32, 64 or 128 */
+    int32_t head_dim;     /* 64, 96 or 128 */
+} mi355_kv_cache4;
+
+/* As mi355_kv_cache_write.  Of each 32 elements of a token and head, with ext the one
+ * farthest from zero (the positive one of two):
+ *   d = -ext / 8 rounded to eight significant bits, then to fp16 (to nearest, ties to even; one zero);
+ *   nibble = 8 + x / d rounded to nearest, ties to even, within 0 .. 15 (d 0: 8).
+ * A NaN, an infinity or a d beyond 8160 (magnitudes of 65408 and more) makes all scales of its token
+ * and head NaN, keys' and values'.  Tokens do not touch one another.  Among the tokens that
+ * one call writes, of all sequences, each place of the cache may stand once. */
+mi355_status mi355_kv_cache4_write(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                   const mi355_tensor* k, const mi355_tensor* v, const int32_t* n_new);
+/* As mi355_kv_cache_read: (nibble - 8) * d, exact in F32 and in F16. */
+mi355_status mi355_kv_cache4_read(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                  const int32_t* pos, const mi355_tensor* k, const mi355_tensor* v);
+/* As mi355_kv_cache_attn, over the cache's exact values: a query that attends to
+ * nothing gives zeros, one that sees a token with NaN scales NaN.  lse (device F32
+ * [n_seq][n_q][n_head], or NULL) takes log sum exp(scale q . k) over the tokens that the
+ * query sees, -inf where there is none; rows from n_q[s] on are left as they are.
+ * mi355_kv_cache4_attn_workspace_size as mi355_kv_cache_attn_workspace_size. */
+int mi355_supports_kv_cache4_attn(const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
+                                  const mi355_tensor* dst);
+size_t mi355_kv_cache4_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache,
+                                           const mi355_kv_seqs* seqs, const mi355_tensor* q, int32_t window);
+mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                  const mi355_tensor* q, const int32_t* n_q, float scale, int causal, int32_t window,
+                                  const mi355_tensor* dst, float* lse);
+/* What an attention looked at: adds to sums[s][h][t] (device F32 [n_seq][n_head_kv]
+ * [max_blocks * block_tokens]) the softmax weight of token t, exp(scale q . k - lse),
+ * summed over the queries that see it and the heads of key head h's group.  lse as
+ * mi355_kv_cache4_attn gave it for the same queries, scale, causal and window.  Places of
+ * tokens that no query sees are left as they are.  The same call gives the same bits. */
+mi355_status mi355_kv_cache4_weights(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                     const mi355_tensor* q, const int32_t* n_q, const float* lse, float scale,
+                                     int causal, int32_t window, float* sums);
+/* Brings sequences down to n_keep[s] tokens (device int32, within 0 .. max_keep; NULL: max_keep) where they
+ * have more: each head keeps, of its n = n_kv[s] tokens, the last `recent`, the
+ * first `first` (as many as n_keep[s] leaves), and of the others those with the largest
+ * sums, the lower token of equal ones (a NaN is the smallest number; tokens of blocks that are not
+ * there come last).  Kept tokens move together in place, in their order, from place 0 on;
+ * keys keep the positions that they were turned by.  Places from n_out[s] on are left as they are.  Outputs:
+ *   n_out[s] = min(n, n_keep[s]), the sequence's length from now on;
+ *   kept[s][h][j] (int32 [n_seq][n_head_kv][max_keep]): where token j stood, the others left as they are;
+ *   sums_out[s][h][..] (as sums): the kept tokens' sums, then zeros up to n, the others left as they are.
+ * A kept token whose block is not there leaves a NaN key in its place; one that moves to such a block is
+ * lost.  No output may overlap an input.  Sequences share no blocks. */
+mi355_status mi355_kv_cache4_evict(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                   const float* sums, const int32_t* n_keep, int32_t max_keep, int32_t first,
+                                   int32_t recent, float* sums_out, int32_t* kept, int32_t* n_out);
+
 /* ---- SAM3 ViT image encoder ----------------------------------------------
  * The graph sam3_build_vit_graph builds (sam3.cpp:3836-3853) run on this
  * backend: the prefix (patch embedding, tiled pos_embed, ln_pre;

@@ -89,6 +89,11 @@ class KvCache(C.Structure):
                 ("n_blocks", C.c_int32), ("n_head_kv", C.c_int32), ("block_tokens", C.c_int32), ("head_dim", C.c_int32)]
 
 
+class KvCache4(C.Structure):
+    """struct mi355_kv_cache4 (device pointers)."""
+    _fields_ = list(KvCache._fields_)
+
+
 class KvSeqs(C.Structure):
     """struct mi355_kv_seqs (device pointers)."""
     _fields_ = [("table", C.c_void_p), ("n_kv", C.c_void_p), ("n_seq", C.c_int32), ("max_blocks", C.c_int32)]
@@ -182,6 +187,15 @@ def lib():
         "mi355_supports_kv_cache_attn": (I, [C.POINTER(KvCache), C.POINTER(KvSeqs), T, T]),
         "mi355_kv_cache_attn_workspace_size": (SZ, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, C.c_int32]),
         "mi355_kv_cache_attn": (I, [P, C.POINTER(KvCache), C.POINTER(KvSeqs), T, P, F, I, C.c_int32, T]),
+        "mi355_supports_qk_norm_rope": (I, [T, T, C.POINTER(RopeParams), T, T]),
+        "mi355_qk_norm_rope": (I, [P, T, T, P, P, F, P, C.POINTER(RopeParams), T, T]),
+        "mi355_kv_cache4_write": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, T, P]),
+        "mi355_kv_cache4_read": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), P, T, T]),
+        "mi355_supports_kv_cache4_attn": (I, [C.POINTER(KvCache4), C.POINTER(KvSeqs), T, T]),
+        "mi355_kv_cache4_attn_workspace_size": (SZ, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, C.c_int32]),
+        "mi355_kv_cache4_attn": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, P, F, I, C.c_int32, T, P]),
+        "mi355_kv_cache4_weights": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, P, P, F, I, C.c_int32, P]),
+        "mi355_kv_cache4_evict": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), P, P, C.c_int32, C.c_int32, C.c_int32, P, P, P]),
         "mi355_vit_workspace_size": (SZ, [C.POINTER(VitHparams)]),
         "mi355_vit_prefix": (I, [P, C.POINTER(VitHparams), P, T, P, P, P, P]),
         "mi355_vit_block_forward": (I, [P, C.POINTER(VitHparams), C.POINTER(VitBlock), P]),
@@ -369,6 +383,22 @@ def kv_cache(k, v, k_scale, v_scale) -> KvCache:
     return c
 
 
+def kv_cache4(k, v, k_scale, v_scale) -> KvCache4:
+    """mi355_kv_cache4 over torch tensors: k, v uint8 [n_blocks, n_head_kv, block_tokens, head_dim / 2], k_scale float16
+    [n_blocks, n_head_kv, block_tokens, head_dim / 32], v_scale float16 [n_blocks, n_head_kv, head_dim / 32, block_tokens],
+    all contiguous."""
+    n, h, bt, half = k.shape
+    if v.shape != k.shape or half % 16 or tuple(k_scale.shape) != (n, h, bt, half // 16) or tuple(v_scale.shape) != (
+            n, h, half // 16, bt) or not all(x.is_contiguous() for x in (k, v, k_scale, v_scale)):
+        raise ValueError("kv_cache4: k, v [n_blocks, n_head_kv, block_tokens, head_dim / 2], k_scale [.., block_tokens, head_dim / 32], "
+                         "v_scale [.., head_dim / 32, block_tokens], contiguous")
+    if any(x.element_size() != 1 for x in (k, v)) or any(str(x.dtype) != "torch.float16" for x in (k_scale, v_scale)):
+        raise ValueError("kv_cache4: k, v hold bytes and the scales float16")
+    c = KvCache4(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n, h, bt, 2 * half)
+    c._keep = (k, v, k_scale, v_scale)
+    return c
+
+
 def kv_seqs(table, n_kv) -> KvSeqs:
     """mi355_kv_seqs over torch int32 tensors: table [n_seq, max_blocks], n_kv [n_seq]."""
     if any(str(x.dtype) != "torch.int32" or not x.is_contiguous() for x in (table, n_kv)) or tuple(n_kv.shape) != (table.shape[0],):
@@ -489,6 +519,37 @@ class Context:
 
     def kv_cache_attn_workspace_size(self, cache: KvCache, seqs: KvSeqs, q: Tensor, window: int = 0) -> int:
         return int(self.L.mi355_kv_cache_attn_workspace_size(self.h, cache, seqs, q, window))
+
+    def qk_norm_rope(self, q: Tensor | None, k: Tensor | None, eps: float, pos: int, params: RopeParams, q_dst: Tensor | None,
+                     k_dst: Tensor | None, q_w: int = 0, k_w: int = 0):
+        """The RMS norm of every head of q and k, times q_w and k_w, and their rotary positions."""
+        self._check(self.L.mi355_qk_norm_rope(self.h, q, k, q_w or None, k_w or None, eps, pos, params, q_dst, k_dst))
+
+    def kv_cache4_write(self, cache: KvCache4, seqs: KvSeqs, k: Tensor, v: Tensor, n_new: int = 0):
+        self._check(self.L.mi355_kv_cache4_write(self.h, cache, seqs, k, v, n_new or None))
+
+    def kv_cache4_read(self, cache: KvCache4, seqs: KvSeqs, k: Tensor | None, v: Tensor | None, pos: int = 0):
+        self._check(self.L.mi355_kv_cache4_read(self.h, cache, seqs, pos or None, k, v))
+
+    def kv_cache4_attn(self, cache: KvCache4, seqs: KvSeqs, q: Tensor, dst: Tensor, scale: float, n_q: int = 0, causal: bool = True,
+                       window: int = 0, lse: int = 0):
+        """lse: device float32 [n_seq, n_q, n_head] for the logarithms of the softmax's sums."""
+        self._check(self.L.mi355_kv_cache4_attn(self.h, cache, seqs, q, n_q or None, scale, 1 if causal else 0, window, dst, lse or None))
+
+    def kv_cache4_attn_workspace_size(self, cache: KvCache4, seqs: KvSeqs, q: Tensor, window: int = 0) -> int:
+        return int(self.L.mi355_kv_cache4_attn_workspace_size(self.h, cache, seqs, q, window))
+
+    def kv_cache4_weights(self, cache: KvCache4, seqs: KvSeqs, q: Tensor, lse: int, sums: int, scale: float, n_q: int = 0,
+                          causal: bool = True, window: int = 0):
+        """Adds each cached token's softmax weights to sums, device float32 [n_seq, n_head_kv, max_blocks * block_tokens]."""
+        self._check(self.L.mi355_kv_cache4_weights(self.h, cache, seqs, q, n_q or None, lse or None, scale, 1 if causal else 0, window,
+                                                   sums or None))
+
+    def kv_cache4_evict(self, cache: KvCache4, seqs: KvSeqs, sums: int, sums_out: int, max_keep: int, kept: int, n_out: int,
+                        n_keep: int = 0, first: int = 0, recent: int = 0):
+        """Keeps the first, the most recent and the heaviest tokens; kept: device int32 [n_seq, n_head_kv, max_keep]."""
+        self._check(self.L.mi355_kv_cache4_evict(self.h, cache, seqs, sums or None, n_keep or None, max_keep, first, recent,
+                                                 sums_out or None, kept or None, n_out or None))
 
     def reserve_workspace(self, size: int):
         self._check(self.L.mi355_reserve_workspace(self.h, size))

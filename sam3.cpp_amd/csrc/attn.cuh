@@ -1,5 +1,6 @@
 // Device code that the attention kernels share: reductions over the two halves of a wavefront, LDS
-// layouts of key and value tiles, transposing LDS reads.
+// layouts of key and value tiles, transposing LDS reads; and those over a cache: the tokens that queries see,
+// sums over a column's lanes, accesses past the caches.
 #pragma once
 #include "common.cuh"
 
@@ -47,6 +48,62 @@ __device__ __forceinline__ uint2 lds_read_tr16(const void* a) {
     typedef short v4s __attribute__((ext_vector_type(4)));
     const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(a));
     return __builtin_bit_cast(uint2, r);
+}
+
+namespace {
+constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
+constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
+}  // namespace
+
+// The tokens that a sequence's queries can see, and its queries.
+struct KvRange {
+    int n_kv, nq, pos0;  // length, queries, position of the first query
+    int lo, hi;          // tokens lo .. hi - 1 (lo a multiple of a step) are seen by some query
+};
+template <class Args>
+__device__ __forceinline__ KvRange kv_range(const Args& a, int s) {
+    KvRange r;
+    r.n_kv = (int)min((int64_t)max(a.c.n_kv[s], 0), (int64_t)a.c.max_blocks * a.c.bt);
+    r.nq = a.nq ? min(max(a.nq[s], 0), a.n_q) : a.n_q;
+    r.pos0 = r.n_kv - r.nq;
+    r.lo = a.window > 0 ? (int)(max((int64_t)r.pos0 - a.window + 1, (int64_t)0) & ~(int64_t)(KV_STEP - 1)) : 0;
+    r.hi = r.n_kv;
+    return r;
+}
+// Tokens of each of `splits` ranges: whole workgroup steps
+__device__ __forceinline__ int kv_chunk(const KvRange& r, int splits) {
+    const int n = max(r.hi - r.lo, 1), per = (n + splits - 1) / splits;
+    return (per + KV_SPAN - 1) / KV_SPAN * KV_SPAN;
+}
+
+__device__ __forceinline__ float read_lane(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
+
+
+// 2^-e and 2^e of a magnitude's exponent e, both normal
+struct Pow2 {
+    float down, up;
+};
+__device__ __forceinline__ Pow2 pow2_of(float top) {
+    const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -126), 126);
+    return {__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23)};
+}
+
+// max and sum over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48)
+__device__ __forceinline__ float col_max(float v) {
+    v = fmaxf(v, lane_swap_f<16>(v));
+    return fmaxf(v, lane_swap_f<32>(v));
+}
+__device__ __forceinline__ float col_sum(float v) {
+    v += lane_swap_f<16>(v);
+    return v + lane_swap_f<32>(v);
+}
+
+// A store past the caches of the workgroup's XCD, for a workgroup on another one, and a load of such
+__device__ __forceinline__ v2f get_through(const float* p) {
+    return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void put_through(float* p, v2f v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 }  // namespace mi355

@@ -321,6 +321,21 @@ struct RopeArgs {
     uint8_t axis[ROPE_PAIRS];
 };
 hipError_t launch_rope_multi(const RopeArgs& a, hipStream_t st);
+// Norm of each head's ne0 elements, times a weight, and its pairs turned; queries and keys in one launch
+struct QkArgs {
+    RopeArgs r;                // of the pairs, positions, tokens and batches (its src, dst, strides, heads and f16 unused)
+    struct Side {
+        const char* src;       // null: none
+        char* dst;
+        int64_t s_nb[3], d_nb[3];
+        const float* w;        // [ne0] or null
+        int heads;
+    } q, k;
+    float eps;
+    bool s16, d16;
+};
+constexpr int QK_MAX = 256;
+hipError_t launch_qk_norm_rope(const QkArgs& a, hipStream_t st);
 
 struct KvView {
     uint8_t *k, *v;
@@ -361,6 +376,50 @@ struct KvAttnPlan {
 };
 KvAttnPlan kv_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);
 hipError_t launch_kv_attn(const KvAttnArgs& a, const KvAttnPlan& p, int D, hipStream_t st);
+
+// ---- the 4-bit cache (kv4.cuh, kv4cache.hip, kv4attn.hip)
+struct Kv4View {
+    uint8_t *k, *v;
+    uint16_t *k_scale, *v_scale;  // [block][head][token][D / 32], [block][head][D / 32][token]
+    int n_blocks, heads, bt, bt_log2;
+    const int32_t* table;
+    const int32_t* n_kv;
+    int n_seq, max_blocks;
+};
+hipError_t launch_kv4_write(const Kv4View& c, const KvRows& r, int D, hipStream_t st);
+hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t st);
+struct Kv4EvictArgs {
+    Kv4View c;
+    const float* sums;         // [n_seq][heads][max_blocks * bt]
+    float* sums_out;
+    const int32_t* n_keep;     // [n_seq] or null
+    int max_keep, first, recent;
+    int32_t* kept;             // [n_seq][heads][max_keep]
+    int32_t* n_out;            // [n_seq]
+};
+hipError_t launch_kv4_evict(const Kv4EvictArgs& a, int D, hipStream_t st);
+struct Kv4AttnArgs {
+    Kv4View c;
+    const char* q;             // [D, n_q, heads, n_seq]
+    char* dst;                 // [D, heads, n_q, n_seq]
+    int64_t q_nb[3], d_nb[3];  // q: query, head, sequence; dst: head, query, sequence
+    int n_q, heads, group;     // group = heads / c.heads
+    const int32_t* nq;         // [n_seq] or null
+    float scale;
+    int causal, window;
+    bool q16, d16;
+    float* lse;                // [n_seq][n_q][heads] or null
+    float* part;
+    uint32_t* arrived;         // as KvAttnArgs'
+};
+struct Kv4AttnPlan {
+    int tiles;                 // workgroups over a sequence's rows
+    int splits;                // ranges of the tokens
+    size_t bytes;              // of part
+};
+Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);
+hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hipStream_t st);
+hipError_t launch_kv4_weights(const Kv4AttnArgs& a, float* sums, int D, hipStream_t st);
 
 // ---- SAM3 ViT glue (rows of E contiguous floats)
 struct LnArgs {

@@ -1,0 +1,359 @@
+// The 4-bit cache (kv4.cuh): written as tokens arrive, read back, and brought down to the tokens with the
+// largest sums of softmax weights.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn.cuh"
+#include "kv4.cuh"
+
+namespace mi355 {
+
+// -ext / 8 as the group's scale
+__device__ __forceinline__ uint16_t kv4_scale(float hi, float lo) {
+    const float ext = hi >= -lo ? hi : lo;
+    uint32_t u = __float_as_uint(ext * -0.125f);
+    u = (u + 0x7fffu + ((u >> 16) & 1)) & 0xffff0000u;  // eight significant bits, ties to even
+    const float d = __uint_as_float(u);
+    const uint16_t h = f2h(d);
+    return !(fabsf(d) <= 8160.0f) ? KV4_NAN : h == 0x8000 ? (uint16_t)0 : h;  // (one zero, whatever the elements' signs)
+}
+// 8 + x / d rounded to nearest even within 0 .. 15: the product with the reciprocal is at most one off, and
+// the remainder x - q d is exact in one fma (q d has twelve bits, and x lies within a step of it)
+__device__ __forceinline__ uint32_t kv4_nibble(float x, float d, float id) {
+    float q = rintf(x * id);
+    const float r = __builtin_fmaf(-q, d, x), half = 0.5f * fabsf(d);
+    if (fabsf(r) > half || (fabsf(r) == half && ((int)q & 1))) q += (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;
+    return (uint32_t)(int)(fminf(fmaxf(q, -8.0f), 7.0f) + 8.0f);
+}
+
+// D / 4 lanes to a token and head, eight elements each, the keys' lanes before the values': four lanes share a
+// group.  A token with an element that is not finite, or whose group's scale would pass 8160, has NaN scales in all its
+// groups, of keys and values: a key's NaN score is then what stands for it wherever it is seen, and its values need not be
+// told apart.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const KvRows r) {
+    constexpr int L = D / 4, TW = 64 / L;  // lanes of a token, tokens of a wavefront
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int h = blockIdx.y, s = blockIdx.z;
+    const int i = (blockIdx.x * 4 + w) * TW + lane / L, p = lane % L;
+    const int end = kv4_len(c, s), n_new = r.idx ? min(max(r.idx[s], 0), r.n_tok) : r.n_tok;
+    const int t = end - n_new + i;
+    int id = -1;
+    if (lane < TW * L && i < n_new && t >= 0) id = kv4_block(c, s, t);
+    if (__builtin_amdgcn_ballot_w64(id >= 0) == 0) return;
+    const bool val = p >= L / 2;
+    const int piece = val ? p - L / 2 : p;
+    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (id >= 0) {
+        const char* src = (val ? r.v + i * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : r.k + i * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2]) + piece * (F16 ? 16 : 32);
+        if constexpr (F16) {
+            const v8h y = *reinterpret_cast<const v8h_a2*>(src);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (float)y[j];
+        } else {
+            const v4f y0 = *reinterpret_cast<const v4f_a4*>(src), y1 = *reinterpret_cast<const v4f_a4*>(src + 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = j < 4 ? y0[j & 3] : y1[j & 3];
+        }
+    }
+    float hi = x[0], lo = x[0];
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi = fmaxf(hi, x[j]);
+        lo = fminf(lo, x[j]);
+        nan |= x[j] != x[j];
+    }
+    hi = fmaxf(hi, lane_swap_f<1>(hi));
+    hi = fmaxf(hi, lane_swap_f<2>(hi));
+    lo = fminf(lo, lane_swap_f<1>(lo));
+    lo = fminf(lo, lane_swap_f<2>(lo));
+    uint16_t s16 = kv4_scale(hi, lo);
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(nan || s16 == KV4_NAN);
+    if (bad >> (lane / L * L) & ((1ull << L) - 1)) s16 = KV4_NAN;
+    const float d = h2f(s16), id_d = d != 0.0f && d == d ? 1.0f / d : 0.0f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) word |= (id_d == 0.0f ? 8u : kv4_nibble(x[j], d, id_d)) << (4 * (j >> 1) + 16 * (j & 1));
+    if (id < 0) return;
+    const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
+    const int tok = t & (c.bt - 1);
+    *reinterpret_cast<uint32_t*>((val ? c.v : c.k) + (at + tok) * (D / 2) + 4 * piece) = word;
+    if ((piece & 3) == 0) {
+        if (val) c.v_scale[at * (D / 32) + (piece >> 2) * c.bt + tok] = s16;
+        else c.k_scale[(at + tok) * (D / 32) + (piece >> 2)] = s16;
+    }
+}
+
+// Thread per eight elements of a row; blockIdx.y: keys or values.
+template <bool F16>
+__global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4View c, const KvRows r, const int D8, const int64_t total) {
+    const bool val = r.k ? blockIdx.y == 1 : true;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= total) return;
+    const uint32_t row = (uint32_t)(i / D8);
+    const int e = (int)(i - (int64_t)row * D8);
+    const uint32_t hs = row / (uint32_t)r.n_tok;
+    const int t = (int)(row - hs * r.n_tok), s = (int)(hs / (uint32_t)c.heads), h = (int)(hs - (uint32_t)s * c.heads);
+    const int p = r.idx ? r.idx[(int64_t)s * r.n_tok + t] : t;
+    const int id = kv4_block(c, s, p);
+    if (p < 0 || p >= kv4_len(c, s) || id < 0) return;
+    const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
+    const int tok = p & (c.bt - 1), groups = D8 >> 2;
+    const uint32_t w = reinterpret_cast<const uint32_t*>(val ? c.v : c.k)[(at + tok) * D8 + e];
+    const float d = h2f(val ? c.v_scale[at * groups + (e >> 2) * c.bt + tok] : c.k_scale[(at + tok) * groups + (e >> 2)]);
+    char* o = (val ? r.v + t * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : r.k + t * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2]) + e * (F16 ? 16 : 32);
+    float y[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) y[x] = (float)((int)(w >> (4 * (x >> 1) + 16 * (x & 1)) & 15) - 8) * d;
+    if constexpr (F16) {
+        u32x4 z;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) z[x] = (uint32_t)f2h(y[2 * x]) | (uint32_t)f2h(y[2 * x + 1]) << 16;
+        *reinterpret_cast<u32x4_a2*>(o) = z;
+    } else {
+        *reinterpret_cast<v4f_a4*>(o) = v4f{y[0], y[1], y[2], y[3]};
+        *reinterpret_cast<v4f_a4*>(o + 16) = v4f{y[4], y[5], y[6], y[7]};
+    }
+}
+
+// ---- eviction
+// The tokens that one sequence and head keeps, in their order, and their sums: a workgroup each.  The m-th largest key
+// among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each), then one
+// walk over the tokens keeps what lies above it and as many of its equals, the first ones, as are missing.
+namespace {
+constexpr int EV_T = 1024;
+struct EvictSpan {
+    int n, keep, first, body;  // length; kept; tokens 0 .. first - 1 and body .. n - 1 are kept anyway
+};
+}  // namespace
+__device__ __forceinline__ EvictSpan evict_span(const Kv4EvictArgs& a, int s) {
+    EvictSpan e;
+    e.n = kv4_len(a.c, s);
+    e.keep = min(e.n, a.n_keep ? min(max(a.n_keep[s], 0), a.max_keep) : a.max_keep);
+    const int recent = min(a.recent, e.keep);
+    e.first = min(a.first, e.keep - recent);
+    e.body = e.n - recent;
+    return e;
+}
+// floats in the order of unsigned keys: tokens that are not there 0, NaN 1, then the numbers (both zeros alike)
+__device__ __forceinline__ uint32_t evict_key(float x, bool there) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return !there ? 0u : x != x ? 1u : u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t lanes_below() { return (1ull << (threadIdx.x & 63)) - 1; }
+
+__global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) {
+    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t wave[2][EV_T / 64];
+    __shared__ uint32_t found[2];
+    const Kv4View& c = a.c;
+    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+    const EvictSpan e = evict_span(a, s);
+    const int64_t room = (int64_t)c.max_blocks * c.bt, row = (int64_t)s * c.heads + h;
+    const float* sums = a.sums + row * room;
+    float* out = a.sums_out + row * room;
+    int32_t* kept = a.kept + row * a.max_keep;
+    if (h == 0 && t == 0) a.n_out[s] = e.keep;
+    if (e.keep == e.n) {
+        for (int i = t; i < e.n; i += EV_T) {
+            kept[i] = i;
+            out[i] = sums[i];
+        }
+        return;
+    }
+    auto key_at = [&](int i) { return evict_key(sums[i], kv4_block(c, s, i) >= 0); };
+    const int body = e.body - e.first;                 // tokens to choose among
+    uint32_t need = e.keep - e.first - (e.n - e.body); // and how many
+    uint32_t cut = 0, mask = 0;                        // the key's digits so far
+    const bool choose = need > 0 && (int)need < body;
+    if (choose) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+            for (int i = t; i < bins; i += EV_T) hist[i] = 0;
+            __syncthreads();
+            for (int i0 = 0; i0 < body; i0 += EV_T) {
+                const int i = i0 + t;
+                const uint32_t k = i < body ? key_at(e.first + i) : 0;
+                const bool on = i < body && (k & mask) == cut;
+                const uint32_t digit = k >> shift & (bins - 1);
+                // the digit of the wavefront's first lane is counted at once: most weights may be alike
+                const uint64_t act = __builtin_amdgcn_ballot_w64(on);
+                if (act == 0) continue;
+                const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(act));
+                const uint64_t same = __builtin_amdgcn_ballot_w64(on && digit == lead);
+                if ((t & 63) == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
+                if (on && digit != lead) atomicAdd(&hist[digit], 1u);
+            }
+            __syncthreads();
+            // from the top: the bin in which the need-th lies.  The first wavefront's lanes take bins / 64 each.
+            if (t < 64) {
+                const int per = bins / 64, b1 = bins - t * per;  // bins b1 - per .. b1 - 1
+                uint32_t mine = 0;
+                for (int b = 0; b < per; ++b) mine += hist[b1 - 1 - b];
+                uint32_t above = mine;
+                for (int o = 1; o < 64; o <<= 1) {
+                    const uint32_t v = __shfl_up(above, o, 64);
+                    if (t >= o) above += v;
+                }
+                above -= mine;
+                if (above < need && need <= above + mine) {
+                    int b = b1 - 1;
+                    while (above + hist[b] < need) above += hist[b--];
+                    found[0] = (uint32_t)b;
+                    found[1] = need - above;
+                }
+            }
+            __syncthreads();
+            cut |= found[0] << shift;
+            mask |= (uint32_t)(bins - 1) << shift;
+            need = found[1];
+            __syncthreads();
+        }
+    }
+    // kept: the first and the last ones, keys above cut, and the first `need` that equal it
+    int at = 0;
+    uint32_t equals = 0;
+    for (int i0 = 0; i0 < e.n; i0 += EV_T) {
+        const int i = i0 + t;
+        const bool in = i < e.n, mid = in && i >= e.first && i < e.body;
+        const float x = in ? sums[i] : 0.0f;
+        const uint32_t k = mid && choose ? evict_key(x, kv4_block(c, s, i) >= 0) : 0;
+        const bool eq = mid && choose && k == cut;
+        const uint64_t be = __builtin_amdgcn_ballot_w64(eq);
+        if ((t & 63) == 0) wave[0][t >> 6] = (uint32_t)__popcll(be);
+        __syncthreads();
+        uint32_t before = equals;
+        for (int w = 0; w < EV_T / 64; ++w) {
+            if (w == t >> 6) before = equals;
+            equals += wave[0][w];
+        }
+        const bool keep = in && (!mid || (choose ? k > cut || (eq && before + __popcll(be & lanes_below()) < need) : need > 0));
+        const uint64_t bk = __builtin_amdgcn_ballot_w64(keep);
+        if ((t & 63) == 0) wave[1][t >> 6] = (uint32_t)__popcll(bk);
+        __syncthreads();
+        int mine = at;
+        for (int w = 0; w < EV_T / 64; ++w) {
+            if (w == t >> 6) mine = at;
+            at += wave[1][w];
+        }
+        if (keep) {
+            mine += __popcll(bk & lanes_below());
+            kept[mine] = i;
+            out[mine] = x;
+        }
+    }
+    for (int i = e.keep + t; i < e.n; i += EV_T) out[i] = 0.0f;
+}
+
+// Kept rows go to their places, in order and in place: place j's row comes from kept[j] >= j.  A workgroup moves one
+// slice of a sequence and head's rows (16 bytes of the keys' or values' nibbles, or a scale of a group),
+// 1024 places at a time; the next places' rows are asked for before these are written, which no later row's
+// source is among, and written once all of the workgroup has what it asked for.
+template <int D>
+__global__ __launch_bounds__(EV_T) void kv4_move_kernel(const Kv4EvictArgs a, const int items) {
+    constexpr int NS = D / 32, G = D / 32, SL = 2 * NS + 2 * G;  // 16-byte slices of a row, groups, slices in all
+    const Kv4View& c = a.c;
+    // the slices of an item run on one XCD, whose L2 has their common lines
+    const int gb = blockIdx.x / (8 * SL), rb = blockIdx.x % (8 * SL), item = gb * 8 + (rb & 7), sl = rb >> 3;
+    if (item >= items) return;
+    const int h = item % c.heads, s = item / c.heads;
+    const EvictSpan e = evict_span(a, s);
+    if (e.keep == e.n) return;
+    const int32_t* kept = a.kept + (int64_t)item * a.max_keep;
+    const bool wide = sl < 2 * NS, val = wide ? sl >= NS : sl >= 2 * NS + G;
+    const int part = wide ? sl % NS : (sl - 2 * NS) % G;
+    struct Piece {
+        u32x4 x;
+        int j;
+        bool nan;
+    };
+    auto place = [&](int id, int tok) -> char* {
+        const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
+        if (wide) return reinterpret_cast<char*>(val ? c.v : c.k) + (at + tok) * (D / 2) + 16 * part;
+        return reinterpret_cast<char*>(val ? c.v_scale + at * G + part * c.bt + tok : c.k_scale + (at + tok) * G + part);
+    };
+    auto fetch = [&](int j0) {
+        Piece p;
+        p.j = j0 + (int)threadIdx.x;
+        p.x = u32x4{0, 0, 0, 0};
+        p.nan = false;
+        const int src = p.j < e.keep ? kept[p.j] : -1;
+        if (src <= p.j) {  // (none, or where it is already)
+            p.j = -1;
+            return p;
+        }
+        const int id = kv4_block(c, s, src);
+        if (id < 0) p.nan = true;
+        else if (wide) p.x = *reinterpret_cast<const u32x4*>(place(id, src & (c.bt - 1)));
+        else p.x[0] = *reinterpret_cast<const uint16_t*>(place(id, src & (c.bt - 1)));
+        return p;
+    };
+    Piece next = fetch(0);
+    for (int j0 = 0; j0 < e.keep; j0 += EV_T) {
+        const Piece p = next;
+        if (j0 + EV_T < e.keep) next = fetch(j0 + EV_T);
+        asm volatile("" ::"v"(p.x) : "memory");  // (this step's row has arrived)
+        lds_barrier();
+        if (p.j < 0) continue;
+        const int id = kv4_block(c, s, p.j);
+        if (id < 0) continue;
+        char* d = place(id, p.j & (c.bt - 1));
+        // a row whose block is not there leaves a NaN key: its place never shows what stood there
+        if (p.nan) {
+            if (!wide) *reinterpret_cast<uint16_t*>(d) = KV4_NAN;
+        } else if (wide) *reinterpret_cast<u32x4*>(d) = p.x;
+        else *reinterpret_cast<uint16_t*>(d) = (uint16_t)p.x[0];
+    }
+}
+
+template <int D>
+static void kv4_write_go(const Kv4View& c, const KvRows& r, hipStream_t st) {
+    constexpr int per = 4 * (64 / (D / 4));
+    const dim3 g((unsigned)((r.n_tok + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seq);
+    if (r.f16) kv4_write_kernel<D, true><<<g, 256, 0, st>>>(c, r);
+    else kv4_write_kernel<D, false><<<g, 256, 0, st>>>(c, r);
+}
+
+hipError_t launch_kv4_write(const Kv4View& c, const KvRows& r, int D, hipStream_t st) {
+    if (c.n_seq <= 0 || r.n_tok <= 0 || c.max_blocks <= 0 || c.n_blocks <= 0) return hipSuccess;
+    switch (D) {
+        case 64: kv4_write_go<64>(c, r, st); break;
+        case 96: kv4_write_go<96>(c, r, st); break;
+        case 128: kv4_write_go<128>(c, r, st); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t st) {
+    const int64_t total = (int64_t)r.n_tok * c.heads * c.n_seq * (D / 8);
+    if (total <= 0 || c.max_blocks <= 0 || c.n_blocks <= 0) return hipSuccess;
+    if ((total + 255) / 256 > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 g((unsigned)((total + 255) / 256), r.k && r.v ? 2 : 1);
+    if (r.f16) kv4_read_kernel<true><<<g, 256, 0, st>>>(c, r, D / 8, total);
+    else kv4_read_kernel<false><<<g, 256, 0, st>>>(c, r, D / 8, total);
+    return hipGetLastError();
+}
+
+template <int D>
+static void kv4_move_go(const Kv4EvictArgs& a, hipStream_t st) {
+    const int items = a.c.heads * a.c.n_seq;
+    kv4_move_kernel<D><<<(unsigned)((int64_t)(items + 7) / 8 * 8 * (D / 8)), EV_T, 0, st>>>(a, items);
+}
+
+hipError_t launch_kv4_evict(const Kv4EvictArgs& a, int D, hipStream_t st) {
+    if (a.c.n_seq <= 0) return hipSuccess;
+    if ((int64_t)(a.c.heads * (int64_t)a.c.n_seq + 7) / 8 * 8 * (D / 8) > INT32_MAX) return hipErrorInvalidValue;
+    kv4_select_kernel<<<dim3((unsigned)a.c.heads, (unsigned)a.c.n_seq), EV_T, 0, st>>>(a);
+    if (a.c.n_blocks <= 0 || a.c.max_blocks <= 0 || a.max_keep <= 0) return hipGetLastError();
+    switch (D) {
+        case 64: kv4_move_go<64>(a, st); break;
+        case 96: kv4_move_go<96>(a, st); break;
+        case 128: kv4_move_go<128>(a, st); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace mi355

@@ -35,30 +35,8 @@ constexpr float KV_LIFT_SUM = 8.0f;  // the same where a lane's sum of 32 of the
 // 4096 queries over 5120 tokens 504 us, 459 where all are alike (those groups' exponentials a second time); single tokens
 // of 32 sequences over 16384 186 us either way.
 constexpr float KV_THIN = -8.0f, KV_THIN_SUM = -5.0f;
-constexpr int KV_STEP = 32;          // tokens of one step of a wavefront
-constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
 constexpr int KV_RANGES = 64;        // ranges of a row that one workgroup joins, at most
 }  // namespace
-
-// The tokens that a sequence's queries can see, and its queries.
-struct KvRange {
-    int n_kv, nq, pos0;  // length, queries, position of the first query
-    int lo, hi;          // tokens lo .. hi - 1 (lo a multiple of a step) are seen by some query
-};
-__device__ __forceinline__ KvRange kv_range(const KvAttnArgs& a, int s) {
-    KvRange r;
-    r.n_kv = (int)min((int64_t)max(a.c.n_kv[s], 0), (int64_t)a.c.max_blocks * a.c.bt);
-    r.nq = a.nq ? min(max(a.nq[s], 0), a.n_q) : a.n_q;
-    r.pos0 = r.n_kv - r.nq;
-    r.lo = a.window > 0 ? (int)(max((int64_t)r.pos0 - a.window + 1, (int64_t)0) & ~(int64_t)(KV_STEP - 1)) : 0;
-    r.hi = r.n_kv;
-    return r;
-}
-// Tokens of each of `splits` ranges: whole workgroup steps
-__device__ __forceinline__ int kv_chunk(const KvRange& r, int splits) {
-    const int n = max(r.hi - r.lo, 1), per = (n + splits - 1) / splits;
-    return (per + KV_SPAN - 1) / KV_SPAN * KV_SPAN;
-}
 
 // log2 of a block's scale, -inf for 0; the instruction takes no subnormals
 __device__ __forceinline__ float scale_log2(float v) {
@@ -85,8 +63,6 @@ __device__ __forceinline__ void group_scales(const KvAttnArgs& a, int hk, float 
     x.lv = x.id >= 0 ? scale_log2(vs) : 0.0f;
     x.rv = 1.0f / vs;
 }
-__device__ __forceinline__ float read_lane(float v, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i)); }
-
 // four bytes of keys as the halves u - 128 (exact): 0x64uu is the half 1024 + u
 __device__ __forceinline__ void key_halves(uint32_t v, uint32_t* o) {
     const h2v off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
@@ -98,33 +74,6 @@ __device__ __forceinline__ uint32_t value_halves(uint32_t t0, uint32_t t1, int b
     const h2v mul = {(_Float16)32768.0f, (_Float16)32768.0f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
     const h2v u = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(t1, t0, 0x0c040c00u | (uint32_t)b | (uint32_t)b << 16));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, mul, off));
-}
-
-// 2^-e and 2^e of a magnitude's exponent e, both normal
-struct Pow2 {
-    float down, up;
-};
-__device__ __forceinline__ Pow2 pow2_of(float top) {
-    const int e = min(max((int)((__float_as_uint(top) >> 23) & 255) - 127, -126), 126);
-    return {__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23)};
-}
-
-// max and sum over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48)
-__device__ __forceinline__ float col_max(float v) {
-    v = fmaxf(v, lane_swap_f<16>(v));
-    return fmaxf(v, lane_swap_f<32>(v));
-}
-__device__ __forceinline__ float col_sum(float v) {
-    v += lane_swap_f<16>(v);
-    return v + lane_swap_f<32>(v);
-}
-
-// A store past the caches of the workgroup's XCD, for a workgroup on another one, and a load of such
-__device__ __forceinline__ v2f get_through(const float* p) {
-    return __builtin_bit_cast(v2f, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-}
-__device__ __forceinline__ void put_through(float* p, v2f v) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Four elements from e on of row pr (sequence, query, head in that order), joined from the row's n ranges in the ranges'

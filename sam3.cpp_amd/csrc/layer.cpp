@@ -1,5 +1,6 @@
 // C-ABI entry points of the nodes around a layer's products: RMS norm with the residual and an 8-bit
-// output, dequantized rows, rotary positions, the 8-bit key/value cache and its attention.
+// output, dequantized rows, rotary positions, also with the norms of queries and keys before them, the
+// 8-bit and 4-bit key/value caches with their attention, and the eviction of cached tokens.
 #include <climits>
 #include <cmath>
 
@@ -148,7 +149,40 @@ mi355_status check_rope(mi355_context* ctx, const mi355_tensor* src, const mi355
     return MI355_STATUS_SUCCESS;
 }
 
-mi355_status check_cache(mi355_context* ctx, const char* op, const mi355_kv_cache* c, const mi355_kv_seqs* s) {
+// Queries or keys of qk_norm_rope, and their output
+mi355_status check_qk(mi355_context* ctx, const mi355_tensor* x, const mi355_tensor* y, const mi355_rope_params* p) {
+    if (!has_data(x) || !has_data(y)) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: null argument");
+    if (!dims_ok(x) || !dims_ok(y)) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: negative ne/nb or not the ggml layout");
+    if (!is_float(x->type) || !is_float(y->type)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: tensors must be F32 or F16");
+    if (!same_ne(x, y)) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: shape mismatch");
+    if (p->n_dims > x->ne[0]) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: n_dims %d beyond ne0", p->n_dims);
+    if (x->ne[0] > QK_MAX) return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: heads of more than %d elements", QK_MAX);
+    if (!rows_ok(x) || !rows_ok(y)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: rows must be contiguous and aligned to their type");
+    if (!rows_fit(x)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: sizes beyond the launch limits");
+    return MI355_STATUS_SUCCESS;
+}
+mi355_status check_qk_norm_rope(mi355_context* ctx, const mi355_tensor* q, const mi355_tensor* k, const mi355_rope_params* p,
+                                const mi355_tensor* q_dst, const mi355_tensor* k_dst, RopeArgs* a) {
+    if ((!q && !k) || !p || !q != !q_dst || !k != !k_dst)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: null argument, or a source without its output");
+    if (!rope_table(p, a)) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: parameters out of range, or sections that do not make n_dims / 2 pairs");
+    for (int i = 0; i < 2; ++i) {
+        const mi355_tensor *x = i ? k : q, *y = i ? k_dst : q_dst;
+        if (!x) continue;
+        const mi355_status st = check_qk(ctx, x, y, p);
+        if (st != MI355_STATUS_SUCCESS) return st;
+    }
+    if (q && k) {
+        if (q->type != k->type || q_dst->type != k_dst->type) return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: q and k must have the same types");
+        if (q->ne[0] != k->ne[0] || q->ne[2] != k->ne[2] || q->ne[3] != k->ne[3])
+            return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: q and k must have the same head size, tokens and batches");
+    }
+    return MI355_STATUS_SUCCESS;
+}
+
+// either cache; SCALES: alignment of its scales
+template <int SCALES = 4, class Cache>
+mi355_status check_cache(mi355_context* ctx, const char* op, const Cache* c, const mi355_kv_seqs* s) {
     if (!c || !s || (c->n_blocks && (!c->k || !c->v || !c->k_scale || !c->v_scale)) || (!s->table && s->n_seq && s->max_blocks) ||
         (!s->n_kv && s->n_seq))
         return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: null argument", op);
@@ -159,25 +193,29 @@ mi355_status check_cache(mi355_context* ctx, const char* op, const mi355_kv_cach
     if (!(c->head_dim == 64 || c->head_dim == 96 || c->head_dim == 128))
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: head size %d (supported: 64, 96, 128)", op, c->head_dim);
     if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) ||
-        ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale) | reinterpret_cast<uintptr_t>(s->table) |
-          reinterpret_cast<uintptr_t>(s->n_kv)) & 3))
-        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: the cache must be 16-byte aligned, scales, table and lengths 4-byte", op);
+        ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & (SCALES - 1)) ||
+        ((reinterpret_cast<uintptr_t>(s->table) | reinterpret_cast<uintptr_t>(s->n_kv)) & 3))
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: the cache must be 16-byte aligned, scales %d-byte, table and lengths 4-byte", op, SCALES);
     if (c->n_head_kv > 65535 || s->n_seq > 65535 || (int64_t)s->max_blocks * c->block_tokens > 1 << 30)
         return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: sizes beyond the launch limits", op);
     return MI355_STATUS_SUCCESS;
 }
 
-KvView kv_view(const mi355_kv_cache* c, const mi355_kv_seqs* s) {
-    KvView v;
+template <class View, class Cache>
+View view_as(const Cache* c, const mi355_kv_seqs* s) {
+    View v;
     v.k = c->k; v.v = c->v; v.k_scale = c->k_scale; v.v_scale = c->v_scale;
     v.n_blocks = c->n_blocks; v.heads = c->n_head_kv; v.bt = c->block_tokens;
     v.bt_log2 = __builtin_ctz((unsigned)c->block_tokens);
     v.table = s->table; v.n_kv = s->n_kv; v.n_seq = s->n_seq; v.max_blocks = s->max_blocks;
     return v;
 }
+KvView kv_view(const mi355_kv_cache* c, const mi355_kv_seqs* s) { return view_as<KvView>(c, s); }
+Kv4View kv4_view(const mi355_kv_cache4* c, const mi355_kv_seqs* s) { return view_as<Kv4View>(c, s); }
 
 // k and v [head_dim, n_tokens, n_head_kv, n_seq] of a write or read (either null only when reading)
-mi355_status kv_rows(mi355_context* ctx, const char* op, const mi355_kv_cache* c, const mi355_kv_seqs* s, const mi355_tensor* k,
+template <class Cache>
+mi355_status kv_rows(mi355_context* ctx, const char* op, const Cache* c, const mi355_kv_seqs* s, const mi355_tensor* k,
                      const mi355_tensor* v, const int32_t* idx, KvRows* r) {
     const mi355_tensor* one = k ? k : v;
     r->k = r->v = nullptr;
@@ -200,19 +238,33 @@ mi355_status kv_rows(mi355_context* ctx, const char* op, const mi355_kv_cache* c
     return MI355_STATUS_SUCCESS;
 }
 
-mi355_status check_attn(mi355_context* ctx, const mi355_kv_cache* c, const mi355_kv_seqs* s, const mi355_tensor* q,
-                        const mi355_tensor* dst) {
-    const mi355_status st = check_cache(ctx, "kv_cache_attn", c, s);
+// q [head_dim, n_q, n_head, n_seq] over a cache
+template <int SCALES = 4, class Cache>
+mi355_status check_queries(mi355_context* ctx, const char* op, const Cache* c, const mi355_kv_seqs* s, const mi355_tensor* q) {
+    const mi355_status st = check_cache<SCALES>(ctx, op, c, s);
     if (st != MI355_STATUS_SUCCESS) return st;
-    if (!q || !dst || !has_data(q) || !has_data(dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache_attn: null argument");
-    if (!dims_ok(q) || !dims_ok(dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache_attn: negative ne/nb or not the ggml layout");
-    if (!is_float(q->type) || !is_float(dst->type)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache_attn: q and dst must be F32 or F16");
+    if (!q || !has_data(q)) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: null argument", op);
+    if (!dims_ok(q)) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: negative ne/nb or not the ggml layout", op);
+    if (!is_float(q->type)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: q must be F32 or F16", op);
     if (q->ne[0] != c->head_dim || q->ne[3] != s->n_seq || q->ne[2] < 1 || q->ne[2] % c->n_head_kv != 0)
-        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache_attn: q must be [head_dim, n_q, n_head, n_seq], n_head a multiple of n_head_kv");
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: q must be [head_dim, n_q, n_head, n_seq], n_head a multiple of n_head_kv", op);
+    if (!rows_ok(q)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: rows must be contiguous and aligned to their type", op);
+    if (!rows_fit(q) || q->ne[2] > 65535 || q->ne[1] > INT_MAX / 2) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: sizes beyond the launch limits", op);
+    return MI355_STATUS_SUCCESS;
+}
+
+// and what the attention gives for it, [head_dim, n_head, n_q, n_seq]
+template <int SCALES = 4, class Cache>
+mi355_status check_attn(mi355_context* ctx, const char* op, const Cache* c, const mi355_kv_seqs* s, const mi355_tensor* q,
+                        const mi355_tensor* dst) {
+    const mi355_status st = check_queries<SCALES>(ctx, op, c, s, q);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (!dst || !has_data(dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: null argument", op);
+    if (!dims_ok(dst)) return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: negative ne/nb or not the ggml layout", op);
+    if (!is_float(dst->type)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: q and dst must be F32 or F16", op);
     if (dst->ne[0] != q->ne[0] || dst->ne[1] != q->ne[2] || dst->ne[2] != q->ne[1] || dst->ne[3] != q->ne[3])
-        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache_attn: dst must be [head_dim, n_head, n_q, n_seq]");
-    if (!rows_ok(q) || !rows_ok(dst)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache_attn: rows must be contiguous and aligned to their type");
-    if (!rows_fit(q) || q->ne[2] > 65535 || q->ne[1] > INT_MAX / 2) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache_attn: sizes beyond the launch limits");
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: dst must be [head_dim, n_head, n_q, n_seq]", op);
+    if (!rows_ok(dst)) return fail(ctx, MI355_STATUS_UNSUPPORTED, "%s: rows must be contiguous and aligned to their type", op);
     return MI355_STATUS_SUCCESS;
 }
 
@@ -220,6 +272,35 @@ KvAttnPlan attn_plan(const mi355_context* ctx, const mi355_kv_cache* c, const mi
                      int window) {
     return kv_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, window, c->head_dim,
                         q->type == T_F16, ctx->cus);
+}
+
+Kv4AttnPlan attn4_plan(const mi355_context* ctx, const mi355_kv_cache4* c, const mi355_kv_seqs* s, const mi355_tensor* q,
+                       int window) {
+    return kv4_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, window, c->head_dim,
+                         q->type == T_F16, ctx->cus);
+}
+
+// The arguments that the 4-bit cache's attention and its weights' sums share, checked
+mi355_status attn4_args(mi355_context* ctx, const char* op, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
+                        const int32_t* n_q, float scale, int causal, int32_t window, float* lse, Kv4AttnArgs* a) {
+    if ((reinterpret_cast<uintptr_t>(n_q) | reinterpret_cast<uintptr_t>(lse)) & 3)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: n_q and lse must be 4-byte aligned", op);
+    if (!std::isfinite(scale) || window < 0 || (causal | 1) != 1)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "%s: scale must be finite, window not negative, causal 0 or 1", op);
+    if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "%s: null context", op);
+    *a = Kv4AttnArgs{};
+    a->c = kv4_view(cache, seqs);
+    if (cache->n_blocks == 0) a->c.max_blocks = 0;  // nothing to attend to
+    a->q = static_cast<const char*>(q->data);
+    strides(q, a->q_nb);
+    a->n_q = (int)q->ne[1]; a->heads = (int)q->ne[2];
+    a->group = a->heads / cache->n_head_kv;
+    a->nq = n_q;
+    a->scale = scale; a->causal = causal;
+    a->window = window < 1 << 30 ? window : 1 << 30;
+    a->q16 = q->type == T_F16;
+    a->lse = lse;
+    return MI355_STATUS_SUCCESS;
 }
 
 }  // namespace
@@ -324,7 +405,7 @@ mi355_status mi355_kv_cache_read(mi355_context* ctx, const mi355_kv_cache* cache
 }
 
 int mi355_supports_kv_cache_attn(const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q, const mi355_tensor* dst) {
-    return check_attn(nullptr, cache, seqs, q, dst) == MI355_STATUS_SUCCESS;
+    return check_attn(nullptr, "kv_cache_attn", cache, seqs, q, dst) == MI355_STATUS_SUCCESS;
 }
 
 size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs,
@@ -335,7 +416,7 @@ size_t mi355_kv_cache_attn_workspace_size(const mi355_context* ctx, const mi355_
 
 mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                                  const int32_t* n_q, float scale, int causal, int32_t window, const mi355_tensor* dst) {
-    const mi355_status st = check_attn(ctx, cache, seqs, q, dst);
+    const mi355_status st = check_attn(ctx, "kv_cache_attn", cache, seqs, q, dst);
     if (st != MI355_STATUS_SUCCESS) return st;
     if (reinterpret_cast<uintptr_t>(n_q) & 3) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache_attn: n_q must be 4-byte aligned");
     if (!std::isfinite(scale) || window < 0 || (causal | 1) != 1)
@@ -364,6 +445,148 @@ mi355_status mi355_kv_cache_attn(mi355_context* ctx, const mi355_kv_cache* cache
     a.arrived = static_cast<uint32_t*>(ctx->arrived);
     Timed tm(ctx, p.nt == 0 ? "kv_cache_attn_128" : p.nt == 2 ? "kv_cache_attn_32" : "kv_cache_attn_16");  // by the rows of a workgroup
     return hip_check(ctx, tm.done(launch_kv_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache_attn launch");
+}
+
+int mi355_supports_qk_norm_rope(const mi355_tensor* q, const mi355_tensor* k, const mi355_rope_params* p, const mi355_tensor* q_dst,
+                                const mi355_tensor* k_dst) {
+    return check_qk_norm_rope(nullptr, q, k, p, q_dst, k_dst, nullptr) == MI355_STATUS_SUCCESS;
+}
+
+mi355_status mi355_qk_norm_rope(mi355_context* ctx, const mi355_tensor* q, const mi355_tensor* k, const float* q_w, const float* k_w,
+                                float eps, const int32_t* pos, const mi355_rope_params* p, const mi355_tensor* q_dst,
+                                const mi355_tensor* k_dst) {
+    QkArgs a;
+    const mi355_status st = check_qk_norm_rope(ctx, q, k, p, q_dst, k_dst, &a.r);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if ((reinterpret_cast<uintptr_t>(q_w) | reinterpret_cast<uintptr_t>(k_w)) & 3)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: weights must be 4-byte aligned");
+    if (!(eps >= 0.0f)) return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: eps must not be negative");
+    if ((!pos && !((!q || empty(q)) && (!k || empty(k)))) || (reinterpret_cast<uintptr_t>(pos) & 3))
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: pos null or not 4-byte aligned");
+    if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "qk_norm_rope: null context");
+    (void)hipSetDevice(ctx->device);
+    const mi355_tensor *one = q ? q : k, *out = q ? q_dst : k_dst;
+    auto side = [](const mi355_tensor* x, const mi355_tensor* y, const float* w) {
+        QkArgs::Side z{};
+        if (!x || empty(x)) return z;
+        z.src = static_cast<const char*>(x->data);
+        z.dst = static_cast<char*>(y->data);
+        strides(x, z.s_nb);
+        strides(y, z.d_nb);
+        z.w = w;
+        z.heads = (int)x->ne[1];
+        return z;
+    };
+    a.q = side(q, q_dst, q_w);
+    a.k = side(k, k_dst, k_w);
+    a.r.ne0 = (int)one->ne[0]; a.r.tokens = (int)one->ne[2]; a.r.batch = (int)one->ne[3];
+    a.r.pairs = p->n_dims / 2;
+    a.r.halves = p->pairs == MI355_ROPE_HALVES;
+    a.r.pos = pos;
+    a.eps = eps;
+    a.s16 = one->type == T_F16; a.d16 = out->type == T_F16;
+    Timed tm(ctx, "qk_norm_rope");
+    return hip_check(ctx, tm.done(launch_qk_norm_rope(a, ctx->stream)), "qk_norm_rope launch");
+}
+
+mi355_status mi355_kv_cache4_write(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* k,
+                                   const mi355_tensor* v, const int32_t* n_new) {
+    mi355_status st = check_cache<8>(ctx, "kv_cache4_write", cache, seqs);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (!k || !v) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_write: null argument");
+    KvRows r;
+    st = kv_rows(ctx, "kv_cache4_write", cache, seqs, k, v, n_new, &r);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_write: null context");
+    (void)hipSetDevice(ctx->device);
+    Timed tm(ctx, "kv_cache4_write");
+    return hip_check(ctx, tm.done(launch_kv4_write(kv4_view(cache, seqs), r, cache->head_dim, ctx->stream)), "kv_cache4_write launch");
+}
+
+mi355_status mi355_kv_cache4_read(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const int32_t* pos,
+                                  const mi355_tensor* k, const mi355_tensor* v) {
+    mi355_status st = check_cache<8>(ctx, "kv_cache4_read", cache, seqs);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (!k && !v) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_read: neither k nor v");
+    KvRows r;
+    st = kv_rows(ctx, "kv_cache4_read", cache, seqs, k, v, pos, &r);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_read: null context");
+    (void)hipSetDevice(ctx->device);
+    Timed tm(ctx, "kv_cache4_read");
+    return hip_check(ctx, tm.done(launch_kv4_read(kv4_view(cache, seqs), r, cache->head_dim, ctx->stream)), "kv_cache4_read launch");
+}
+
+int mi355_supports_kv_cache4_attn(const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q, const mi355_tensor* dst) {
+    return check_attn<8>(nullptr, "kv_cache4_attn", cache, seqs, q, dst) == MI355_STATUS_SUCCESS;
+}
+
+size_t mi355_kv_cache4_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                           const mi355_tensor* q, int32_t window) {
+    if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
+    return attn4_plan(ctx, cache, seqs, q, window).bytes;
+}
+
+mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
+                                  const int32_t* n_q, float scale, int causal, int32_t window, const mi355_tensor* dst, float* lse) {
+    const mi355_status st = check_attn<8>(ctx, "kv_cache4_attn", cache, seqs, q, dst);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    Kv4AttnArgs a;
+    const mi355_status sa = attn4_args(ctx, "kv_cache4_attn", cache, seqs, q, n_q, scale, causal, window, lse, &a);
+    if (sa != MI355_STATUS_SUCCESS) return sa;
+    a.dst = static_cast<char*>(dst->data);
+    strides(dst, a.d_nb);
+    a.d16 = dst->type == T_F16;
+    if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
+    (void)hipSetDevice(ctx->device);
+    const Kv4AttnPlan p = attn4_plan(ctx, cache, seqs, q, a.window);
+    mi355_status ws = p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
+    if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes, false);
+    if (ws != MI355_STATUS_SUCCESS) return ws;
+    a.part = static_cast<float*>(ctx->ws);
+    a.arrived = static_cast<uint32_t*>(ctx->arrived);
+    Timed tm(ctx, "kv_cache4_attn_16");
+    return hip_check(ctx, tm.done(launch_kv4_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache4_attn launch");
+}
+
+mi355_status mi355_kv_cache4_weights(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
+                                     const int32_t* n_q, const float* lse, float scale, int causal, int32_t window, float* sums) {
+    const mi355_status st = check_queries<8>(ctx, "kv_cache4_weights", cache, seqs, q);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    Kv4AttnArgs a;
+    const mi355_status sa = attn4_args(ctx, "kv_cache4_weights", cache, seqs, q, n_q, scale, causal, window, const_cast<float*>(lse), &a);
+    if (sa != MI355_STATUS_SUCCESS) return sa;
+    if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0 || a.c.max_blocks == 0) return MI355_STATUS_SUCCESS;
+    if (!lse || !sums) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_weights: null argument");
+    if (reinterpret_cast<uintptr_t>(sums) & 3) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_weights: sums must be 4-byte aligned");
+    (void)hipSetDevice(ctx->device);
+    Timed tm(ctx, "kv_cache4_weights");
+    return hip_check(ctx, tm.done(launch_kv4_weights(a, sums, cache->head_dim, ctx->stream)), "kv_cache4_weights launch");
+}
+
+mi355_status mi355_kv_cache4_evict(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const float* sums,
+                                   const int32_t* n_keep, int32_t max_keep, int32_t first, int32_t recent, float* sums_out,
+                                   int32_t* kept, int32_t* n_out) {
+    const mi355_status st = check_cache<8>(ctx, "kv_cache4_evict", cache, seqs);
+    if (st != MI355_STATUS_SUCCESS) return st;
+    if (max_keep < 0 || first < 0 || recent < 0)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: max_keep, first and recent must not be negative");
+    if (seqs->n_seq && (!n_out || (seqs->max_blocks && (!sums || !sums_out || (max_keep && !kept)))))
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: null argument");
+    if ((reinterpret_cast<uintptr_t>(sums) | reinterpret_cast<uintptr_t>(sums_out) | reinterpret_cast<uintptr_t>(n_keep) |
+         reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(n_out)) & 3)
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: sums, counts and kept must be 4-byte aligned");
+    if (seqs->n_seq && (n_out == seqs->n_kv || n_out == n_keep || (sums && sums == sums_out)))
+        return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: outputs must not be the inputs");
+    if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: null context");
+    (void)hipSetDevice(ctx->device);
+    Kv4EvictArgs a;
+    a.c = kv4_view(cache, seqs);
+    a.sums = sums; a.sums_out = sums_out;
+    a.n_keep = n_keep; a.max_keep = max_keep; a.first = first; a.recent = recent;
+    a.kept = kept; a.n_out = n_out;
+    Timed tm(ctx, "kv_cache4_evict");
+    return hip_check(ctx, tm.done(launch_kv4_evict(a, cache->head_dim, ctx->stream)), "kv_cache4_evict launch");
 }
 
 }  // extern "C"

@@ -4,6 +4,8 @@
 // pos * turn modulo 2^64 is the angle modulo a turn; turn itself is good to 2^-61 (rope_table), so
 // the angle to 2^-30 of a turn at the ends of int32.  What is left within an eighth of a turn is a
 // fp32 angle for two Taylor series.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -195,6 +197,135 @@ hipError_t launch_rope_multi(const RopeArgs& a, hipStream_t st) {
     if (a.f16) a.halves ? rope_go<true, true>(a, pieces, st) : rope_go<true, false>(a, pieces, st);
     else a.halves ? rope_go<false, true>(a, pieces, st) : rope_go<false, false>(a, pieces, st);
     return hipGetLastError();
+}
+
+// The norm of a head and its rotation in one pass: y = turned(x / sqrt(mean(x^2) + eps) * w).
+// G lanes to a head, four pairs or eight elements behind them each; a thread's H heads share its angles and weights.
+// Queries and keys are one list of heads, H neighbours at a time, so that each thread has heads of one side.  The squares
+// and their sum are fp32, in a tree over the lanes.  Bound by memory, every element moving once.
+template <bool S16, bool D16, bool HALVES, int G, int H>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs a, const int qb, const int blocks, const int64_t items) {
+    const RopeArgs& p = a.r;
+    const int c = threadIdx.x % G;
+    const int64_t at = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G, i = min(at, items - 1);  // (all lanes take part in the sums)
+    const int bt = (int)(i / blocks), hb = (int)(i - (int64_t)bt * blocks);
+    const int b = bt / p.tokens, t = bt - b * p.tokens;
+    const bool key = hb >= qb;
+    const QkArgs::Side& z = key ? a.k : a.q;
+    const int h0 = H * (key ? hb - qb : hb);
+    const char* src = z.src + t * z.s_nb[1] + b * z.s_nb[2];
+    char* dst = z.dst + t * z.d_nb[1] + b * z.d_nb[2];
+    const int turning = (p.pairs + 3) / 4, p0 = 4 * c, rest = 2 * p.pairs + 8 * (c - turning);
+    constexpr int SS = S16 ? 2 : 4, DS = D16 ? 2 : 4;
+    const bool turn = c < turning;
+    // elements of this lane: two runs of four (HALVES) or one of eight, whole or some; behind the pairs one of eight
+    const int e0 = turn ? (HALVES ? p0 : 2 * p0) : rest, e1 = turn && HALVES ? p0 + p.pairs : e0 + 4;
+    const int n0 = turn ? (HALVES ? min(max(p.pairs - p0, 0), 4) : min(max(2 * (p.pairs - p0), 0), 8)) : min(max(p.ne0 - rest, 0), 8);
+    const bool whole = turn ? p0 + 4 <= p.pairs : n0 == 8;
+    // element j of the lane's eight, and whether there is one
+    auto elem = [&](int j) { return j < 4 ? e0 + j : e1 + j - 4; };
+    auto is = [&](int j) { return turn && HALVES ? (j & 3) < n0 : j < n0; };
+    float x[H][8], w[8];
+    auto fetch = [&](const char* s, float (&v)[8]) {
+        if (whole) {
+            float lo[4], hi[4];
+            rope_ld<S16, 4>(s + SS * e0, lo);
+            rope_ld<S16, 4>(s + SS * e1, hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = is(j) ? rope_ld1<S16>(s, elem(j)) : 0.0f;
+        }
+    };
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[k][j] = 0.0f;
+        if (h0 + k < z.heads) fetch(src + (h0 + k) * z.s_nb[0], x[k]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = z.w && is(j) ? z.w[elem(j)] : 1.0f;
+    float cs[4], sn[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int pr = min(p0 + j, p.pairs - 1);
+        const int pos = p.pos[(int64_t)p.axis[pr] * p.batch * p.tokens + bt];
+        turn_sincos((uint64_t)(int64_t)pos * p.turn[pr], cs[j], sn[j]);
+    }
+    const float per = 1.0f / (float)p.ne0;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = __builtin_fmaf(x[k][j], x[k][j], s);
+        if constexpr (G >= 2) s += lane_swap_f<1>(s);
+        if constexpr (G >= 4) s += lane_swap_f<2>(s);
+        if constexpr (G >= 8) s += lane_swap_f<4>(s);
+        if constexpr (G >= 16) s += lane_swap_f<8>(s);
+        if constexpr (G >= 32) s += lane_swap_f<16>(s);
+        if constexpr (G >= 64) s += lane_swap_f<32>(s);
+        const float f = 1.0f / sqrtf(s * per + a.eps);
+        float v[8], y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = v[j] = x[k][j] * f * w[j];
+        if (turn) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                constexpr int A = HALVES ? 1 : 2, B = HALVES ? 4 : 1;  // pair j: elements A j and A j + B of the eight
+                y[A * j] = v[A * j] * cs[j] - v[A * j + B] * sn[j];
+                y[A * j + B] = v[A * j] * sn[j] + v[A * j + B] * cs[j];
+            }
+        }
+        if (at >= items || h0 + k >= z.heads) continue;
+        char* d = dst + (h0 + k) * z.d_nb[0];
+        if (whole) {
+            const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
+            rope_st<D16, 4>(d + DS * e0, lo);
+            rope_st<D16, 4>(d + DS * e1, hi);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (is(j)) rope_st1<D16>(d, elem(j), y[j]);
+        }
+    }
+}
+
+template <bool S16, bool D16, bool HALVES>
+static hipError_t qk_go(const QkArgs& a, hipStream_t st) {
+    const RopeArgs& p = a.r;
+    const int pieces = (p.pairs + 3) / 4 + (p.ne0 - 2 * p.pairs + 7) / 8;
+    const int64_t bt = (int64_t)p.tokens * p.batch;
+    const int qh = a.q.src ? a.q.heads : 0, kh = a.k.src ? a.k.heads : 0;
+    auto go = [&](auto g, auto hh) {
+        constexpr int G = decltype(g)::value, H = decltype(hh)::value;
+        const int qb = (qh + H - 1) / H, blocks = qb + (kh + H - 1) / H;
+        const int64_t items = bt * blocks, wgs = (items + 256 / G - 1) / (256 / G);
+        if (items <= 0) return hipSuccess;
+        if (wgs > INT32_MAX) return hipErrorInvalidValue;
+        qk_norm_rope_kernel<S16, D16, HALVES, G, H><<<(unsigned)wgs, 256, 0, st>>>(a, qb, blocks, items);
+        return hipGetLastError();
+    };
+    auto heads = [&](auto g) {
+        // four heads to a thread where that leaves enough threads to occupy the CUs
+        if (bt * ((qh + 3) / 4 + (kh + 3) / 4) * decltype(g)::value >= 1 << 17) return go(g, std::integral_constant<int, 4>());
+        return go(g, std::integral_constant<int, 1>());
+    };
+    if (pieces <= 8) return heads(std::integral_constant<int, 8>());
+    if (pieces <= 16) return heads(std::integral_constant<int, 16>());
+    if (pieces <= 32) return heads(std::integral_constant<int, 32>());
+    if (pieces <= 64) return heads(std::integral_constant<int, 64>());
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_qk_norm_rope(const QkArgs& a, hipStream_t st) {
+    const bool hv = a.r.halves;
+    if (a.s16) {
+        if (a.d16) return hv ? qk_go<true, true, true>(a, st) : qk_go<true, true, false>(a, st);
+        return hv ? qk_go<true, false, true>(a, st) : qk_go<true, false, false>(a, st);
+    }
+    if (a.d16) return hv ? qk_go<false, true, true>(a, st) : qk_go<false, true, false>(a, st);
+    return hv ? qk_go<false, false, true>(a, st) : qk_go<false, false, false>(a, st);
 }
 
 }  // namespace mi355
