@@ -413,7 +413,7 @@ struct Kv4AttnArgs {
     uint32_t* arrived;         // as KvAttnArgs'
 };
 struct Kv4AttnPlan {
-    int tiles;                 // workgroups over a sequence's rows
+    int rows, tiles;           // of a workgroup (16, or 128 whose ranges a second kernel joins), workgroups over a sequence's rows
     int splits;                // ranges of the tokens
     size_t bytes;              // of part
 };

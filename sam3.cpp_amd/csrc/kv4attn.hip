@@ -17,6 +17,7 @@ constexpr float KV4_LOG2E = 1.44269504088896340736f, KV4_LN2 = 0.693147180559945
 constexpr float KV4_NONE = -1e30f;   // a reference that nothing has been taken against yet
 constexpr float KV4_LIFT = 12.0f;    // probabilities are raised by 2^12 to keep small ones in fp16's normal range
 constexpr float KV4_ROOM = 15.0f;    // and their reference moves when one would pass 2^15
+constexpr float KV4_LIFT_SUM = 8.0f; // the same where a lane's sum of 32 of them, and not each, is held below 2^15
 constexpr int KV4_RANGES = 64;       // ranges of a row that one workgroup joins, at most
 }  // namespace
 
@@ -173,6 +174,52 @@ __device__ __forceinline__ char* out_at(const Kv4AttnArgs& a, int64_t pr) {
 __device__ __forceinline__ void put_four(const Kv4AttnArgs& a, char* out, int e, v4f y) {
     if (a.d16) *reinterpret_cast<v4h_a2*>(out + 2 * e) = __builtin_convertvector(y, v4h);
     else *reinterpret_cast<v4f_a4*>(out + 4 * e) = y;
+}
+
+// Four elements from e on of row pr, joined from the row's n ranges in the ranges' order and written.  ONE: other workgroups
+// of this launch wrote the partial sums.
+template <int D, bool ONE>
+__device__ __forceinline__ void join_ranges(const Kv4AttnArgs& a, int splits, int n, int64_t pr, int e) {
+    const int64_t all = (int64_t)a.c.n_seq * a.n_q * a.heads;
+    const float* ml = a.part + (int64_t)splits * all * D + pr * 4;
+    const float* po = a.part + pr * D + e;
+    auto get = [](const float* q) {
+        if constexpr (!ONE) return *reinterpret_cast<const v4f*>(q);
+        const v2f lo = get_through(q), hi = get_through(q + 2);
+        return v4f{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int B = 8;  // ranges whose loads are on their way together
+    float m = KV4_NONE, l = 0.0f, la = 0.0f;
+    v4f o = {0, 0, 0, 0};
+    for (int x0 = 0; x0 < n; x0 += B) {
+        v4f z[B], y[B];
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            z[x] = v4f{KV4_NONE, 0, 0, 0};
+            y[x] = v4f{0, 0, 0, 0};
+            if (x0 + x < n) {
+                z[x] = get(ml + (x0 + x) * all * 4);
+                y[x] = get(po + (x0 + x) * all * D);
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int x = 0; x < B; ++x) mn = fmaxf(mn, z[x][0]);
+        const float old = __builtin_amdgcn_exp2f(m - mn);
+        l *= old;
+        la *= old;
+        o = o * old;
+        m = mn;
+#pragma unroll
+        for (int x = 0; x < B; ++x) {
+            const float up = __builtin_amdgcn_exp2f(z[x][0] - m);
+            l += z[x][1] * up;
+            la += z[x][2] * up;
+            o = o + y[x] * up;
+        }
+    }
+    put_four(a, out_at(a, pr), e, o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (e == 0) put_lse(a, pr, m, la);
 }
 
 // A workgroup takes 16 rows and one range of the tokens, its four wavefronts every fourth step of 32 tokens; the cache's
@@ -400,46 +447,385 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
     if (!join) return;
     asm volatile("" ::: "memory");
     for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
-        const int y = i / (D / 4), e = 4 * (i % (D / 4));
-        const int64_t pr = number(y);
+        const int64_t pr = number(i / (D / 4));
         if (pr < 0) break;
-        constexpr int B = 8;  // ranges whose loads are on their way together
-        float m = KV4_NONE, l = 0.0f, la = 0.0f;
-        v4f o = {0, 0, 0, 0};
-        for (int x0 = 0; x0 < ranges; x0 += B) {
-            v2f z[B], lo[B], hi[B];
-            float za[B];
+        join_ranges<D, true>(a, splits, ranges, pr, 4 * (i % (D / 4)));
+    }
+}
+
+// Many query rows: a workgroup takes 128 rows in four wavefronts of 32 and streams the tokens through LDS in tiles of 64,
+// nibbles becoming halves once for all four on the way: a thread loads its words of a row ahead of time and
+// writes them after the previous tile's products.  Scores and output as fattn.hip's (v_mfma_f32_32x32x16_f16, S^T = K Q^T,
+// the probabilities' registers as the operand of O^T += V^T P^T, V^T by transposing reads); a tile's scores are
+// computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.
+//
+// V row slot of 16-byte chunk c in row r: c ^ this.  The transposing reads take four chunks from each of four rows, which lie
+// in distinct quarters of the banks (as fattn.hip's vswz); with heads of 128 the chunks are turned within their
+// quarter too, so that the sixteen lanes of a write, four rows of four quarters, take distinct banks.
+template <int D>
+__device__ __forceinline__ int v4swz(int r) { return D == 128 ? 5 * (r & 3) : vswz<D>(r); }
+
+template <int D, bool QS, bool PS>
+__global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, const int splits, const int tiles) {
+    constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
+    constexpr bool AHEAD = !((QS && D > 64) || (PS && D > 96));  // scores a tile ahead; else the second halves have their registers
+    constexpr int NW = D / 32;                      // words of a thread, together where a row's are a power of two
+    constexpr int VW = D == 96 ? 1 : NW, NV = NW / VW, G = D / 32;
+    __shared__ __attribute__((aligned(16))) _Float16 sK[2][64 * D];
+    __shared__ __attribute__((aligned(16))) _Float16 sV[2][64 * D];
+    const Kv4View& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Eight items (one to an XCD, whose bytes stay in its L2) at a time, and of them the last row tiles
+    // first: causal ones are the longest.
+    const int items = splits * c.heads * c.n_seq, first = blockIdx.x / (8 * tiles) * 8, left = blockIdx.x - first * tiles;
+    const int many = min(8, items - first), item = first + left % many, tile = tiles - 1 - left / many;
+    const int sp = item % splits, hk = item / splits % c.heads, s = item / splits / c.heads;
+    const KvRange kr = kv_range(a, s);
+    const int rows = kr.nq * a.group, row0 = tile * 128;
+    if (row0 >= rows) return;
+    const int chunk = kv_chunk(kr, splits);
+    if (sp > 0 && kr.lo + sp * chunk >= kr.hi) return;
+    const int iq_first = row0 / a.group, iq_last = (min(row0 + 128, rows) - 1) / a.group;
+    const int lo_tile = a.window > 0 ? max(kr.pos0 + iq_first - a.window + 1, 0) & ~63 : 0;
+    const int tb = max(kr.lo + sp * chunk, lo_tile);  // (a multiple of 32: blocks are met at 16-token steps)
+    const int te = min(min(kr.lo + sp * chunk + chunk, kr.hi), a.causal ? kr.pos0 + iq_last + 1 : kr.hi);
+
+    // this lane's query row
+    const int r = row0 + 32 * w + lr, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
+    const bool on = r < rows;
+    const int pos = kr.pos0 + iq;
+    const int see_hi = on ? (a.causal ? min(pos + 1, te) : te) : 0, see_lo = a.window > 0 ? pos - a.window + 1 : 0;
+    // tokens that every row of the wavefront sees (rows past the last one see what they like)
+    const int iq0 = __builtin_amdgcn_readfirstlane(iq), iq31 = min(__builtin_amdgcn_readlane(iq, 31), iq_last);
+    const int all_hi = a.causal ? min(kr.pos0 + iq0 + 1, te) : te, all_lo = a.window > 0 ? kr.pos0 + iq31 - a.window + 1 : 0;
+    v8h q[NC], ql[QS ? NC : 1];
+    float qscale = a.scale < 0.0f ? -1.0f : 1.0f;
+    {
+        const char* p = row_at(a, s, iq, h);
+        if constexpr (QS) {
+            float top = 0.0f;
 #pragma unroll
-            for (int x = 0; x < B; ++x) {
-                z[x] = v2f{KV4_NONE, 0.0f};
-                za[x] = 0.0f;
-                lo[x] = hi[x] = v2f{0, 0};
-                if (x0 + x < ranges) {
-                    z[x] = get_through(ml + ((x0 + x) * all + pr) * 4);
-                    if (e == 0) za[x] = get_through(ml + ((x0 + x) * all + pr) * 4 + 2)[0];
-                    lo[x] = get_through(a.part + ((x0 + x) * all + pr) * D + e);
-                    hi[x] = get_through(a.part + ((x0 + x) * all + pr) * D + e + 2);
+            for (int m = 0; m < NC; ++m)
+                if (on) {
+                    const v4f x0 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g)), x1 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g) + 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fabsf(x0[j]), fabsf(x1[j])));
+                }
+            const Pow2 z = pow2_of(xmax32(top));
+            const float down = z.down * qscale;
+            qscale = z.up;
+#pragma unroll
+            for (int m = 0; m < NC; ++m) {
+                v4f x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+                if (on) {
+                    x0 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g)) * down;
+                    x1 = *reinterpret_cast<const v4f_a4*>(p + 4 * (16 * m + 8 * g) + 16) * down;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float y = j < 4 ? x0[j & 3] : x1[j & 3];
+                    q[m][j] = (_Float16)y;
+                    ql[m][j] = (_Float16)(y - (float)q[m][j]);
                 }
             }
-            float mn = m;
+        } else {
 #pragma unroll
-            for (int x = 0; x < B; ++x) mn = fmaxf(mn, z[x][0]);
-            const float old = __builtin_amdgcn_exp2f(m - mn);
-            l *= old;
-            la *= old;
-            o = o * old;
-            m = mn;
+            for (int m = 0; m < NC; ++m) {
+                const v8h z = {0, 0, 0, 0, 0, 0, 0, 0};
+                q[m] = on ? *reinterpret_cast<const v8h_a2*>(p + 2 * (16 * m + 8 * g)) : z;
+                if (a.scale < 0.0f) q[m] = -q[m];
+            }
+            qscale = 1.0f;
+        }
+    }
+    const float f = fmaxf(fabsf(a.scale) * KV4_LOG2E * qscale, 1e-37f);  // (0 times a hidden score)
+
+    int tile0 = 0;  // the step's tile
+    // blocks of 16 tokens each, of the sixteen tiles that the step's tile is of, and of the sixteen after
+    int cur = -1, nxt = -1;
+    auto group_of = [&](int t) { return kv4_block(c, s, tb + 64 * t + 16 * lane); };
+    auto staged = [&](int t) {  // block of this wavefront's 16 rows of a tile of this or the next sixteen
+        const int i = 4 * (t & 15) + w;
+        return max((t >> 4) == (tile0 >> 4) ? __builtin_amdgcn_readlane(cur, i) : __builtin_amdgcn_readlane(nxt, i), 0);
+    };
+    // staging: wavefront w takes rows 16 w .. + 15 of a tile, unit j of a lane words VW (u % UR) on of row u / UR, u = lane + 64 j
+    constexpr int UR = D / 8 / VW;
+    typedef uint32_t unit_t __attribute__((ext_vector_type(VW == 1 ? 1 : VW)));
+    struct Staged {
+        unit_t x[NV];
+        uint16_t d[NV];
+    } kreg, vreg;
+    auto load_one = [&](bool val, Staged& z, int t) {
+        const int64_t at = ((int64_t)staged(t) * c.heads + hk) * c.bt;
+        const int in = (tb + 64 * t + 16 * w) & (c.bt - 1);
+        const uint8_t* p = (val ? c.v : c.k) + (at + in) * (D / 2);
 #pragma unroll
-            for (int x = 0; x < B; ++x) {
-                const float y2 = __builtin_amdgcn_exp2f(z[x][0] - m);
-                l += z[x][1] * y2;
-                la += za[x] * y2;
-                o = o + v4f{lo[x][0], lo[x][1], hi[x][0], hi[x][1]} * y2;
+        for (int j = 0; j < NV; ++j) {
+            const int u = lane + 64 * j, row = u / UR, grp = u % UR * VW / 4;
+            z.x[j] = *reinterpret_cast<const unit_t*>(p + 4 * VW * u);
+            z.d[j] = val ? c.v_scale[at * G + grp * c.bt + in + row] : c.k_scale[(at + in + row) * G + grp];
+        }
+    };
+    // LDS addresses: a row's bytes are a power of two (D = 96: are added afterwards), so that a chunk further on is one
+    // exclusive or away.
+    int kst[NV], vst[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int u = lane + 64 * j, row = 16 * w + u / UR, chunk8 = VW * (u % UR);
+        kst[j] = row * 2 * D + 16 * (chunk8 ^ kswz<D>(row));
+        vst[j] = row * 2 * D + 16 * (chunk8 ^ v4swz<D>(row));
+    }
+    auto store8 = [&](bool val, _Float16* lds, const Staged& z, int i) {
+        const int j = i / VW, e = i % VW;
+        // (values of no scale: their token's scores are NaN or hidden)
+        const uint16_t d16 = val ? (uint16_t)finite_scales(z.d[j]) : z.d[j];
+        const _Float16 d = __builtin_bit_cast(_Float16, d16);
+        uint32_t o[4];
+        word_halves(z.x[j][e], h2v{d, d}, o);
+        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(lds) + ((val ? vst[j] : kst[j]) ^ (16 * e))) = u32x4{o[0], o[1], o[2], o[3]};
+    };
+    auto store_one = [&](bool val, _Float16* lds, const Staged& z) {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) store8(val, lds, z, i);
+    };
+    const int krow = lr * 2 * D, kchunk = 16 * (g ^ kswz<D>(lr));
+    auto key_frag = [&](const _Float16* lds, int pre, int m, int kh) {
+        const int at = D == 96 ? krow + (pre ^ (32 * m)) : pre ^ (32 * m);
+        return *reinterpret_cast<const v8h*>(reinterpret_cast<const char*>(lds) + at + kh * 64 * D);
+    };
+    const int kpre = D == 96 ? kchunk : krow + kchunk;
+    const int vrow = 4 * g + ((lane & 15) >> 2), vpre = vrow * 2 * D + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v4swz<D>(vrow)) + 8 * (lane & 1);
+
+    v16f O[NDB];
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) O[i][e] = 0.0f;
+    float m_ref = KV4_NONE, l_sum = 0.0f, l_all = 0.0f;
+    auto score = [&](const _Float16* lds, v16f* S) {
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        S[0] = S[1] = z;
+#pragma unroll
+        for (int m = 0; m < NC; ++m)
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                const v8h k8 = key_frag(lds, kpre, m, kh);
+                S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, q[m], S[kh], 0, 0, 0);
+                if constexpr (QS) S[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[m], S[kh], 0, 0, 0);
+            }
+    };
+    // The token of score i of group j from the lane's first one of the tile.
+    auto token = [](int j, int i) { return 32 * (j >> 1) + 16 * (j & 1) + 8 * (i >> 2) + (i & 3); };
+    // Probabilities of a tile from its scores, at the reference as it stands: pair n of its sixteen
+    uint32_t P[2][8], PL[2][PS ? 8 : 1];
+    struct Sums {
+        float s, all;
+    };
+    auto pair = [&](const v16f* S, int n, Sums& sums) {
+        const v16f& x = S[n >> 3];
+        const int i = 2 * (n & 7);
+        const v2f p = {__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], f, -m_ref)), __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], f, -m_ref))};
+        const h2v ph = __builtin_convertvector(p, h2v), ones = {(_Float16)1.0f, (_Float16)1.0f};
+        P[n >> 3][n & 7] = __builtin_bit_cast(uint32_t, ph);
+        if constexpr (PS) {
+            const h2v pl = __builtin_convertvector((v2f{p[0] - (float)ph[0], p[1] - (float)ph[1]}), h2v);
+            PL[n >> 3][n & 7] = __builtin_bit_cast(uint32_t, pl);
+            sums.s += p[0] + p[1];
+        } else {
+            sums.s = __builtin_amdgcn_fdot2(ph, ones, sums.s, false);
+            if (a.lse) sums.all += p[0] + p[1];
+        }
+    };
+    // What is left when a tile's pairs are done: the sums, and the reference where it has to move.
+    auto settle = [&](const v16f* S, Sums& sums) {
+        if (__builtin_amdgcn_ballot_w64(!(sums.s <= 32768.0f))) {
+            // some probability is too large, or may be: the reference moves to the tile's own largest
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, S[kh][i] * f);
+            const float mn = fmaxf(m_ref, xmax32(top) - KV4_LIFT_SUM), am = __builtin_amdgcn_exp2f(m_ref - mn);
+            m_ref = mn;
+            l_sum *= am;
+            l_all *= am;
+#pragma unroll
+            for (int b = 0; b < NDB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) O[b][e] *= am;
+            sums = Sums{0.0f, 0.0f};
+#pragma unroll
+            for (int n = 0; n < 16; ++n) pair(S, n, sums);
+        }
+        l_sum += sums.s;
+        l_all += sums.all;
+    };
+    // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
+    // a product's fragments are read while the product before multiplies, and pairs go between the products.
+    auto score_softmax = [&](const _Float16* lds, v16f* Sn, const v16f* S) {
+        int pre = kpre;
+        asm volatile("" : "+v"(pre));  // (the addresses are made here: kept over the loop, they would push the queries out)
+        const v16f z = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        v8h k8[2], k8n[2];
+        auto frag = [&](int m, v8h* o) {
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) o[kh] = key_frag(lds, pre, m, kh);
+        };
+        if constexpr (QS) __builtin_amdgcn_s_setprio(1);
+        frag(0, k8);
+        Sn[0] = Sn[1] = z;
+        Sums sums = {0.0f, 0.0f};
+#pragma unroll
+        for (int m = 0; m < NC; ++m) {
+            if (m + 1 < NC) frag(m + 1, k8n);
+#pragma unroll
+            for (int kh = 0; kh < 2; ++kh) {
+                Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], q[m], Sn[kh], 0, 0, 0);
+                if constexpr (QS) Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], ql[m], Sn[kh], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 16 * m / NC; n < 16 * (m + 1) / NC; ++n) pair(S, n, sums);
+            k8[0] = k8n[0];
+            k8[1] = k8n[1];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (QS) __builtin_amdgcn_s_setprio(0);
+        settle(S, sums);
+    };
+    // Scores of blocks that are not there are hidden, and so are those that a row does not see, before anything
+    // is made of them.
+    uint64_t off = 0;  // of the groups of cur
+    auto hide = [&](v16f* S, int t) {
+        const int t0 = tb + 64 * t + 4 * g, shift = 4 * (t & 15);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t n = off >> (shift + j) & 1 ? 0u : (uint32_t)max(see_hi - see_lo, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = S[j >> 1][8 * (j & 1) + i];
+                S[j >> 1][8 * (j & 1) + i] = (uint32_t)(token(j, i) + t0 - see_lo) < n ? x : -__builtin_inff();
             }
         }
-        put_four(a, out_at(a, pr), e, o * (l == 0.0f ? 0.0f : 1.0f / l));
-        if (e == 0) put_lse(a, pr, m, la);
+    };
+    // The output of the tile in lds, and the staged bytes of the next ones into their buffers between the products
+    auto output_store = [&](const _Float16* lds, _Float16* vnext, _Float16* knext) {
+        int pre = vpre;
+        asm volatile("" : "+v"(pre));
+        auto frag = [&](int i) {  // product i: 16 tokens i / NDB, output block i % NDB
+            const int b = i % NDB;
+            const char* vt = reinterpret_cast<const char*>(lds) + (D == 96 ? pre + 64 * b : pre ^ (64 * b)) + 16 * (i / NDB) * 2 * D;
+            const uint2 lo = lds_read_tr16(vt), hi = lds_read_tr16(vt + 8 * 2 * D);
+            return __builtin_bit_cast(v8h, (u32x4{lo.x, lo.y, hi.x, hi.y}));
+        };
+        v8h v8[2] = {frag(0), frag(1)}, v8n[2];
+        static_assert(NDB == NW, "a unit of both to two products");
+#pragma unroll
+        for (int x = 0; x < 2 * NDB; ++x) {
+            if (x + 1 < 2 * NDB) {
+                v8n[0] = frag(2 * x + 2);
+                v8n[1] = frag(2 * x + 3);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int i = 2 * x + y, kh = i / NDB / 2, hh = i / NDB & 1, b = i % NDB;
+                const u32x4 p = {P[kh][4 * hh], P[kh][4 * hh + 1], P[kh][4 * hh + 2], P[kh][4 * hh + 3]};
+                O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, p), O[b], 0, 0, 0);
+                if constexpr (PS) {
+                    const u32x4 e = {PL[kh][4 * hh], PL[kh][4 * hh + 1], PL[kh][4 * hh + 2], PL[kh][4 * hh + 3]};
+                    O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
+                }
+            }
+            if (x < NW) store8(true, vnext, vreg, x);
+            else store8(false, knext, kreg, x - NW);
+            v8[0] = v8n[0];
+            v8[1] = v8n[1];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    const int nt = te > tb ? (te - tb + 63) / 64 : 0;
+    if (nt > 0) {
+        // Step t: the scores of tile t + 1 beside the softmax of tile t (AHEAD; else its own before it), and its
+        // output; then the words of K(t + 2) (t + 1) and V(t + 1), loaded a step before, become halves in the buffers
+        // that step t - 1 read last.  One barrier a step.
+        cur = group_of(0);
+        nxt = group_of(16);
+        off = __builtin_amdgcn_ballot_w64(cur < 0);
+        v16f SA[2], SB[2];
+        load_one(false, kreg, 0);
+        store_one(false, sK[0], kreg);
+        load_one(true, vreg, 0);
+        store_one(true, sV[0], vreg);
+        load_one(false, kreg, 1);
+        if constexpr (AHEAD) {
+            store_one(false, sK[1], kreg);
+            load_one(false, kreg, 2);
+        }
+        load_one(true, vreg, 1);
+        __syncthreads();
+        if constexpr (AHEAD) score(sK[0], SA);
+        auto step = [&](int t, int cb, v16f* Sc, v16f* Sn) {
+            const int t0 = tb + 64 * t;
+            lds_barrier();
+            tile0 = t;
+            if ((t & 15) == 0 && t > 0) {
+                cur = nxt;
+                off = __builtin_amdgcn_ballot_w64(cur < 0);
+                nxt = group_of(t + 16);
+            }
+            if constexpr (!AHEAD) score(sK[cb], Sc);
+            if (t0 < all_lo || t0 + 64 > all_hi || ((off >> (4 * (t & 15))) & 15)) hide(Sc, t);
+            if constexpr (AHEAD) {
+                score_softmax(sK[cb ^ 1], Sn, Sc);
+            } else {
+                Sums sums = {0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < 16; ++n) pair(Sc, n, sums);
+                settle(Sc, sums);
+            }
+            output_store(sV[cb], sV[cb ^ 1], sK[AHEAD ? cb : cb ^ 1]);
+            load_one(true, vreg, t + 2);
+            load_one(false, kreg, t + (AHEAD ? 3 : 2));
+        };
+        for (int t = 0; t < nt; t += 2) {
+            step(t, 0, SA, AHEAD ? SB : SA);
+            if (t + 1 < nt) step(t + 1, 1, AHEAD ? SB : SA, SA);
+        }
     }
+
+    if (!on) return;
+    l_sum = xsum32(l_sum);
+    l_all = PS ? l_sum : xsum32(l_all);
+    const int64_t pr = ((int64_t)s * a.n_q + iq) * a.heads + h, all = (int64_t)c.n_seq * a.n_q * a.heads;
+    const float z = splits > 1 ? 1.0f : l_sum == 0.0f ? 0.0f : 1.0f / l_sum;
+    if (g == 0) {
+        if (splits > 1) *reinterpret_cast<v4f*>(a.part + (int64_t)splits * all * D + (sp * all + pr) * 4) = v4f{m_ref, l_sum, l_all, 0.0f};
+        else put_lse(a, pr, m_ref, l_all);
+    }
+    float* part = a.part + (sp * all + pr) * D;
+    char* out = out_at(a, pr);
+#pragma unroll
+    for (int b = 0; b < NDB; ++b)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            const int e = 32 * b + 8 * i4 + 4 * g;
+            const v4f y = v4f{O[b][4 * i4], O[b][4 * i4 + 1], O[b][4 * i4 + 2], O[b][4 * i4 + 3]} * z;
+            if (splits > 1) *reinterpret_cast<v4f*>(part + e) = y;
+            else put_four(a, out, e, y);
+        }
+}
+
+// The joins of kv4_tiles_kernel's ranges: thread per four elements of a row
+template <int D>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnArgs a, const int splits) {
+    constexpr int C4 = D / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pr = i / C4, all = (int64_t)a.c.n_seq * a.n_q * a.heads;
+    if (pr >= all) return;
+    const KvRange kr = kv_range(a, (int)(pr / a.heads / a.n_q));
+    if (pr / a.heads % a.n_q >= kr.nq) return;
+    const int chunk = kv_chunk(kr, splits);
+    join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), pr, (int)(i - pr * C4) * 4);
 }
 
 // ---- the weights' sums by token
@@ -523,36 +909,48 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(const Kv4AttnArgs a, f
     }
 }
 
-// The ranges of the tokens for n_q queries.
+// The kernel, its row tiles and the ranges of the tokens for n_q queries.
 Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus) {
     if (window > 0) max_tokens = std::min<int64_t>(max_tokens, (int64_t)window + n_q + KV_STEP);  // (kv_range)
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
     const int64_t steps = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);  // of 128 tokens
     cus = std::max(cus, 1);
     Kv4AttnPlan p;
-    p.tiles = (int)((rows + 15) / 16);
+    p.rows = rows > 64 ? 128 : 16;
+    p.tiles = (int)((rows + p.rows - 1) / p.rows);
     const int64_t wgs = items * p.tiles;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps, KV4_RANGES}));
-    if (wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps, p.rows == 16 ? KV4_RANGES : 32}));
+    if (p.rows == 16 && wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
     p.bytes = p.splits > 1 ? (size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 : 0;
     return p;
 }
 
+template <int D, bool QS, bool PS>
+static void kv4_attn_go(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
+    const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
+    if (p.rows == 16) kv4_rows_kernel<D, QS, PS><<<(unsigned)((items + 7) / 8 * 8 * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles);
+    else kv4_tiles_kernel<D, QS, PS><<<(unsigned)(items * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles);
+}
+
 template <int D>
 static hipError_t kv4_attn_d(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
-    const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
-    const unsigned n = (unsigned)((items + 7) / 8 * 8 * p.tiles);
-    if (a.q16 && a.d16) kv4_rows_kernel<D, false, false><<<n, 256, 0, st>>>(a, p.splits, p.tiles);
-    else if (a.q16) kv4_rows_kernel<D, false, true><<<n, 256, 0, st>>>(a, p.splits, p.tiles);
-    else if (a.d16) kv4_rows_kernel<D, true, false><<<n, 256, 0, st>>>(a, p.splits, p.tiles);
-    else kv4_rows_kernel<D, true, true><<<n, 256, 0, st>>>(a, p.splits, p.tiles);
+    if (a.q16 && a.d16) kv4_attn_go<D, false, false>(a, p, st);
+    else if (a.q16) kv4_attn_go<D, false, true>(a, p, st);
+    else if (a.d16) kv4_attn_go<D, true, false>(a, p, st);
+    else kv4_attn_go<D, true, true>(a, p, st);
+    if (p.rows != 16 && p.splits > 1) {
+        const int64_t n = (int64_t)a.c.n_seq * a.n_q * a.heads * (D / 4);
+        kv4_join_kernel<D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a, p.splits);
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hipStream_t st) {
     if ((int64_t)a.n_q * a.heads * a.c.n_seq <= 0) return hipSuccess;
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
-    if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || (p.splits > 1 && (!a.part || !a.arrived))) return hipErrorInvalidValue;
+    if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || (int64_t)a.n_q * a.heads * a.c.n_seq * (D / 4) > (int64_t)INT32_MAX * 256 ||
+        (p.splits > 1 && (!a.part || (p.rows == 16 && !a.arrived))))
+        return hipErrorInvalidValue;
     switch (D) {
         case 64: return kv4_attn_d<64>(a, p, st);
         case 96: return kv4_attn_d<96>(a, p, st);

@@ -540,12 +540,12 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
     if ((int64_t)a.n_q * a.heads * a.c.n_seq == 0) return MI355_STATUS_SUCCESS;
     (void)hipSetDevice(ctx->device);
     const Kv4AttnPlan p = attn4_plan(ctx, cache, seqs, q, a.window);
-    mi355_status ws = p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
+    mi355_status ws = p.rows == 16 && p.splits > 1 ? ensure_arrived(ctx) : MI355_STATUS_SUCCESS;
     if (ws == MI355_STATUS_SUCCESS) ws = ensure_ws(ctx, p.bytes, false);
     if (ws != MI355_STATUS_SUCCESS) return ws;
     a.part = static_cast<float*>(ctx->ws);
     a.arrived = static_cast<uint32_t*>(ctx->arrived);
-    Timed tm(ctx, "kv_cache4_attn_16");
+    Timed tm(ctx, p.rows == 16 ? "kv_cache4_attn_16" : "kv_cache4_attn_128");  // by the rows of a workgroup
     return hip_check(ctx, tm.done(launch_kv4_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache4_attn launch");
 }
 
