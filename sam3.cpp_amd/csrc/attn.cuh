@@ -58,15 +58,15 @@ constexpr int KV_SPAN = 4 * KV_STEP; // tokens of one step of a workgroup
 // The tokens that a sequence's queries can see, and its queries.
 struct KvRange {
     int n_kv, nq, pos0;  // length, queries, position of the first query
-    int lo, hi;          // tokens lo .. hi - 1 (lo a multiple of a step) are seen by some query
+    int lo, hi;          // tokens lo .. hi - 1 (lo a multiple of STEP) are seen by some query
 };
-template <class Args>
+template <int STEP = KV_STEP, class Args>
 __device__ __forceinline__ KvRange kv_range(const Args& a, int s) {
     KvRange r;
     r.n_kv = (int)min((int64_t)max(a.c.n_kv[s], 0), (int64_t)a.c.max_blocks * a.c.bt);
     r.nq = a.nq ? min(max(a.nq[s], 0), a.n_q) : a.n_q;
     r.pos0 = r.n_kv - r.nq;
-    r.lo = a.window > 0 ? (int)(max((int64_t)r.pos0 - a.window + 1, (int64_t)0) & ~(int64_t)(KV_STEP - 1)) : 0;
+    r.lo = a.window > 0 ? (int)(max((int64_t)r.pos0 - a.window + 1, (int64_t)0) & ~(int64_t)(STEP - 1)) : 0;
     r.hi = r.n_kv;
     return r;
 }

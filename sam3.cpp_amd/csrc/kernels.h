@@ -415,7 +415,9 @@ struct Kv4AttnArgs {
 struct Kv4AttnPlan {
     int rows, tiles;           // of a workgroup (16, or 128 whose ranges a second kernel joins), workgroups over a sequence's rows
     int splits;                // ranges of the tokens
-    size_t bytes;              // of part
+    bool pre;                  // whether the tokens' halves are made before, max_tiles of 64 tokens a sequence and key head,
+    int max_tiles;
+    size_t halves, bytes;      // at this offset from part; of both
 };
 Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hipStream_t st);

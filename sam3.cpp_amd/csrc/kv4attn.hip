@@ -18,6 +18,8 @@ constexpr float KV4_NONE = -1e30f;   // a reference that nothing has been taken 
 constexpr float KV4_LIFT = 12.0f;    // probabilities are raised by 2^12 to keep small ones in fp16's normal range
 constexpr float KV4_ROOM = 15.0f;    // and their reference moves when one would pass 2^15
 constexpr float KV4_LIFT_SUM = 8.0f; // the same where a lane's sum of 32 of them, and not each, is held below 2^15
+constexpr int KV4_TILE = 64;         // tokens of a tile of the many rows' kernel; where a sequence's seen tokens begin
+constexpr int KV4_PRE_ROWS = 256;    // rows of a key head from which the cache's halves are made by a launch of their own
 constexpr int KV4_RANGES = 64;       // ranges of a row that one workgroup joins, at most
 }  // namespace
 
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
     const int item = gb * 8 + (rb & 7), tile = rb >> 3;
     if (item >= splits * c.heads * c.n_seq) return;
     const int sp = item % splits, hk = item / splits % c.heads, s = item / splits / c.heads;
-    const KvRange kr = kv_range(a, s);
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
     const int rows = kr.nq * a.group, row0 = tile * 16;
     if (row0 >= rows) return;
     const int chunk = kv_chunk(kr, splits), tb = kr.lo + sp * chunk;
@@ -465,12 +467,70 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
 template <int D>
 __device__ __forceinline__ int v4swz(int r) { return D == 128 ? 5 * (r & 3) : vswz<D>(r); }
 
-template <int D, bool QS, bool PS>
-__global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, const int splits, const int tiles) {
+// A thread's words of a tile of 64 tokens: wavefront w has rows 16 w .. + 15, unit j of a lane words VW (u % UR) on of row
+// u / UR, u = lane + 64 j.  As halves they lie in rows of D, a row's 16-byte chunks exchanged as kswz and v4swz say.
+template <int D>
+struct TileWords {
+    static constexpr int NW = D / 32, VW = D == 96 ? 1 : NW, NV = NW / VW, G = D / 32, UR = D / 8 / VW;
+    typedef uint32_t unit_t __attribute__((ext_vector_type(VW)));
+    unit_t x[NV];
+    uint16_t d[NV];
+    // keys or values; at: place of the block's first token and head, in: the wavefront's first row in the block
+    __device__ __forceinline__ void load(const Kv4View& c, bool val, int64_t at, int in, int lane) {
+        const uint8_t* p = (val ? c.v : c.k) + (at + in) * (D / 2);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int u = lane + 64 * j, row = u / UR, grp = u % UR * VW / 4;
+            x[j] = *reinterpret_cast<const unit_t*>(p + 4 * VW * u);
+            d[j] = val ? c.v_scale[at * G + grp * c.bt + in + row] : c.k_scale[(at + in + row) * G + grp];
+        }
+    }
+    static __device__ __forceinline__ int place(bool val, int j, int w, int lane) {
+        const int u = lane + 64 * j, row = 16 * w + u / UR, chunk8 = VW * (u % UR);
+        return row * 2 * D + 16 * (chunk8 ^ (val ? v4swz<D>(row) : kswz<D>(row)));
+    }
+    // eight elements of the thread's D / 4 as halves; chunks further on are one exclusive or away
+    __device__ __forceinline__ void store(bool val, void* tile, const int* places, int i) const {
+        const int j = i / VW, e = i % VW;
+        // (values of no scale: their token's scores are NaN or hidden)
+        const _Float16 s = __builtin_bit_cast(_Float16, val ? (uint16_t)finite_scales(d[j]) : d[j]);
+        uint32_t o[4];
+        word_halves(x[j][e], h2v{s, s}, o);
+        *reinterpret_cast<u32x4*>(static_cast<char*>(tile) + (places[j] ^ (16 * e))) = u32x4{o[0], o[1], o[2], o[3]};
+    }
+};
+
+// Tiles of 64 tokens as halves, keys then values, in memory as they will lie in LDS: where many row tiles read
+// them, the conversion is done once.  A workgroup a tile.
+template <int D>
+__global__ __launch_bounds__(256) void kv4_halves_kernel(const Kv4AttnArgs a, char* tiles, const int max_tiles) {
+    const Kv4View& c = a.c;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hk = blockIdx.y, s = blockIdx.z;
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
+    const int t = kr.lo + KV4_TILE * blockIdx.x + 16 * w;
+    if (kr.lo + KV4_TILE * (int)blockIdx.x >= kr.hi || kr.nq == 0) return;
+    const int id = max(kv4_block(c, s, t), 0), in = t & (c.bt - 1);  // (what is not there or not yet is hidden later)
+    const int64_t at = ((int64_t)id * c.heads + hk) * c.bt;
+    char* out = tiles + (((int64_t)s * c.heads + hk) * max_tiles + blockIdx.x) * (KV4_TILE * D * 4);
+    TileWords<D> z[2];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) z[v].load(c, v, at, in, lane);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        int places[TileWords<D>::NV];
+#pragma unroll
+        for (int j = 0; j < TileWords<D>::NV; ++j) places[j] = TileWords<D>::place(v, j, w, lane);
+#pragma unroll
+        for (int i = 0; i < TileWords<D>::NW; ++i) z[v].store(v, out + v * (KV4_TILE * D * 2), places, i);
+    }
+}
+
+// PRE: the tiles are kv4_halves_kernel's, and go to LDS past the registers.
+template <int D, bool QS, bool PS, bool PRE>
+__global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, const int splits, const int tiles, const char* halves, const int max_tiles) {
     constexpr int NC = D / 16, NDB = D / 32;        // score products, output blocks
     constexpr bool AHEAD = !((QS && D > 64) || (PS && D > 96));  // scores a tile ahead; else the second halves have their registers
-    constexpr int NW = D / 32;                      // words of a thread, together where a row's are a power of two
-    constexpr int VW = D == 96 ? 1 : NW, NV = NW / VW, G = D / 32;
+    constexpr int NW = TileWords<D>::NW, NV = TileWords<D>::NV;
     __shared__ __attribute__((aligned(16))) _Float16 sK[2][64 * D];
     __shared__ __attribute__((aligned(16))) _Float16 sV[2][64 * D];
     const Kv4View& c = a.c;
@@ -481,14 +541,14 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
     const int items = splits * c.heads * c.n_seq, first = blockIdx.x / (8 * tiles) * 8, left = blockIdx.x - first * tiles;
     const int many = min(8, items - first), item = first + left % many, tile = tiles - 1 - left / many;
     const int sp = item % splits, hk = item / splits % c.heads, s = item / splits / c.heads;
-    const KvRange kr = kv_range(a, s);
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
     const int rows = kr.nq * a.group, row0 = tile * 128;
     if (row0 >= rows) return;
     const int chunk = kv_chunk(kr, splits);
     if (sp > 0 && kr.lo + sp * chunk >= kr.hi) return;
     const int iq_first = row0 / a.group, iq_last = (min(row0 + 128, rows) - 1) / a.group;
     const int lo_tile = a.window > 0 ? max(kr.pos0 + iq_first - a.window + 1, 0) & ~63 : 0;
-    const int tb = max(kr.lo + sp * chunk, lo_tile);  // (a multiple of 32: blocks are met at 16-token steps)
+    const int tb = max(kr.lo + sp * chunk, lo_tile);  // (a multiple of 64)
     const int te = min(min(kr.lo + sp * chunk + chunk, kr.hi), a.causal ? kr.pos0 + iq_last + 1 : kr.hi);
 
     // this lane's query row
@@ -549,45 +609,29 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
         const int i = 4 * (t & 15) + w;
         return max((t >> 4) == (tile0 >> 4) ? __builtin_amdgcn_readlane(cur, i) : __builtin_amdgcn_readlane(nxt, i), 0);
     };
-    // staging: wavefront w takes rows 16 w .. + 15 of a tile, unit j of a lane words VW (u % UR) on of row u / UR, u = lane + 64 j
-    constexpr int UR = D / 8 / VW;
-    typedef uint32_t unit_t __attribute__((ext_vector_type(VW == 1 ? 1 : VW)));
-    struct Staged {
-        unit_t x[NV];
-        uint16_t d[NV];
-    } kreg, vreg;
-    auto load_one = [&](bool val, Staged& z, int t) {
-        const int64_t at = ((int64_t)staged(t) * c.heads + hk) * c.bt;
-        const int in = (tb + 64 * t + 16 * w) & (c.bt - 1);
-        const uint8_t* p = (val ? c.v : c.k) + (at + in) * (D / 2);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int u = lane + 64 * j, row = u / UR, grp = u % UR * VW / 4;
-            z.x[j] = *reinterpret_cast<const unit_t*>(p + 4 * VW * u);
-            z.d[j] = val ? c.v_scale[at * G + grp * c.bt + in + row] : c.k_scale[(at + in + row) * G + grp];
-        }
+    TileWords<D> kreg, vreg;
+    auto load_one = [&](bool val, TileWords<D>& z, int t) {
+        z.load(c, val, ((int64_t)staged(t) * c.heads + hk) * c.bt, (tb + 64 * t + 16 * w) & (c.bt - 1), lane);
     };
-    // LDS addresses: a row's bytes are a power of two (D = 96: are added afterwards), so that a chunk further on is one
-    // exclusive or away.
     int kst[NV], vst[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const int u = lane + 64 * j, row = 16 * w + u / UR, chunk8 = VW * (u % UR);
-        kst[j] = row * 2 * D + 16 * (chunk8 ^ kswz<D>(row));
-        vst[j] = row * 2 * D + 16 * (chunk8 ^ v4swz<D>(row));
+        kst[j] = TileWords<D>::place(false, j, w, lane);
+        vst[j] = TileWords<D>::place(true, j, w, lane);
     }
-    auto store8 = [&](bool val, _Float16* lds, const Staged& z, int i) {
-        const int j = i / VW, e = i % VW;
-        // (values of no scale: their token's scores are NaN or hidden)
-        const uint16_t d16 = val ? (uint16_t)finite_scales(z.d[j]) : z.d[j];
-        const _Float16 d = __builtin_bit_cast(_Float16, d16);
-        uint32_t o[4];
-        word_halves(z.x[j][e], h2v{d, d}, o);
-        *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(lds) + ((val ? vst[j] : kst[j]) ^ (16 * e))) = u32x4{o[0], o[1], o[2], o[3]};
-    };
-    auto store_one = [&](bool val, _Float16* lds, const Staged& z) {
+    auto store_one = [&](bool val, _Float16* lds, const TileWords<D>& z) {
 #pragma unroll
-        for (int i = 0; i < NW; ++i) store8(val, lds, z, i);
+        for (int i = 0; i < NW; ++i) z.store(val, lds, val ? vst : kst, i);
+    };
+    // PRE: a wavefront's quarter of a tile's keys or values, 1 KiB at a time
+    v4i rsrc;
+    if constexpr (PRE) rsrc = make_rsrc(halves + (((int64_t)s * c.heads + hk) * max_tiles + (tb - kr.lo) / 64) * (256 * D), (int64_t)((te - tb + 63) / 64) * (256 * D));
+    auto dma = [&](bool val, _Float16* lds, int t) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int at = 1024 * (w * (D / 32) + i);
+            dma_b128_so(rsrc, (uint32_t)__builtin_amdgcn_readfirstlane(lds_addr(lds) + at), 16 * lane, t * (256 * D) + (val ? 128 * D : 0) + at);
+        }
     };
     const int krow = lr * 2 * D, kchunk = 16 * (g ^ kswz<D>(lr));
     auto key_frag = [&](const _Float16* lds, int pre, int m, int kh) {
@@ -736,8 +780,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
                     O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
                 }
             }
-            if (x < NW) store8(true, vnext, vreg, x);
-            else store8(false, knext, kreg, x - NW);
+            if constexpr (!PRE) {
+                if (x < NW) vreg.store(true, vnext, vst, x);
+                else kreg.store(false, knext, kst, x - NW);
+            }
             v8[0] = v8n[0];
             v8[1] = v8n[1];
             __builtin_amdgcn_sched_barrier(0);
@@ -753,21 +799,37 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
         nxt = group_of(16);
         off = __builtin_amdgcn_ballot_w64(cur < 0);
         v16f SA[2], SB[2];
-        load_one(false, kreg, 0);
-        store_one(false, sK[0], kreg);
-        load_one(true, vreg, 0);
-        store_one(true, sV[0], vreg);
-        load_one(false, kreg, 1);
-        if constexpr (AHEAD) {
-            store_one(false, sK[1], kreg);
-            load_one(false, kreg, 2);
+        if constexpr (PRE) {
+            dma(false, sK[0], 0);
+            dma(true, sV[0], 0);
+            if (AHEAD && nt > 1) dma(false, sK[1], 1);
+            if (AHEAD) {  // (the others' are waited for at the first step)
+                if (nt > 1) wait_vmcnt<D / 16>();
+                else wait_vmcnt<D / 32>();
+                lds_barrier();
+            }
+        } else {
+            load_one(false, kreg, 0);
+            store_one(false, sK[0], kreg);
+            load_one(true, vreg, 0);
+            store_one(true, sV[0], vreg);
+            load_one(false, kreg, 1);
+            if constexpr (AHEAD) {
+                store_one(false, sK[1], kreg);
+                load_one(false, kreg, 2);
+            }
+            load_one(true, vreg, 1);
+            __syncthreads();
         }
-        load_one(true, vreg, 1);
-        __syncthreads();
         if constexpr (AHEAD) score(sK[0], SA);
         auto step = [&](int t, int cb, v16f* Sc, v16f* Sn) {
             const int t0 = tb + 64 * t;
+            if constexpr (PRE) wait_vmcnt<0>();
             lds_barrier();
+            if constexpr (PRE) {  // into the buffers that step t - 1 read last
+                if (t + 1 < nt) dma(true, sV[cb ^ 1], t + 1);
+                if (AHEAD ? t + 2 < nt : t + 1 < nt) dma(false, sK[AHEAD ? cb : cb ^ 1], t + (AHEAD ? 2 : 1));
+            }
             tile0 = t;
             if ((t & 15) == 0 && t > 0) {
                 cur = nxt;
@@ -785,8 +847,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
                 settle(Sc, sums);
             }
             output_store(sV[cb], sV[cb ^ 1], sK[AHEAD ? cb : cb ^ 1]);
-            load_one(true, vreg, t + 2);
-            load_one(false, kreg, t + (AHEAD ? 3 : 2));
+            if constexpr (!PRE) {
+                load_one(true, vreg, t + 2);
+                load_one(false, kreg, t + (AHEAD ? 3 : 2));
+            }
         };
         for (int t = 0; t < nt; t += 2) {
             step(t, 0, SA, AHEAD ? SB : SA);
@@ -822,7 +886,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnArgs a, cons
     constexpr int C4 = D / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, pr = i / C4, all = (int64_t)a.c.n_seq * a.n_q * a.heads;
     if (pr >= all) return;
-    const KvRange kr = kv_range(a, (int)(pr / a.heads / a.n_q));
+    const KvRange kr = kv_range<KV4_TILE>(a, (int)(pr / a.heads / a.n_q));
     if (pr / a.heads % a.n_q >= kr.nq) return;
     const int chunk = kv_chunk(kr, splits);
     join_ranges<D, false>(a, splits, max((kr.hi - kr.lo + chunk - 1) / chunk, 1), pr, (int)(i - pr * C4) * 4);
@@ -839,7 +903,7 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(const Kv4AttnArgs a, f
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int hk = blockIdx.y, s = blockIdx.z;
-    const KvRange kr = kv_range(a, s);
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
     const int t0 = kr.lo + (blockIdx.x * 4 + w) * KV_STEP;
     if (t0 >= kr.hi) return;
     const int rows = kr.nq * a.group;
@@ -918,10 +982,14 @@ Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t m
     Kv4AttnPlan p;
     p.rows = rows > 64 ? 128 : 16;
     p.tiles = (int)((rows + p.rows - 1) / p.rows);
+    p.max_tiles = (int)((max_tokens + KV4_TILE - 1) / KV4_TILE) + (window > 0);
+    const double pre = (double)items * p.max_tiles * (KV4_TILE * D * 4);
+    p.pre = p.rows == 128 && rows >= KV4_PRE_ROWS && pre <= (double)(1 << 30);
     const int64_t wgs = items * p.tiles;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps, p.rows == 16 ? KV4_RANGES : 32}));
     if (p.rows == 16 && wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
-    p.bytes = p.splits > 1 ? (size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 : 0;
+    p.halves = p.splits > 1 ? ((size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 + 255) / 256 * 256 : 0;
+    p.bytes = p.halves + (p.pre ? (size_t)pre : 0);
     return p;
 }
 
@@ -929,11 +997,14 @@ template <int D, bool QS, bool PS>
 static void kv4_attn_go(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
     if (p.rows == 16) kv4_rows_kernel<D, QS, PS><<<(unsigned)((items + 7) / 8 * 8 * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles);
-    else kv4_tiles_kernel<D, QS, PS><<<(unsigned)(items * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles);
+    else if (p.pre) kv4_tiles_kernel<D, QS, PS, true><<<(unsigned)(items * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles, reinterpret_cast<char*>(a.part) + p.halves, p.max_tiles);
+    else kv4_tiles_kernel<D, QS, PS, false><<<(unsigned)(items * p.tiles), 256, 0, st>>>(a, p.splits, p.tiles, nullptr, 0);
 }
 
 template <int D>
 static hipError_t kv4_attn_d(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStream_t st) {
+    if (p.pre)
+        kv4_halves_kernel<D><<<dim3((unsigned)p.max_tiles, (unsigned)a.c.heads, (unsigned)a.c.n_seq), 256, 0, st>>>(a, reinterpret_cast<char*>(a.part) + p.halves, p.max_tiles);
     if (a.q16 && a.d16) kv4_attn_go<D, false, false>(a, p, st);
     else if (a.q16) kv4_attn_go<D, false, true>(a, p, st);
     else if (a.d16) kv4_attn_go<D, true, false>(a, p, st);
@@ -949,7 +1020,7 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hi
     if ((int64_t)a.n_q * a.heads * a.c.n_seq <= 0) return hipSuccess;
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
     if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || (int64_t)a.n_q * a.heads * a.c.n_seq * (D / 4) > (int64_t)INT32_MAX * 256 ||
-        (p.splits > 1 && (!a.part || (p.rows == 16 && !a.arrived))))
+        (p.bytes && !a.part) || (p.splits > 1 && p.rows == 16 && !a.arrived))
         return hipErrorInvalidValue;
     switch (D) {
         case 64: return kv4_attn_d<64>(a, p, st);
