@@ -681,15 +681,13 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
             if (a.lse) sums.all += p[0] + p[1];
         }
     };
-    // What is left when a tile's pairs are done: the sums, and the reference where it has to move.
-    auto settle = [&](const v16f* S, Sums& sums) {
+    // What is left when the pairs of half a tile are done: the sums, and the reference where it has to move.
+    auto settle = [&](const v16f* S, int kh, Sums& sums) {
         if (__builtin_amdgcn_ballot_w64(!(sums.s <= 32768.0f))) {
-            // some probability is too large, or may be: the reference moves to the tile's own largest
+            // some probability is too large, or may be: the reference moves to the half's own largest
             float top = -__builtin_inff();
 #pragma unroll
-            for (int kh = 0; kh < 2; ++kh)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, S[kh][i] * f);
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, S[kh][i] * f);
             const float mn = fmaxf(m_ref, xmax32(top) - KV4_LIFT_SUM), am = __builtin_amdgcn_exp2f(m_ref - mn);
             m_ref = mn;
             l_sum *= am;
@@ -700,12 +698,12 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
                 for (int e = 0; e < 16; ++e) O[b][e] *= am;
             sums = Sums{0.0f, 0.0f};
 #pragma unroll
-            for (int n = 0; n < 16; ++n) pair(S, n, sums);
+            for (int n = 0; n < 8; ++n) pair(S, 8 * kh + n, sums);
         }
         l_sum += sums.s;
         l_all += sums.all;
     };
-    // The scores Sn of the tile in lds beside the probabilities of the tile before it, whose scores S are there:
+    // The scores Sn of the tile in lds beside the first half's probabilities of the tile before it, whose scores S are there:
     // a product's fragments are read while the product before multiplies, and pairs go between the products.
     auto score_softmax = [&](const _Float16* lds, v16f* Sn, const v16f* S) {
         int pre = kpre;
@@ -729,13 +727,13 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
                 if constexpr (QS) Sn[kh] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[kh], ql[m], Sn[kh], 0, 0, 0);
             }
 #pragma unroll
-            for (int n = 16 * m / NC; n < 16 * (m + 1) / NC; ++n) pair(S, n, sums);
+            for (int n = 8 * m / NC; n < 8 * (m + 1) / NC; ++n) pair(S, n, sums);
             k8[0] = k8n[0];
             k8[1] = k8n[1];
             __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (QS) __builtin_amdgcn_s_setprio(0);
-        settle(S, sums);
+        settle(S, 0, sums);
     };
     // Scores of blocks that are not there are hidden, and so are those that a row does not see, before anything
     // is made of them.
@@ -752,8 +750,9 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
             }
         }
     };
-    // The output of the tile in lds, and the staged bytes of the next ones into their buffers between the products
-    auto output_store = [&](const _Float16* lds, _Float16* vnext, _Float16* knext) {
+    // The output of the tile in lds, and between the products of its first half the second one's probabilities, between
+    // those of the second one the staged words of the next tiles into their buffers
+    auto output_store = [&](const v16f* S, const _Float16* lds, _Float16* vnext, _Float16* knext) {
         int pre = vpre;
         asm volatile("" : "+v"(pre));
         auto frag = [&](int i) {  // product i: 16 tokens i / NDB, output block i % NDB
@@ -764,6 +763,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
         };
         v8h v8[2] = {frag(0), frag(1)}, v8n[2];
         static_assert(NDB == NW, "a unit of both to two products");
+        Sums sums = {0.0f, 0.0f};
 #pragma unroll
         for (int x = 0; x < 2 * NDB; ++x) {
             if (x + 1 < 2 * NDB) {
@@ -780,9 +780,13 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
                     O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[y], __builtin_bit_cast(v8h, e), O[b], 0, 0, 0);
                 }
             }
-            if constexpr (!PRE) {
-                if (x < NW) vreg.store(true, vnext, vst, x);
-                else kreg.store(false, knext, kst, x - NW);
+            if (x < NDB) {
+#pragma unroll
+                for (int n = 8 * x / NDB; n < 8 * (x + 1) / NDB; ++n) pair(S, 8 + n, sums);
+                if (x == NDB - 1) settle(S, 1, sums);
+            } else if constexpr (!PRE) {
+                vreg.store(true, vnext, vst, x - NDB);
+                kreg.store(false, knext, kst, x - NDB);
             }
             v8[0] = v8n[0];
             v8[1] = v8n[1];
@@ -843,10 +847,10 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
             } else {
                 Sums sums = {0.0f, 0.0f};
 #pragma unroll
-                for (int n = 0; n < 16; ++n) pair(Sc, n, sums);
-                settle(Sc, sums);
+                for (int n = 0; n < 8; ++n) pair(Sc, n, sums);
+                settle(Sc, 0, sums);
             }
-            output_store(sV[cb], sV[cb ^ 1], sK[AHEAD ? cb : cb ^ 1]);
+            output_store(Sc, sV[cb], sV[cb ^ 1], sK[AHEAD ? cb : cb ^ 1]);
             if constexpr (!PRE) {
                 load_one(true, vreg, t + 2);
                 load_one(false, kreg, t + (AHEAD ? 3 : 2));
