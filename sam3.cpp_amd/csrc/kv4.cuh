@@ -34,15 +34,19 @@ __device__ __forceinline__ int kv4_block(const Kv4View& c, int s, int t) {
     return id >= 0 && id < c.n_blocks ? id : -1;
 }
 
-// nibbles 0 and 4 (SHIFT 0) or 1 and 5 (SHIFT 4) of w as the halves u - 8: 0x640u is the half 1024 + u, 0x64u0 1024 + 16 u
+// nibbles 0 and 4 (SHIFT 0) or 1 and 5 (SHIFT 4) of w as the halves u - 8: 0x640u is the half 1024 + u, 0x64u0 1024 + 16 u.
+// (Of an instruction's operands one may be a scalar: with the exponents in a vector register the mask is one, and both
+// take one instruction.)
 template <int SHIFT>
 __device__ __forceinline__ h2v nibble_pair(uint32_t w) {
+    uint32_t exps = 0x64006400u;
+    asm("" : "+v"(exps));
     if constexpr (SHIFT == 0) {
         const h2v off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-        return __builtin_bit_cast(h2v, (w & 0x000f000fu) | 0x64006400u) + off;
+        return __builtin_bit_cast(h2v, (w & 0x000f000fu) | exps) + off;
     } else {
         const h2v mul = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-72.0f, (_Float16)-72.0f};
-        return __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w & 0x00f000f0u) | 0x64006400u), mul, off);
+        return __builtin_elementwise_fma(__builtin_bit_cast(h2v, (w & 0x00f000f0u) | exps), mul, off);
     }
 }
 // the four pairs of a word, times d

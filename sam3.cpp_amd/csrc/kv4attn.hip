@@ -15,11 +15,9 @@ namespace mi355 {
 namespace {
 constexpr float KV4_LOG2E = 1.44269504088896340736f, KV4_LN2 = 0.69314718055994530942f;
 constexpr float KV4_NONE = -1e30f;   // a reference that nothing has been taken against yet
-constexpr float KV4_LIFT = 12.0f;    // probabilities are raised by 2^12 to keep small ones in fp16's normal range
-constexpr float KV4_ROOM = 15.0f;    // and their reference moves when one would pass 2^15
+constexpr float KV4_LIFT = 12.0f;    // probabilities are raised by 2^12 to keep small ones in fp16's normal range, and their reference moves when one passes 2^15
 constexpr float KV4_LIFT_SUM = 8.0f; // the same where a lane's sum of 32 of them, and not each, is held below 2^15
 constexpr int KV4_TILE = 64;         // tokens of a tile of the many rows' kernel; where a sequence's seen tokens begin
-constexpr int KV4_PRE_ROWS = 256;    // rows of a key head from which the cache's halves are made by a launch of their own
 constexpr int KV4_RANGES = 64;       // ranges of a row that one workgroup joins, at most
 }  // namespace
 
@@ -232,7 +230,7 @@ __device__ __forceinline__ void join_ranges(const Kv4AttnArgs& a, int splits, in
 // PS: for an F32 output the probabilities enter as two halves; for an F16 one the fp32 sum is of the halves that the
 // product takes, whose roundings then cancel, and lse has a sum of its own of the probabilities before them.
 template <int D, bool QS, bool PS>
-__global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, const int splits, const int tiles) {
+__global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(const Kv4AttnArgs a, const int splits, const int tiles) {
     constexpr int KM = D / 32, NB = D / 16;
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -259,7 +257,13 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
     row.load(row_at(a, s, iq, hk * a.group + (r - iq * a.group)), on, g);
     const int pos = kr.pos0 + iq;
     const int see_hi = on ? (a.causal ? min(pos + 1, te) : te) : 0, see_lo = a.window > 0 ? pos - a.window + 1 : 0;
-    const float f = a.scale * KV4_LOG2E * row.up;
+    const float f = fmaxf(fabsf(a.scale) * KV4_LOG2E * row.up, 1e-37f);  // (0 times a hidden score)
+    if (a.scale < 0.0f)
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+            row.q[m] = -row.q[m];
+            if constexpr (QS) row.ql[m] = -row.ql[m];
+        }
 
     float m_ref = KV4_NONE, l_sum = 0.0f, l_all = 0.0f;  // (l_all: before the rounding)
     v4f O[NB];
@@ -312,11 +316,6 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
         }
         if (t0 + KV_SPAN < te) next = ask(t0 + KV_SPAN);
 
-        float x[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][i] = S[u][i] * f;
         if (!(x0.there[0] && x0.there[1] && t0 >= all_lo && t0 + KV_STEP <= all_hi)) {
             val.clean();
 #pragma unroll
@@ -324,37 +323,51 @@ __global__ __launch_bounds__(256) void kv4_rows_kernel(const Kv4AttnArgs a, cons
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int tt = t0 + 16 * u + 4 * g + i;
-                    if (!(x0.there[u] && tt >= see_lo && tt < see_hi)) x[u][i] = -__builtin_inff();
+                    if (!(x0.there[u] && tt >= see_lo && tt < see_hi)) S[u][i] = -__builtin_inff();
                 }
         }
-        const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-        if (__builtin_amdgcn_ballot_w64(top > m_ref + KV4_ROOM)) {
+        // at the reference as it stands, which moves to the step's largest where one would pass 2^15
+        float p[2][4];
+        auto raise = [&]() {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[u][i], f, -m_ref));
+        };
+        auto largest = [](const float (&x)[2][4]) {
+            return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        };
+        raise();
+        if (__builtin_amdgcn_ballot_w64(largest(p) > 32768.0f)) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = fmaxf(top, S[u][i] * f);
             const float mn = fmaxf(m_ref, col_max(top) - KV4_LIFT), am = __builtin_amdgcn_exp2f(m_ref - mn);
             m_ref = mn;
             l_sum *= am;
             l_all *= am;
 #pragma unroll
             for (int b = 0; b < NB; ++b) O[b] *= am;
+            raise();
         }
         u32x4 P, PL;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(x[u][i] - m_ref);
-            const h2v h0 = __builtin_convertvector((v2f{p[0], p[1]}), h2v), h1 = __builtin_convertvector((v2f{p[2], p[3]}), h2v);
+            const h2v h0 = __builtin_convertvector((v2f{p[u][0], p[u][1]}), h2v), h1 = __builtin_convertvector((v2f{p[u][2], p[u][3]}), h2v);
             P[2 * u] = __builtin_bit_cast(uint32_t, h0);
             P[2 * u + 1] = __builtin_bit_cast(uint32_t, h1);
             if constexpr (PS) {
-                l_sum += (p[0] + p[1]) + (p[2] + p[3]);
-                const h2v e0 = __builtin_convertvector((v2f{p[0] - (float)h0[0], p[1] - (float)h0[1]}), h2v);
-                const h2v e1 = __builtin_convertvector((v2f{p[2] - (float)h1[0], p[3] - (float)h1[1]}), h2v);
+                l_sum += (p[u][0] + p[u][1]) + (p[u][2] + p[u][3]);
+                const h2v e0 = __builtin_convertvector((v2f{p[u][0] - (float)h0[0], p[u][1] - (float)h0[1]}), h2v);
+                const h2v e1 = __builtin_convertvector((v2f{p[u][2] - (float)h1[0], p[u][3] - (float)h1[1]}), h2v);
                 PL[2 * u] = __builtin_bit_cast(uint32_t, e0);
                 PL[2 * u + 1] = __builtin_bit_cast(uint32_t, e1);
             } else {
                 const h2v ones = {(_Float16)1.0f, (_Float16)1.0f};
                 l_sum = __builtin_amdgcn_fdot2(h1, ones, __builtin_amdgcn_fdot2(h0, ones, l_sum, false), false);
-                if (a.lse) l_all += (p[0] + p[1]) + (p[2] + p[3]);
+                if (a.lse) l_all += (p[u][0] + p[u][1]) + (p[u][2] + p[u][3]);
             }
         }
 #pragma unroll
@@ -977,21 +990,55 @@ __global__ __launch_bounds__(256) void kv4_weights_kernel(const Kv4AttnArgs a, f
     }
 }
 
-// The kernel, its row tiles and the ranges of the tokens for n_q queries.
+// The kernel, its row tiles and the ranges of the tokens for n_q queries: of 16 rows, of 128, and of 128 with the tokens'
+// halves made before, each at its best number of ranges, the cheapest by the rounds of workgroups over the CUs.  A step of
+// 128 tokens takes a workgroup so long, in microseconds, with one, two .. workgroups on its CU (heads of 128 and 64, of 96
+// between them; F32 queries); where one row tile reads a sequence's tokens alone, its share of the memory at least.  Then the
+// partial sums, which a last workgroup joins past the caches or a second launch does, and the halves' launch.
+// One token of 32 sequences over 16384, 32 heads of 128 over 8: four ranges 104 us, two 117, eight 106; of one sequence: 24
+// ranges 16.1 us, 16 16.5, 8 22.9.  80 rows of 32 sequences and 4 heads of 3000 tokens: 16 rows 47, 128 41, with halves 90;
+// 126 rows of 16 heads of 2424: 14.5, 18.2, 31; 1024 rows of 64 heads of 2048: 103, 77, 86; 5184 rows of 8 heads of 64 over 15552:
+// 443, 256, 215.
 Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus) {
     if (window > 0) max_tokens = std::min<int64_t>(max_tokens, (int64_t)window + n_q + KV_STEP);  // (kv_range)
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
     const int64_t steps = std::max<int64_t>((max_tokens + KV_SPAN - 1) / KV_SPAN, 1);  // of 128 tokens
     cus = std::max(cus, 1);
     Kv4AttnPlan p;
-    p.rows = rows > 64 ? 128 : 16;
-    p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.max_tiles = (int)((max_tokens + KV4_TILE - 1) / KV4_TILE) + (window > 0);
-    const double pre = (double)items * p.max_tiles * (KV4_TILE * D * 4);
-    p.pre = p.rows == 128 && rows >= KV4_PRE_ROWS && pre <= (double)(1 << 30);
-    const int64_t wgs = items * p.tiles;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * cus + wgs - 1) / wgs, steps, p.rows == 16 ? KV4_RANGES : 32}));
-    if (p.rows == 16 && wgs > KV_ARRIVALS) p.splits = 1;  // (workgroups enough without)
+    const double pre = (double)items * p.max_tiles * (KV4_TILE * D * 4), values = (double)rows * items * D;
+    static const float us[3][2][2][4] = {
+        // 16 rows                                             128 rows                                     with halves
+        {{{1.35f, 1.75f, 2.1f, 2.4f}, {1.0f, 1.2f, 1.45f, 1.7f}}, {{1.5f, 1.95f, 2.35f, 2.35f}, {1.1f, 1.3f, 1.6f, 1.9f}}},
+        {{{3.05f, 5.0f}, {2.45f, 3.9f}}, {{3.8f, 7.0f}, {2.6f, 4.6f}}},
+        {{{2.45f, 4.2f}, {1.75f, 2.2f, 3.4f}}, {{3.4f, 6.0f}, {2.0f, 3.4f}}}};
+    double best = 1e300;
+    for (int kind = 0; kind < 3; ++kind) {
+        if ((kind > 0 && rows <= 16) || (kind == 2 && pre > (double)(1 << 30))) break;
+        const float *wide = us[kind][q16 ? 0 : 1][0], *narrow = us[kind][q16 ? 0 : 1][1];
+        const int64_t row = kind ? 128 : 16, tiles = (rows + row - 1) / row;
+        const int cap = kind == 0 ? (q16 || D == 64 ? 4 : 3) : kind == 2 && q16 && D == 64 ? 3 : 2;  // workgroups of a CU
+        for (int s = 1; s <= std::min<int64_t>(steps, kind ? 32 : KV4_RANGES); ++s) {
+            if (kind == 0 && s > 1 && items * tiles > KV_ARRIVALS) break;
+            const double per = (double)((steps + s - 1) / s), mem = tiles == 1 ? D / 128.0 : 0.0;
+            auto step = [&](int load) {
+                const int i = load - 1;
+                const double t = D == 128 ? wide[i] : D == 64 ? narrow[i] : 0.5 * (wide[std::min(i, 1)] + narrow[std::min(i, 1)]) * (i > 1 ? wide[i] / wide[1] : 1.0);
+                return per * std::max(t, mem * (0.12 + 0.78 * load));
+            };
+            const int64_t n = tiles * (kind ? items * s : (items * s + 7) / 8 * 8), full = (int64_t)cap * cus, rest = n % full;
+            double t = (double)(n / full) * step(cap) + (rest ? step((int)((rest + cus - 1) / cus)) : 0.0);
+            if (s > 1) t += kind ? 4.0 + 1.2e-6 * s * values : 0.5 + 0.3 * s + 4e-6 * s * values;
+            if (kind == 2) t += 4.0 + 1.3 * pre / 4.5e6;
+            if (t < best) {
+                best = t;
+                p.rows = (int)row;
+                p.splits = s;
+                p.pre = kind == 2;
+            }
+        }
+    }
+    p.tiles = (int)((rows + p.rows - 1) / p.rows);
     p.halves = p.splits > 1 ? ((size_t)p.splits * n_seq * n_q * heads * (D + 4) * 4 + 255) / 256 * 256 : 0;
     p.bytes = p.halves + (p.pre ? (size_t)pre : 0);
     return p;
