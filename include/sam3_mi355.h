@@ -444,7 +444,10 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
  * [max_blocks * block_tokens]) the softmax weight of token t, exp(scale q . k - lse),
  * summed over the queries that see it and the heads of key head h's group.  lse as
  * mi355_kv_cache4_attn gave it for the same queries, scale, causal and window.  Places of
- * tokens that no query sees are left as they are.  The same call gives the same bits. */
+ * tokens that no query sees are left as they are.  The same call gives the same bits.
+ * mi355_kv_cache4_weights_workspace_size as the attention's. */
+size_t mi355_kv_cache4_weights_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache,
+                                              const mi355_kv_seqs* seqs, const mi355_tensor* q, int32_t window);
 mi355_status mi355_kv_cache4_weights(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
                                      const mi355_tensor* q, const int32_t* n_q, const float* lse, float scale,
                                      int causal, int32_t window, float* sums);

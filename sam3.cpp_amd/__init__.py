@@ -194,6 +194,7 @@ def lib():
         "mi355_supports_kv_cache4_attn": (I, [C.POINTER(KvCache4), C.POINTER(KvSeqs), T, T]),
         "mi355_kv_cache4_attn_workspace_size": (SZ, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, C.c_int32]),
         "mi355_kv_cache4_attn": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, P, F, I, C.c_int32, T, P]),
+        "mi355_kv_cache4_weights_workspace_size": (SZ, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, C.c_int32]),
         "mi355_kv_cache4_weights": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), T, P, P, F, I, C.c_int32, P]),
         "mi355_kv_cache4_evict": (I, [P, C.POINTER(KvCache4), C.POINTER(KvSeqs), P, P, C.c_int32, C.c_int32, C.c_int32, P, P, P]),
         "mi355_vit_workspace_size": (SZ, [C.POINTER(VitHparams)]),
@@ -544,6 +545,9 @@ class Context:
         """Adds each cached token's softmax weights to sums, device float32 [n_seq, n_head_kv, max_blocks * block_tokens]."""
         self._check(self.L.mi355_kv_cache4_weights(self.h, cache, seqs, q, n_q or None, lse or None, scale, 1 if causal else 0, window,
                                                    sums or None))
+
+    def kv_cache4_weights_workspace_size(self, cache: KvCache4, seqs: KvSeqs, q: Tensor, window: int = 0) -> int:
+        return int(self.L.mi355_kv_cache4_weights_workspace_size(self.h, cache, seqs, q, window))
 
     def kv_cache4_evict(self, cache: KvCache4, seqs: KvSeqs, sums: int, sums_out: int, max_keep: int, kept: int, n_out: int,
                         n_keep: int = 0, first: int = 0, recent: int = 0):

@@ -421,7 +421,13 @@ struct Kv4AttnPlan {
 };
 Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus);
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hipStream_t st);
-hipError_t launch_kv4_weights(const Kv4AttnArgs& a, float* sums, int D, hipStream_t st);
+struct Kv4WeightsPlan {
+    bool few;                  // up to 16 rows
+    int splits, chunks;        // ranges (few: of the tokens; else of the rows), workgroups over the tokens
+    size_t bytes;              // of part
+};
+Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t room, int window, int cus);
+hipError_t launch_kv4_weights(const Kv4AttnArgs& a, float* sums, const Kv4WeightsPlan& p, int D, hipStream_t st);
 
 // ---- SAM3 ViT glue (rows of E contiguous floats)
 struct LnArgs {

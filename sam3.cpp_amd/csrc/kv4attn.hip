@@ -910,84 +910,291 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnArgs a, cons
 }
 
 // ---- the weights' sums by token
-// A wavefront keeps 32 tokens' keys as halves and walks over the rows, 16 at a time: S[row][token] = Q K^T gives a lane four
-// rows of one token.  exp(scale q . k - lse) is taken of the difference, so that the largest weights, which have the smallest
-// ones, lose least.  The rows' sums are taken in two levels, 64 tiles and then those, for 32 bits to hold them.
+// S[row][token] = Q K^T gives a lane some rows of one token, whose sum it keeps.  exp(scale q . k - lse) is taken of the
+// difference, so that the largest weights, which have the smallest ones, lose least.
+
+// Up to 16 rows: a wavefront keeps their queries and walks over the tokens, every fourth 32 of its workgroup's range, the
+// next ones' keys and sums asked for a step ahead.
 template <int D, bool QS>
-__global__ __launch_bounds__(256) void kv4_weights_kernel(const Kv4AttnArgs a, float* sums) {
+__global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(const Kv4AttnArgs a, float* sums, const int splits) {
     constexpr int KM = D / 32;
     const Kv4View& c = a.c;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.y, s = blockIdx.z;
+    const int item = blockIdx.x / splits, sp = blockIdx.x % splits, hk = item % c.heads, s = item / c.heads;
     const KvRange kr = kv_range<KV4_TILE>(a, s);
-    const int t0 = kr.lo + (blockIdx.x * 4 + w) * KV_STEP;
-    if (t0 >= kr.hi) return;
-    const int rows = kr.nq * a.group;
-    // queries that see one of these tokens
-    const int q_lo = a.causal ? max(t0 - kr.pos0, 0) : 0;
-    const int q_hi = a.window > 0 ? (int)min((int64_t)kr.nq, (int64_t)t0 + KV_STEP - 1 + a.window - kr.pos0) : kr.nq;
-    if (q_lo >= q_hi) return;
-    Keys<D> key[2];
-    bool there[2];
+    const int rows = kr.nq * a.group, chunk = kv_chunk(kr, splits), tb = kr.lo + sp * chunk, te = min(tb + chunk, kr.hi);
+    if (rows == 0 || tb >= te) return;
+    Row<D, QS> row;
+    const int iq = col / a.group, h = hk * a.group + (col - iq * a.group);
+    const bool on = col < rows;
+    row.load(row_at(a, s, iq, h), on, g);
+    const float lse = on ? a.lse[((int64_t)s * a.n_q + iq) * a.heads + h] : 0.0f;
+    float l[4], f[4];
+    int lo[4], hi[4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int id = kv4_block(c, s, t0 + 16 * u);
-        there[u] = id >= 0;
-        const int64_t tok = ((int64_t)max(id, 0) * c.heads + hk) * c.bt + ((t0 + 16 * u) & (c.bt - 1));
-        key[u].load(c.k + tok * (D / 2), c.k_scale + tok * KM, col, g);
+    for (int i = 0; i < 4; ++i) {
+        const int y = 4 * g + i, pos = kr.pos0 + y / a.group;
+        l[i] = __shfl(lse, y, 64);
+        f[i] = QS ? a.scale * __shfl(row.up, y, 64) : a.scale;
+        hi[i] = y < rows ? (a.causal ? min(pos + 1, kr.hi) : kr.hi) : 0;
+        lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
     }
-    v8h k8[2][KM];
+    float* out = sums + ((int64_t)s * c.heads + hk) * c.max_blocks * c.bt;
+    int ids = -1, at = 32;
+    struct Step {
+        bool there[2];
+        float old[2];
+    };
+    Keys<D> key[2];
+    auto ask = [&](int t0) {
+        Step x;
+        if (at == 32) {  // lane 2 i + u: the block of half u of this wavefront's i-th step from here
+            ids = kv4_block(c, s, t0 + (lane >> 1) * KV_SPAN + 16 * (lane & 1));
+            at = 0;
+        }
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int m = 0; m < KM; ++m) k8[u][m] = key[u].halves(m);
-    float total[2] = {0, 0}, some[2] = {0, 0};
-    int n = 0;
-    const int r_end = min(q_hi * a.group, rows);
-    for (int row0 = q_lo * a.group; row0 < r_end; row0 += 16) {
-        const int r = row0 + col, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
-        const bool on = r < r_end;
-        Row<D, QS> row;
-        row.load(row_at(a, s, iq, h), on, g);
-        const float lse = on ? a.lse[((int64_t)s * a.n_q + iq) * a.heads + h] : 0.0f;
+        for (int u = 0; u < 2; ++u) {
+            const int id = __builtin_amdgcn_readlane(ids, 2 * at + u), t = t0 + 16 * u;
+            x.there[u] = id >= 0;
+            const int64_t tok = ((int64_t)max(id, 0) * c.heads + hk) * c.bt + (t & (c.bt - 1));
+            key[u].load(c.k + tok * (D / 2), c.k_scale + tok * KM, col, g);
+            x.old[u] = t + col < te ? out[t + col] : 0.0f;
+        }
+        ++at;
+        return x;
+    };
+    Step next{};
+    if (tb + w * KV_STEP < te) next = ask(tb + w * KV_STEP);
+    for (int t0 = tb + w * KV_STEP; t0 < te; t0 += KV_SPAN) {
+        const Step x0 = next;
         v4f S[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             S[u] = v4f{0, 0, 0, 0};
 #pragma unroll
             for (int m = 0; m < KM; ++m) {
-                S[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(row.q[m], k8[u][m], S[u], 0, 0, 0);
-                if constexpr (QS) S[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(row.ql[m], k8[u][m], S[u], 0, 0, 0);
+                const v8h k8 = key[u].halves(m);
+                S[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(row.q[m], k8, S[u], 0, 0, 0);
+                if constexpr (QS) S[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(row.ql[m], k8, S[u], 0, 0, 0);
             }
         }
+        if (t0 + KV_SPAN < te) next = ask(t0 + KV_SPAN);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int y = 4 * g + i, q = (row0 + y) / a.group, pos = kr.pos0 + q;
-            const float l = __shfl(lse, y, 64), f = QS ? a.scale * __shfl(row.up, y, 64) : a.scale;
-            const int hi = row0 + y < r_end ? (a.causal ? min(pos + 1, kr.hi) : kr.hi) : 0, lo = a.window > 0 ? pos - a.window + 1 : 0;
+        for (int u = 0; u < 2; ++u) {
+            const int t = t0 + 16 * u + col;
+            float p[4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int t = t0 + 16 * u + col;
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(S[u][i], f, -l) * KV4_LOG2E);
-                some[u] += there[u] && t >= lo && t < hi ? p : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(S[u][i], f[i], -l[i]) * KV4_LOG2E);
+                p[i] = t >= lo[i] && t < hi[i] ? e : 0.0f;
+            }
+            const float sum = col_sum((p[0] + p[1]) + (p[2] + p[3]));
+            if (g == 0 && x0.there[u] && t < te) out[t] = x0.old[u] + sum;
+        }
+    }
+}
+
+// More rows: a workgroup takes 256 tokens, 64 to a wavefront as halves in registers, and a range of the rows, which pass
+// through LDS 32 at a time (an F32 row as two halves, times a power of two).  A lane sums a tile's sixteen rows of a token in a
+// tree, 32 tiles one after another and then those, for 32 bits to hold them.  A range's sums go to part, or are added at once
+// where there is one range.
+template <int D, bool QS>
+__global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4AttnArgs a, float* sums, const int splits, const int chunks) {
+    constexpr int NC = D / 16, NP = D / 32;  // products, pieces of four elements of a thread
+    const Kv4View& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // all chunks of a sequence and key head, the first ones first (causal ones are the longest), on one XCD
+    const int per = 8 * chunks * splits, gb = blockIdx.x / per, rb = blockIdx.x % per;
+    const int item = gb * 8 + (rb & 7), x = (rb >> 3) / splits, sp = (rb >> 3) % splits;
+    if (item >= c.heads * c.n_seq) return;
+    const int hk = item % c.heads, s = item / c.heads;
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
+    const int wg0 = kr.lo + 256 * x, t0 = wg0 + 64 * w;
+    if (wg0 >= kr.hi) return;
+    const int64_t room = (int64_t)c.max_blocks * c.bt;
+    // rows of this range that see one of these tokens
+    const int rows = kr.nq * a.group, share = ((rows + splits - 1) / splits + 31) / 32 * 32;
+    const int q_lo = a.causal ? max(wg0 - kr.pos0, 0) : 0;
+    const int q_hi = a.window > 0 ? (int)max(min((int64_t)kr.nq, (int64_t)wg0 + 255 + a.window - kr.pos0), (int64_t)0) : kr.nq;
+    const int r_lo = (int)max((int64_t)sp * share, (int64_t)q_lo * a.group) & ~31, r_hi = (int)min(min(((int64_t)sp + 1) * share, (int64_t)rows), (int64_t)q_hi * a.group);
+
+    v8h k8[2][NC];
+    bool there[2][2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        // a lane's token, and chunks 8 g on of 16 elements: its row's words come a group at a time
+        const int t = t0 + 32 * b + lr, id = kv4_block(c, s, t);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) there[b][u] = __builtin_amdgcn_readlane(id, 16 * u) >= 0;
+        const int64_t tok = ((int64_t)max(id, 0) * c.heads + hk) * c.bt + (t & (c.bt - 1));
+#pragma unroll
+        for (int m = 0; m < NC; ++m) {
+            const uint32_t word = *reinterpret_cast<const uint32_t*>(c.k + tok * (D / 2) + 8 * m + 4 * g);
+            const _Float16 d = __builtin_bit_cast(_Float16, c.k_scale[tok * (D / 32) + m / 2]);
+            uint32_t o[4];
+            word_halves(word, h2v{d, d}, o);
+            k8[b][m] = __builtin_bit_cast(v8h, u32x4{o[0], o[1], o[2], o[3]});
+        }
+    }
+
+    __shared__ __attribute__((aligned(16))) _Float16 sQ[2][QS ? 2 : 1][32 * D];
+    __shared__ __attribute__((aligned(16))) float sL[2][32], sF[2][32];
+    __shared__ __attribute__((aligned(16))) int sHi[2][32], sLo[2][32];
+    // staging: eight threads to a row
+    const int sr = tid >> 3, part = tid & 7;
+    struct Staged {
+        float q[QS ? 4 * NP : 1], lse;
+        v4h h[QS ? 1 : NP];
+        int pos;
+    };
+    auto load = [&](int row0) {
+        Staged z;
+        const int r = row0 + sr, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
+        const bool on = r >= r_lo && r < r_hi;
+        const char* p = row_at(a, s, iq, h) + part * (D / 8) * (QS ? 4 : 2);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            if constexpr (QS) {
+                const v4f y = on ? *reinterpret_cast<const v4f_a4*>(p + 16 * j) : v4f{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z.q[4 * j + i] = y[i];
+            } else {
+                z.h[j] = on ? *reinterpret_cast<const v4h_a2*>(p + 8 * j) : v4h{0, 0, 0, 0};
             }
         }
-        if (++n == 64) {
-            n = 0;
+        z.lse = on && part == 0 ? a.lse[((int64_t)s * a.n_q + iq) * a.heads + h] : 0.0f;
+        z.pos = on ? kr.pos0 + iq : INT32_MIN;
+        return z;
+    };
+    auto store = [&](const Staged& z, int buf) {
+        float up = 1.0f, down = 1.0f;
+        if constexpr (QS) {
+            float top = 0.0f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) total[u] += some[u], some[u] = 0.0f;
+            for (int j = 0; j < 4 * NP; ++j) top = fmaxf(top, fabsf(z.q[j]));
+            const Pow2 y = pow2_of(group_max<8>(top));
+            up = y.up;
+            down = y.down;
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int e = part * (D / 8) + 4 * j, at = sr * D + 8 * ((e >> 3) ^ kswz<D>(sr)) + (e & 4);
+            if constexpr (QS) {
+                v4h hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = z.q[4 * j + i] * down;
+                    hi[i] = (_Float16)y;
+                    lo[i] = (_Float16)(y - (float)hi[i]);
+                }
+                *reinterpret_cast<v4h*>(&sQ[buf][0][at]) = hi;
+                *reinterpret_cast<v4h*>(&sQ[buf][1][at]) = lo;
+            } else {
+                *reinterpret_cast<v4h*>(&sQ[buf][0][at]) = z.h[j];
+            }
+        }
+        if (part == 0) {
+            const bool on = z.pos != INT32_MIN;
+            sL[buf][sr] = z.lse;
+            sF[buf][sr] = a.scale * up;
+            sHi[buf][sr] = on ? (a.causal ? min(z.pos + 1, kr.hi) : kr.hi) : 0;
+            sLo[buf][sr] = on && a.window > 0 ? z.pos - a.window + 1 : 0;
+        }
+    };
+    float total[2] = {0, 0}, some[2] = {0, 0};
+    const bool all_there = there[0][0] && there[0][1] && there[1][0] && there[1][1];
+    if (r_lo < r_hi) {
+        store(load(r_lo), 0);
+        __syncthreads();
+        int n = 0, buf = 0;
+        for (int row0 = r_lo; row0 < r_hi; row0 += 32, buf ^= 1) {
+            Staged z;
+            if (row0 + 32 < r_hi) z = load(row0 + 32);
+            v16f S[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) S[b][i] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < NC; ++m) {
+                const int at = lr * D + 8 * ((2 * m + g) ^ kswz<D>(lr));
+                const v8h q = *reinterpret_cast<const v8h*>(&sQ[buf][0][at]);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, k8[b][m], S[b], 0, 0, 0);
+                if constexpr (QS) {
+                    const v8h ql = *reinterpret_cast<const v8h*>(&sQ[buf][1][at]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, k8[b][m], S[b], 0, 0, 0);
+                }
+            }
+            // a lane's rows of the tile: 8 j + 4 g .. + 3
+            float p[2][16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const v4f l = *reinterpret_cast<const v4f*>(&sL[buf][8 * j + 4 * g]);
+                const v4f f = QS ? *reinterpret_cast<const v4f*>(&sF[buf][8 * j + 4 * g]) : v4f{a.scale, a.scale, a.scale, a.scale};
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) p[b][4 * j + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][4 * j + i], f[i], -l[i]) * KV4_LOG2E);
+            }
+            // whether every row of the tile sees all of the wavefront's tokens
+            const int first = kr.pos0 + row0 / a.group, last = kr.pos0 + (row0 + 31) / a.group;
+            const bool full = all_there && row0 + 32 <= r_hi && t0 + 64 <= (a.causal ? min(first + 1, kr.hi) : kr.hi) && (a.window == 0 || t0 > last - a.window);
+            if (!full) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    typedef int i4 __attribute__((ext_vector_type(4)));
+                    const i4 hi = *reinterpret_cast<const i4*>(&sHi[buf][8 * j + 4 * g]), lo = *reinterpret_cast<const i4*>(&sLo[buf][8 * j + 4 * g]);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const int t = t0 + 32 * b + lr;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) p[b][4 * j + i] = t >= lo[i] && t < hi[i] ? p[b][4 * j + i] : 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < o; ++i) p[b][i] += p[b][i + o];
+                some[b] += p[b][0];
+            }
+            if (++n == 32) {
+                n = 0;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) total[b] += some[b], some[b] = 0.0f;
+            }
+            if (row0 + 32 < r_hi) store(z, buf ^ 1);
+            __syncthreads();
         }
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const float x = col_sum(total[u] + some[u]);
-        const int t = t0 + 16 * u + col;
-        if (g == 0 && there[u] && t < kr.hi) {
-            float* p = sums + ((int64_t)s * c.heads + hk) * c.max_blocks * c.bt + t;
-            *p += x;
+    for (int b = 0; b < 2; ++b) {
+        const float y = xsum32(total[b] + some[b]);
+        const int t = t0 + 32 * b + lr;
+        if (g == 0 && (lr < 16 ? there[b][0] : there[b][1]) && t < kr.hi) {
+            if (splits > 1) a.part[((int64_t)sp * c.heads * c.n_seq + item) * room + t] = y;
+            else sums[(int64_t)item * room + t] += y;
         }
     }
+}
+
+// sums += the ranges' parts, in their order
+__global__ __launch_bounds__(256) void kv4_weights_join_kernel(const Kv4AttnArgs a, float* sums, const int splits) {
+    const Kv4View& c = a.c;
+    const int hk = blockIdx.y, s = blockIdx.z, item = s * c.heads + hk;
+    const KvRange kr = kv_range<KV4_TILE>(a, s);
+    const int t = kr.lo + blockIdx.x * 256 + threadIdx.x;
+    if (kr.nq == 0 || t >= kr.hi || kv4_block(c, s, t) < 0) return;
+    const int64_t room = (int64_t)c.max_blocks * c.bt, at = (int64_t)item * room + t;
+    float x = 0.0f;
+    for (int i = 0; i < splits; ++i) x += a.part[(int64_t)i * c.heads * c.n_seq * room + at];
+    sums[at] += x;
 }
 
 // The kernel, its row tiles and the ranges of the tokens for n_q queries: of 16 rows, of 128, and of 128 with the tokens'
@@ -1081,22 +1288,39 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hi
     }
 }
 
-template <int D>
-static hipError_t kv4_weights_d(const Kv4AttnArgs& a, float* sums, hipStream_t st) {
-    int64_t tokens = (int64_t)a.c.max_blocks * a.c.bt;
-    if (a.window > 0) tokens = std::min<int64_t>(tokens, (int64_t)a.window + a.n_q + KV_STEP);
-    const dim3 n((unsigned)((tokens + KV_SPAN - 1) / KV_SPAN), (unsigned)a.c.heads, (unsigned)a.c.n_seq);
-    if (a.q16) kv4_weights_kernel<D, false><<<n, 256, 0, st>>>(a, sums);
-    else kv4_weights_kernel<D, true><<<n, 256, 0, st>>>(a, sums);
+// The sums' ranges: up to 16 rows of the tokens, four workgroups to a CU and four steps to a workgroup if there are as many;
+// beyond, of the rows, until the CUs have four workgroups each and no range less than eight tiles.
+Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t room, int window, int cus) {
+    const int64_t tokens = window > 0 ? std::min<int64_t>(room, (int64_t)window + n_q + KV4_TILE) : room;
+    const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
+    cus = std::max(cus, 1);
+    Kv4WeightsPlan p;
+    p.few = rows <= 16;
+    p.chunks = (int)((tokens + 255) / 256);
+    const int64_t have = p.few ? items : items * std::max(p.chunks, 1), most = p.few ? (tokens + 4 * KV_SPAN - 1) / (4 * KV_SPAN) : (rows + 255) / 256;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(4 * cus + have - 1) / have, most, p.few ? 1024 : 16}));
+    p.bytes = p.few || p.splits == 1 ? 0 : (size_t)p.splits * items * room * 4;
+    return p;
+}
+
+template <int D, bool QS>
+static hipError_t kv4_weights_go(const Kv4AttnArgs& a, float* sums, const Kv4WeightsPlan& p, hipStream_t st) {
+    const int64_t items = (int64_t)a.c.heads * a.c.n_seq, n = p.few ? items * p.splits : (items + 7) / 8 * 8 * p.chunks * p.splits;
+    if (n > INT32_MAX) return hipErrorInvalidValue;
+    if (p.few) kv4_weights_rows_kernel<D, QS><<<(unsigned)n, 256, 0, st>>>(a, sums, p.splits);
+    else kv4_weights_tiles_kernel<D, QS><<<(unsigned)n, 256, 0, st>>>(a, sums, p.splits, p.chunks);
+    if (!p.few && p.splits > 1)
+        kv4_weights_join_kernel<<<dim3((unsigned)p.chunks, (unsigned)a.c.heads, (unsigned)a.c.n_seq), 256, 0, st>>>(a, sums, p.splits);
     return hipGetLastError();
 }
 
-hipError_t launch_kv4_weights(const Kv4AttnArgs& a, float* sums, int D, hipStream_t st) {
+hipError_t launch_kv4_weights(const Kv4AttnArgs& a, float* sums, const Kv4WeightsPlan& p, int D, hipStream_t st) {
     if ((int64_t)a.n_q * a.heads * a.c.n_seq <= 0 || a.c.max_blocks <= 0 || a.c.n_blocks <= 0) return hipSuccess;
+    if (p.bytes && !a.part) return hipErrorInvalidValue;
     switch (D) {
-        case 64: return kv4_weights_d<64>(a, sums, st);
-        case 96: return kv4_weights_d<96>(a, sums, st);
-        case 128: return kv4_weights_d<128>(a, sums, st);
+        case 64: return a.q16 ? kv4_weights_go<64, false>(a, sums, p, st) : kv4_weights_go<64, true>(a, sums, p, st);
+        case 96: return a.q16 ? kv4_weights_go<96, false>(a, sums, p, st) : kv4_weights_go<96, true>(a, sums, p, st);
+        case 128: return a.q16 ? kv4_weights_go<128, false>(a, sums, p, st) : kv4_weights_go<128, true>(a, sums, p, st);
         default: return hipErrorInvalidValue;
     }
 }

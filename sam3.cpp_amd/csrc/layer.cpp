@@ -280,6 +280,11 @@ Kv4AttnPlan attn4_plan(const mi355_context* ctx, const mi355_kv_cache4* c, const
                          q->type == T_F16, ctx->cus);
 }
 
+Kv4WeightsPlan weights4_plan(const mi355_context* ctx, const mi355_kv_cache4* c, const mi355_kv_seqs* s, const mi355_tensor* q,
+                             int window) {
+    return kv4_weights_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, window, ctx->cus);
+}
+
 // The arguments that the 4-bit cache's attention and its weights' sums share, checked
 mi355_status attn4_args(mi355_context* ctx, const char* op, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                         const int32_t* n_q, float scale, int causal, int32_t window, float* lse, Kv4AttnArgs* a) {
@@ -549,6 +554,12 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
     return hip_check(ctx, tm.done(launch_kv4_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache4_attn launch");
 }
 
+size_t mi355_kv_cache4_weights_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
+                                              const mi355_tensor* q, int32_t window) {
+    if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
+    return weights4_plan(ctx, cache, seqs, q, window).bytes;
+}
+
 mi355_status mi355_kv_cache4_weights(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                                      const int32_t* n_q, const float* lse, float scale, int causal, int32_t window, float* sums) {
     const mi355_status st = check_queries<8>(ctx, "kv_cache4_weights", cache, seqs, q);
@@ -560,8 +571,12 @@ mi355_status mi355_kv_cache4_weights(mi355_context* ctx, const mi355_kv_cache4* 
     if (!lse || !sums) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_weights: null argument");
     if (reinterpret_cast<uintptr_t>(sums) & 3) return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_weights: sums must be 4-byte aligned");
     (void)hipSetDevice(ctx->device);
-    Timed tm(ctx, "kv_cache4_weights");
-    return hip_check(ctx, tm.done(launch_kv4_weights(a, sums, cache->head_dim, ctx->stream)), "kv_cache4_weights launch");
+    const Kv4WeightsPlan p = weights4_plan(ctx, cache, seqs, q, a.window);
+    const mi355_status ws = ensure_ws(ctx, p.bytes, false);
+    if (ws != MI355_STATUS_SUCCESS) return ws;
+    a.part = static_cast<float*>(ctx->ws);
+    Timed tm(ctx, p.few ? "kv_cache4_weights_16" : "kv_cache4_weights_32");  // by the rows of a step
+    return hip_check(ctx, tm.done(launch_kv4_weights(a, sums, p, cache->head_dim, ctx->stream)), "kv_cache4_weights launch");
 }
 
 mi355_status mi355_kv_cache4_evict(mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const float* sums,
