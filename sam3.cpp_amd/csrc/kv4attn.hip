@@ -1288,8 +1288,10 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hi
     }
 }
 
-// The sums' ranges: up to 16 rows of the tokens, four workgroups to a CU and four steps to a workgroup if there are as many;
-// beyond, of the rows, until the CUs have four workgroups each and no range less than eight tiles.
+// The sums' ranges.  Up to 16 rows of the tokens, to eight workgroups a CU: one token of 32 sequences over 16384, 8 key heads, 57 us
+// with eight ranges, 73 with four, 60 with 32; of one sequence 6.0 us with 128, 11.4 with 16.  Beyond, of the rows, to twelve
+// workgroups a CU and no fewer than 512 rows each: 2 x 2048 queries over 4099, 32 heads of 128 over 8, 134 us with
+// twelve ranges, 151 with four, 312 with one; 64 rows of 64 heads over 2048 12.6 us with one, 20.2 with two.
 Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t room, int window, int cus) {
     const int64_t tokens = window > 0 ? std::min<int64_t>(room, (int64_t)window + n_q + KV4_TILE) : room;
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
@@ -1297,8 +1299,8 @@ Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int
     Kv4WeightsPlan p;
     p.few = rows <= 16;
     p.chunks = (int)((tokens + 255) / 256);
-    const int64_t have = p.few ? items : items * std::max(p.chunks, 1), most = p.few ? (tokens + 4 * KV_SPAN - 1) / (4 * KV_SPAN) : (rows + 255) / 256;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({(4 * cus + have - 1) / have, most, p.few ? 1024 : 16}));
+    const int64_t have = p.few ? items : items * std::max(p.chunks, 1), most = p.few ? (tokens + KV_SPAN - 1) / KV_SPAN : rows / 512;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({((p.few ? 8 : 12) * (int64_t)cus + have - 1) / have, most, p.few ? 2048 : 32}));
     p.bytes = p.few || p.splits == 1 ? 0 : (size_t)p.splits * items * room * 4;
     return p;
 }
