@@ -17,14 +17,89 @@ __device__ __forceinline__ uint16_t kv4_scale(float hi, float lo) {
     const uint16_t h = f2h(d);
     return !(fabsf(d) <= 8160.0f) ? KV4_NAN : h == 0x8000 ? (uint16_t)0 : h;  // (one zero, whatever the elements' signs)
 }
-// 8 + x / d rounded to nearest even within 0 .. 15: the product with the reciprocal is at most one off, and
-// the remainder x - q d is exact in one fma (q d has twelve bits, and x lies within a step of it)
-__device__ __forceinline__ uint32_t kv4_nibble(float x, float d, float id) {
-    float q = rintf(x * id);
-    const float r = __builtin_fmaf(-q, d, x), half = 0.5f * fabsf(d);
-    if (fabsf(r) > half || (fabsf(r) == half && ((int)q & 1))) q += (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;
-    return (uint32_t)(int)(fminf(fmaxf(q, -8.0f), 7.0f) + 8.0f);
-}
+
+// Eight elements, their largest and smallest, whether one is not a number, and their nibbles 8 + nearest_even(x / d) at
+// a scale d and id = 1 / d (or both 0)
+template <bool F16>
+struct Eight4 {
+    u32x4 raw[F16 ? 1 : 2];
+    __device__ __forceinline__ void load(const char* p) {
+        raw[0] = *reinterpret_cast<const u32x4_a2*>(p);
+        if constexpr (!F16) raw[1] = *reinterpret_cast<const u32x4_a2*>(p + 16);
+    }
+    __device__ __forceinline__ void clear() {
+        raw[0] = u32x4{0, 0, 0, 0};
+        if constexpr (!F16) raw[1] = raw[0];
+    }
+    __device__ __forceinline__ h2v pair(int i) const {
+        const uint32_t w = raw[0][i];
+        return __builtin_bit_cast(h2v, w);
+    }
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (F16) {
+            return (float)pair(i >> 1)[i & 1];
+        } else {
+            return __uint_as_float(raw[i >> 2][i & 3]);
+        }
+    }
+    __device__ __forceinline__ void ends(float& hi, float& lo, bool& nan) const {
+        if constexpr (F16) {
+            h2v a = pair(0), b = a;
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const h2v x = pair(i);
+                a = __builtin_elementwise_max(a, x);
+                b = __builtin_elementwise_min(b, x);
+                bad |= (raw[0][i] & 0x7fff7fffu) + 0x04000400u;  // (bit 15: infinite or no number)
+            }
+            hi = fmaxf((float)a[0], (float)a[1]);
+            lo = fminf((float)b[0], (float)b[1]);
+            nan = (bad & 0x80008000u) != 0;
+        } else {
+            hi = lo = (*this)[0];
+            float z = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                hi = fmaxf(hi, (*this)[i]);
+                lo = fminf(lo, (*this)[i]);
+                z = __builtin_fmaf((*this)[i], 0.0f, z);
+            }
+            nan = z != z;
+        }
+    }
+    __device__ __forceinline__ uint32_t word(float d, float id) const {
+        float q[8];
+        if constexpr (F16) {
+            // An element has 11 bits and k + 1/2 steps have 12, so that a quotient is a tie or 2^-12 of it away from one: rounded to
+            // 2^-14 by the sum with 768 ties are exact, whatever the reciprocal's rounding, and the others keep their side.
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = rintf(__builtin_fmaf((*this)[i], id, 768.0f) - 768.0f);
+        } else {
+            // The product with the reciprocal is within 2^-22 of the quotient: where one is near a tie, the remainder x - q d
+            // decides, which is exact in one fma (q d has twelve bits, and x lies within a step of it).
+            float near = 1.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = (*this)[i] * id;
+                q[i] = rintf(y);
+                near = fminf(near, 0.5f - fabsf(y - q[i]));
+            }
+            if (__builtin_amdgcn_ballot_w64(near < 1.52587890625e-5f)) {  // 2^-16
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float r = __builtin_fmaf(-q[i], d, (*this)[i]), half = 0.5f * fabsf(d);
+                    if (fabsf(r) > half || (fabsf(r) == half && ((int)q[i] & 1))) q[i] += (r < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;
+                }
+            }
+        }
+        // four nibbles to a half of the word, as a number
+        float h[2] = {34952.0f, 34952.0f};  // 8 (1 + 16 + 256 + 4096)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i & 1] = __builtin_fmaf(__builtin_amdgcn_fmed3f(q[i], -8.0f, 7.0f), (float)(1 << (4 * (i >> 1))), h[i & 1]);
+        return (uint32_t)h[0] | (uint32_t)h[1] << 16;
+    }
+};
 
 // D / 4 lanes to a token and head, eight elements each, the keys' lanes before the values': four lanes share a
 // group.  A token with an element that is not finite, or whose group's scale would pass 8160, has NaN scales in all its
@@ -38,32 +113,17 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const K
     const int i = (blockIdx.x * 4 + w) * TW + lane / L, p = lane % L;
     const int end = kv4_len(c, s), n_new = r.idx ? min(max(r.idx[s], 0), r.n_tok) : r.n_tok;
     const int t = end - n_new + i;
-    int id = -1;
-    if (lane < TW * L && i < n_new && t >= 0) id = kv4_block(c, s, t);
-    if (__builtin_amdgcn_ballot_w64(id >= 0) == 0) return;
+    const bool on = lane < TW * L && i < n_new && t >= 0;
     const bool val = p >= L / 2;
     const int piece = val ? p - L / 2 : p;
-    float x[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (id >= 0) {
-        const char* src = (val ? r.v + i * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : r.k + i * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2]) + piece * (F16 ? 16 : 32);
-        if constexpr (F16) {
-            const v8h y = *reinterpret_cast<const v8h_a2*>(src);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = (float)y[j];
-        } else {
-            const v4f y0 = *reinterpret_cast<const v4f_a4*>(src), y1 = *reinterpret_cast<const v4f_a4*>(src + 16);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = j < 4 ? y0[j & 3] : y1[j & 3];
-        }
-    }
-    float hi = x[0], lo = x[0];
-    bool nan = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        hi = fmaxf(hi, x[j]);
-        lo = fminf(lo, x[j]);
-        nan |= x[j] != x[j];
-    }
+    Eight4<F16> x;
+    x.clear();
+    if (on) x.load((val ? r.v + i * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : r.k + i * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2]) + piece * (F16 ? 16 : 32));
+    const int id = on ? kv4_block(c, s, t) : -1;
+    if (__builtin_amdgcn_ballot_w64(id >= 0) == 0) return;
+    float hi, lo;
+    bool nan;
+    x.ends(hi, lo, nan);
     hi = fmaxf(hi, lane_swap_f<1>(hi));
     hi = fmaxf(hi, lane_swap_f<2>(hi));
     lo = fminf(lo, lane_swap_f<1>(lo));
@@ -71,10 +131,9 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const K
     uint16_t s16 = kv4_scale(hi, lo);
     const uint64_t bad = __builtin_amdgcn_ballot_w64(nan || s16 == KV4_NAN);
     if (bad >> (lane / L * L) & ((1ull << L) - 1)) s16 = KV4_NAN;
-    const float d = h2f(s16), id_d = d != 0.0f && d == d ? 1.0f / d : 0.0f;
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) word |= (id_d == 0.0f ? 8u : kv4_nibble(x[j], d, id_d)) << (4 * (j >> 1) + 16 * (j & 1));
+    const float d = s16 == KV4_NAN ? 0.0f : h2f(s16);
+    // (a scale of 0 or none: 8 for all, whatever the elements are)
+    const uint32_t word = d == 0.0f ? 0x88888888u : x.word(d, 1.0f / d);
     if (id < 0) return;
     const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
     const int tok = t & (c.bt - 1);
