@@ -144,35 +144,49 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const K
     }
 }
 
-// Thread per eight elements of a row; blockIdx.y: keys or values.
-template <bool F16>
-__global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4View c, const KvRows r, const int D8, const int64_t total) {
-    const bool val = r.k ? blockIdx.y == 1 : true;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= total) return;
-    const uint32_t row = (uint32_t)(i / D8);
-    const int e = (int)(i - (int64_t)row * D8);
-    const uint32_t hs = row / (uint32_t)r.n_tok;
-    const int t = (int)(row - hs * r.n_tok), s = (int)(hs / (uint32_t)c.heads), h = (int)(hs - (uint32_t)s * c.heads);
+// Four lanes to a group of a row: eight elements each; a workgroup takes 256 / (D / 8) rows of a sequence and head at a time,
+// keys and values, so that a lane's places follow from its row's alone.
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4View c, const KvRows r) {
+    constexpr int D8 = D / 8, G = D / 32, R = 256 / D8;
+    const int e = threadIdx.x % D8, t = blockIdx.x * R + threadIdx.x / D8, h = blockIdx.y, s = blockIdx.z;
+    if ((D == 96 && threadIdx.x >= R * D8) || t >= r.n_tok) return;
     const int p = r.idx ? r.idx[(int64_t)s * r.n_tok + t] : t;
-    const int id = kv4_block(c, s, p);
+    const int id = kv4_block(c, s, p);  // (on its way beside the length)
     if (p < 0 || p >= kv4_len(c, s) || id < 0) return;
     const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
-    const int tok = p & (c.bt - 1), groups = D8 >> 2;
-    const uint32_t w = reinterpret_cast<const uint32_t*>(val ? c.v : c.k)[(at + tok) * D8 + e];
-    const float d = h2f(val ? c.v_scale[at * groups + (e >> 2) * c.bt + tok] : c.k_scale[(at + tok) * groups + (e >> 2)]);
-    char* o = (val ? r.v + t * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : r.k + t * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2]) + e * (F16 ? 16 : 32);
-    float y[8];
+    const int tok = p & (c.bt - 1);
+    uint32_t w[2] = {0, 0};
+    uint16_t d[2] = {0, 0};
+    if (r.k) {
+        w[0] = reinterpret_cast<const uint32_t*>(c.k)[(at + tok) * D8 + e];
+        d[0] = c.k_scale[(at + tok) * G + (e >> 2)];
+    }
+    if (r.v) {
+        w[1] = reinterpret_cast<const uint32_t*>(c.v)[(at + tok) * D8 + e];
+        d[1] = c.v_scale[at * G + (e >> 2) * c.bt + tok];
+    }
 #pragma unroll
-    for (int x = 0; x < 8; ++x) y[x] = (float)((int)(w >> (4 * (x >> 1) + 16 * (x & 1)) & 15) - 8) * d;
-    if constexpr (F16) {
-        u32x4 z;
+    for (int x = 0; x < 2; ++x) {
+        char* o = x ? r.v : r.k;
+        if (!o) continue;
+        o += x ? t * r.v_nb[0] + h * r.v_nb[1] + s * r.v_nb[2] : t * r.k_nb[0] + h * r.k_nb[1] + s * r.k_nb[2];
+        const _Float16 f = __builtin_bit_cast(_Float16, d[x]);
+        uint32_t y[4];
+        word_halves(w[x], h2v{f, f}, y);
+        if constexpr (F16) {
+            *reinterpret_cast<u32x4_a2*>(o + 16 * e) = u32x4{y[0], y[1], y[2], y[3]};
+        } else {
+            v4f z[2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) z[x] = (uint32_t)f2h(y[2 * x]) | (uint32_t)f2h(y[2 * x + 1]) << 16;
-        *reinterpret_cast<u32x4_a2*>(o) = z;
-    } else {
-        *reinterpret_cast<v4f_a4*>(o) = v4f{y[0], y[1], y[2], y[3]};
-        *reinterpret_cast<v4f_a4*>(o + 16) = v4f{y[4], y[5], y[6], y[7]};
+            for (int i = 0; i < 4; ++i) {
+                const h2v q = __builtin_bit_cast(h2v, y[i]);
+                z[i >> 1][2 * (i & 1)] = (float)q[0];
+                z[i >> 1][2 * (i & 1) + 1] = (float)q[1];
+            }
+            *reinterpret_cast<v4f_a4*>(o + 32 * e) = z[0];
+            *reinterpret_cast<v4f_a4*>(o + 32 * e + 16) = z[1];
+        }
     }
 }
 
@@ -386,13 +400,20 @@ hipError_t launch_kv4_write(const Kv4View& c, const KvRows& r, int D, hipStream_
 }
 
 hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t st) {
-    const int64_t total = (int64_t)r.n_tok * c.heads * c.n_seq * (D / 8);
-    if (total <= 0 || c.max_blocks <= 0 || c.n_blocks <= 0) return hipSuccess;
-    if ((total + 255) / 256 > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 g((unsigned)((total + 255) / 256), r.k && r.v ? 2 : 1);
-    if (r.f16) kv4_read_kernel<true><<<g, 256, 0, st>>>(c, r, D / 8, total);
-    else kv4_read_kernel<false><<<g, 256, 0, st>>>(c, r, D / 8, total);
-    return hipGetLastError();
+    if (r.n_tok <= 0 || c.n_seq <= 0 || c.max_blocks <= 0 || c.n_blocks <= 0) return hipSuccess;
+    auto go = [&](auto d) {
+        constexpr int DD = decltype(d)::value, R = 256 / (DD / 8);
+        const dim3 g((unsigned)(((int64_t)r.n_tok + R - 1) / R), (unsigned)c.heads, (unsigned)c.n_seq);
+        if (r.f16) kv4_read_kernel<DD, true><<<g, 256, 0, st>>>(c, r);
+        else kv4_read_kernel<DD, false><<<g, 256, 0, st>>>(c, r);
+        return hipGetLastError();
+    };
+    switch (D) {
+        case 64: return go(std::integral_constant<int, 64>());
+        case 96: return go(std::integral_constant<int, 96>());
+        case 128: return go(std::integral_constant<int, 128>());
+        default: return hipErrorInvalidValue;
+    }
 }
 
 template <int D>
