@@ -191,9 +191,6 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4View c, const Kv
 }
 
 // ---- eviction
-// The tokens that one sequence and head keeps, in their order, and their sums: a workgroup each.  The m-th largest key
-// among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each), then one
-// walk over the tokens keeps what lies above it and as many of its equals, the first ones, as are missing.
 namespace {
 constexpr int EV_T = 1024;
 struct EvictSpan {
@@ -214,14 +211,52 @@ __device__ __forceinline__ uint32_t evict_key(float x, bool there) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return !there ? 0u : x != x ? 1u : u >> 31 ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ uint64_t lanes_below() { return (1ull << (threadIdx.x & 63)) - 1; }
+__device__ __forceinline__ int lanes_below(uint64_t m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
 
+// Counts of a workgroup's wavefronts, 64 PER of them in the order of tokens, to the sums of those before each; the sum of
+// all goes behind them.  The first wavefront does it.
+template <int PER>
+__device__ __forceinline__ void scan_counts(uint32_t* count) {
+    typedef uint32_t some __attribute__((ext_vector_type(PER)));
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        some v = reinterpret_cast<some*>(count)[threadIdx.x];
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t x = v[i];
+            v[i] = mine;
+            mine += x;
+        }
+        uint32_t before = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t x = __shfl_up(before, o, 64);
+            if ((int)threadIdx.x >= o) before += x;
+        }
+        if (threadIdx.x == 63) count[64 * PER] = before;
+        before -= mine;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] += before;
+        reinterpret_cast<some*>(count)[threadIdx.x] = v;
+    }
+    __syncthreads();
+}
+
+// The tokens that one sequence and head keeps, in their order, and their sums: a workgroup each.  The m-th largest key
+// among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each); what lies above
+// it is kept, and of its equals the first ones, as many as are missing.  Eight copies of the histogram, by lane, keep a
+// wavefront's lanes off one another's counter, and the digit of its first lane is counted at once, since many sums may be alike.
+// A thread has PER tokens in registers, 1024 apart.  Longer sequences (LONG) are walked PER at a time, once for each digit and
+// twice at the end.  Bound by the chain of loads, three histograms and two scans: 8 sequences of 16384 tokens and 8 heads in
+// 17 us, one of 1280 in 9.
+template <int PER, bool LONG>
 __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t wave[2][EV_T / 64];
+    constexpr int W = EV_T / 64, SPAN = PER * EV_T;
+    __shared__ uint32_t hist[2048][8];
+    __shared__ __attribute__((aligned(16))) uint32_t count[PER * W + 1];
     __shared__ uint32_t found[2];
     const Kv4View& c = a.c;
-    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x;
+    const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, w = t >> 6;
     const EvictSpan e = evict_span(a, s);
     const int64_t room = (int64_t)c.max_blocks * c.bt, row = (int64_t)s * c.heads + h;
     const float* sums = a.sums + row * room;
@@ -235,148 +270,199 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         }
         return;
     }
-    auto key_at = [&](int i) { return evict_key(sums[i], kv4_block(c, s, i) >= 0); };
-    const int body = e.body - e.first;                 // tokens to choose among
-    uint32_t need = e.keep - e.first - (e.n - e.body); // and how many
-    uint32_t cut = 0, mask = 0;                        // the key's digits so far
-    const bool choose = need > 0 && (int)need < body;
-    if (choose) {
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-            for (int i = t; i < bins; i += EV_T) hist[i] = 0;
-            __syncthreads();
-            for (int i0 = 0; i0 < body; i0 += EV_T) {
-                const int i = i0 + t;
-                const uint32_t k = i < body ? key_at(e.first + i) : 0;
-                const bool on = i < body && (k & mask) == cut;
-                const uint32_t digit = k >> shift & (bins - 1);
-                // the digit of the wavefront's first lane is counted at once: most weights may be alike
+    float x[PER];
+    uint32_t key[PER];
+    auto load = [&](int i0) {
+        bool there[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = i0 + j * EV_T + t;
+            x[j] = i < e.n ? sums[i] : 0.0f;
+            there[j] = i < e.n && kv4_block(c, s, i) >= 0;
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) key[j] = evict_key(x[j], there[j]);
+    };
+    auto middle = [&](int i) { return i >= e.first && i < e.body; };
+    uint32_t need = e.keep - e.first - (e.n - e.body);  // of the middle ones; fewer than there are
+    uint32_t cut = 0, mask = 0;                         // the key's digits so far
+    if (!LONG) load(0);
+    const int steps = LONG ? (e.n + SPAN - 1) / SPAN : 1;
+    if (need > 0) {
+        for (int i = t; i < 2048 * 2; i += EV_T) reinterpret_cast<u32x4*>(&hist[0][0])[i] = u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    for (int pass = 0; need > 0 && pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+        for (int step = 0; step < steps; ++step) {
+            if (LONG) load(step * SPAN);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int i = step * SPAN + j * EV_T + t;
+                const bool on = middle(i) && (key[j] & mask) == cut;
+                const uint32_t digit = key[j] >> shift & (bins - 1);
                 const uint64_t act = __builtin_amdgcn_ballot_w64(on);
                 if (act == 0) continue;
                 const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(act));
                 const uint64_t same = __builtin_amdgcn_ballot_w64(on && digit == lead);
-                if ((t & 63) == 0) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
-                if (on && digit != lead) atomicAdd(&hist[digit], 1u);
+                if ((t & 63) == 0) atomicAdd(&hist[lead][0], (uint32_t)__popcll(same));
+                if (on && digit != lead) atomicAdd(&hist[digit][t & 7], 1u);
             }
-            __syncthreads();
-            // from the top: the bin in which the need-th lies.  The first wavefront's lanes take bins / 64 each.
-            if (t < 64) {
-                const int per = bins / 64, b1 = bins - t * per;  // bins b1 - per .. b1 - 1
-                uint32_t mine = 0;
-                for (int b = 0; b < per; ++b) mine += hist[b1 - 1 - b];
-                uint32_t above = mine;
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint32_t v = __shfl_up(above, o, 64);
-                    if (t >= o) above += v;
-                }
-                above -= mine;
-                if (above < need && need <= above + mine) {
-                    int b = b1 - 1;
-                    while (above + hist[b] < need) above += hist[b--];
-                    found[0] = (uint32_t)b;
-                    found[1] = need - above;
-                }
-            }
-            __syncthreads();
-            cut |= found[0] << shift;
-            mask |= (uint32_t)(bins - 1) << shift;
-            need = found[1];
-            __syncthreads();
         }
+        __syncthreads();
+        // from the top: the bin in which the need-th lies.  A thread has the bins 2 (1023 - t) + 1 and 2 (1023 - t), and clears them.
+        uint32_t v[2] = {0, 0};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            u32x4* b = reinterpret_cast<u32x4*>(&hist[2 * (EV_T - 1 - t) + 1 - y][0]);
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const u32x4 n = b[z];
+                v[y] += (n[0] + n[1]) + (n[2] + n[3]);
+                b[z] = u32x4{0, 0, 0, 0};
+            }
+        }
+        uint32_t above = v[0] + v[1];
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t z = __shfl_up(above, o, 64);
+            if ((t & 63) >= o) above += z;
+        }
+        if ((t & 63) == 63) count[w] = above;
+        __syncthreads();
+        above -= v[0] + v[1];
+#pragma unroll
+        for (int i = 0; i < W; ++i) above += i < w ? count[i] : 0;
+        if (above < need && need <= above + v[0] + v[1]) {
+            const bool low = above + v[0] < need;
+            found[0] = 2 * (EV_T - 1 - t) + (low ? 0 : 1);
+            found[1] = need - above - (low ? v[0] : 0);
+        }
+        __syncthreads();
+        cut |= found[0] << shift;
+        mask |= (uint32_t)(bins - 1) << shift;
+        need = found[1];
     }
+    __syncthreads();
     // kept: the first and the last ones, keys above cut, and the first `need` that equal it
     int at = 0;
     uint32_t equals = 0;
-    for (int i0 = 0; i0 < e.n; i0 += EV_T) {
-        const int i = i0 + t;
-        const bool in = i < e.n, mid = in && i >= e.first && i < e.body;
-        const float x = in ? sums[i] : 0.0f;
-        const uint32_t k = mid && choose ? evict_key(x, kv4_block(c, s, i) >= 0) : 0;
-        const bool eq = mid && choose && k == cut;
-        const uint64_t be = __builtin_amdgcn_ballot_w64(eq);
-        if ((t & 63) == 0) wave[0][t >> 6] = (uint32_t)__popcll(be);
+    for (int step = 0; step < steps; ++step) {
+        if (LONG) load(step * SPAN);
+        uint64_t eq[PER], keep[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            eq[j] = __builtin_amdgcn_ballot_w64(need > 0 && middle(step * SPAN + j * EV_T + t) && key[j] == cut);
+            if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(eq[j]);
+        }
+        scan_counts<PER * W / 64>(count);
+        uint32_t before[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) before[j] = equals + count[j * W + w];
+        equals += count[PER * W];
         __syncthreads();
-        uint32_t before = equals;
-        for (int w = 0; w < EV_T / 64; ++w) {
-            if (w == t >> 6) before = equals;
-            equals += wave[0][w];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = step * SPAN + j * EV_T + t;
+            const bool equal = eq[j] >> (t & 63) & 1;
+            keep[j] = __builtin_amdgcn_ballot_w64(i < e.n && (!middle(i) || (need > 0 && (equal ? before[j] + lanes_below(eq[j]) < need : key[j] > cut))));
+            if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(keep[j]);
         }
-        const bool keep = in && (!mid || (choose ? k > cut || (eq && before + __popcll(be & lanes_below()) < need) : need > 0));
-        const uint64_t bk = __builtin_amdgcn_ballot_w64(keep);
-        if ((t & 63) == 0) wave[1][t >> 6] = (uint32_t)__popcll(bk);
+        scan_counts<PER * W / 64>(count);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (!(keep[j] >> (t & 63) & 1)) continue;
+            const int to = at + (int)count[j * W + w] + lanes_below(keep[j]);
+            kept[to] = step * SPAN + j * EV_T + t;
+            out[to] = x[j];
+        }
+        at += (int)count[PER * W];
         __syncthreads();
-        int mine = at;
-        for (int w = 0; w < EV_T / 64; ++w) {
-            if (w == t >> 6) mine = at;
-            at += wave[1][w];
-        }
-        if (keep) {
-            mine += __popcll(bk & lanes_below());
-            kept[mine] = i;
-            out[mine] = x;
-        }
     }
     for (int i = e.keep + t; i < e.n; i += EV_T) out[i] = 0.0f;
 }
 
-// Kept rows go to their places, in order and in place: place j's row comes from kept[j] >= j.  A workgroup moves one
-// slice of a sequence and head's rows (16 bytes of the keys' or values' nibbles, or a scale of a group),
-// 1024 places at a time; the next places' rows are asked for before these are written, which no later row's
-// source is among, and written once all of the workgroup has what it asked for.
+// Kept rows go to their places, in order and in place: place j's row comes from kept[j] >= j.  Four workgroups to a sequence
+// and head: keys, values, and the scales of either.  U rows to a thread at a time: all of the workgroup's are read before any place is
+// written, and no later place's source is among the places before it; the next rows are asked for meanwhile.
+// 8 sequences, 8 heads of 128, half of 16384 tokens: 32 us.
 template <int D>
 __global__ __launch_bounds__(EV_T) void kv4_move_kernel(const Kv4EvictArgs a, const int items) {
-    constexpr int NS = D / 32, G = D / 32, SL = 2 * NS + 2 * G;  // 16-byte slices of a row, groups, slices in all
+    constexpr int G = D / 32, U = 6;
     const Kv4View& c = a.c;
-    // the slices of an item run on one XCD, whose L2 has their common lines
-    const int gb = blockIdx.x / (8 * SL), rb = blockIdx.x % (8 * SL), item = gb * 8 + (rb & 7), sl = rb >> 3;
-    if (item >= items) return;
+    const int item = blockIdx.x >> 2, what = blockIdx.x & 3;
+    const bool val = what & 1, wide = what < 2;
     const int h = item % c.heads, s = item / c.heads;
     const EvictSpan e = evict_span(a, s);
     if (e.keep == e.n) return;
     const int32_t* kept = a.kept + (int64_t)item * a.max_keep;
-    const bool wide = sl < 2 * NS, val = wide ? sl >= NS : sl >= 2 * NS + G;
-    const int part = wide ? sl % NS : (sl - 2 * NS) % G;
-    struct Piece {
-        u32x4 x;
-        int j;
-        bool nan;
-    };
-    auto place = [&](int id, int tok) -> char* {
+    // rows: G lanes of 16 bytes each; scales: a lane
+    const int lanes = wide ? G : 1, tokens = EV_T / lanes, tok0 = (int)threadIdx.x / lanes, part = (int)threadIdx.x - tok0 * lanes;
+    const bool on = tok0 < tokens;
+    char* rows = reinterpret_cast<char*>(val ? c.v : c.k) + 16 * part;
+    auto wide_at = [&](int id, int tok) { return reinterpret_cast<u32x4*>(rows + (((int64_t)id * c.heads + h) * c.bt + tok) * (D / 2)); };
+    auto scale_at = [&](int id, int tok, int g) {
         const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
-        if (wide) return reinterpret_cast<char*>(val ? c.v : c.k) + (at + tok) * (D / 2) + 16 * part;
-        return reinterpret_cast<char*>(val ? c.v_scale + at * G + part * c.bt + tok : c.k_scale + (at + tok) * G + part);
+        return val ? c.v_scale + at * G + g * c.bt + tok : c.k_scale + (at + tok) * G + g;
     };
-    auto fetch = [&](int j0) {
-        Piece p;
-        p.j = j0 + (int)threadIdx.x;
-        p.x = u32x4{0, 0, 0, 0};
-        p.nan = false;
-        const int src = p.j < e.keep ? kept[p.j] : -1;
-        if (src <= p.j) {  // (none, or where it is already)
-            p.j = -1;
-            return p;
+    struct Places {
+        int src[U], from[U], to[U];
+    };
+    auto look_up = [&](int j0) {
+        Places p;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int j = j0 + u * tokens + tok0;
+            const bool in = on && j < e.keep;
+            p.src[u] = in ? kept[j] : -1;
+            p.to[u] = in ? kv4_block(c, s, j) : -1;
+            if (p.src[u] <= j) p.to[u] = -1;  // (where it is already)
         }
-        const int id = kv4_block(c, s, src);
-        if (id < 0) p.nan = true;
-        else if (wide) p.x = *reinterpret_cast<const u32x4*>(place(id, src & (c.bt - 1)));
-        else p.x[0] = *reinterpret_cast<const uint16_t*>(place(id, src & (c.bt - 1)));
+#pragma unroll
+        for (int u = 0; u < U; ++u) p.from[u] = p.to[u] >= 0 ? kv4_block(c, s, p.src[u]) : -1;
         return p;
     };
-    Piece next = fetch(0);
-    for (int j0 = 0; j0 < e.keep; j0 += EV_T) {
-        const Piece p = next;
-        if (j0 + EV_T < e.keep) next = fetch(j0 + EV_T);
-        asm volatile("" ::"v"(p.x) : "memory");  // (this step's row has arrived)
+    auto read = [&](const Places& p, u32x4* x) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x[u] = u32x4{0, 0, 0, 0};
+            const int tok = p.src[u] & (c.bt - 1);
+            if (p.from[u] < 0) {  // a row whose block is not there leaves NaN scales: its place never shows what stood there
+                if (!wide) x[u] = u32x4{KV4_NAN, KV4_NAN, KV4_NAN, KV4_NAN};
+            } else if (wide) {
+                x[u] = *wide_at(p.from[u], tok);
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) x[u][g] = *scale_at(p.from[u], tok, g);
+            }
+        }
+    };
+    Places p = look_up(0);
+    u32x4 x[U];
+    read(p, x);
+    for (int j0 = 0; j0 < e.keep; j0 += U * tokens) {
+        Places next = p;
+        u32x4 ahead[U];
+        if (j0 + U * tokens < e.keep) {
+            next = look_up(j0 + U * tokens);
+            read(next, ahead);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) asm volatile("" ::"v"(x[u]) : "memory");  // (these rows have arrived)
         lds_barrier();
-        if (p.j < 0) continue;
-        const int id = kv4_block(c, s, p.j);
-        if (id < 0) continue;
-        char* d = place(id, p.j & (c.bt - 1));
-        // a row whose block is not there leaves a NaN key: its place never shows what stood there
-        if (p.nan) {
-            if (!wide) *reinterpret_cast<uint16_t*>(d) = KV4_NAN;
-        } else if (wide) *reinterpret_cast<u32x4*>(d) = p.x;
-        else *reinterpret_cast<uint16_t*>(d) = (uint16_t)p.x[0];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int tok = (j0 + u * tokens + tok0) & (c.bt - 1);
+            if (p.to[u] >= 0) {
+                if (wide) {
+                    if (p.from[u] >= 0) *wide_at(p.to[u], tok) = x[u];
+                } else {
+#pragma unroll
+                    for (int g = 0; g < G; ++g) *scale_at(p.to[u], tok, g) = (uint16_t)x[u][g];
+                }
+            }
+            x[u] = ahead[u];
+        }
+        p = next;
     }
 }
 
@@ -419,13 +505,17 @@ hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t
 template <int D>
 static void kv4_move_go(const Kv4EvictArgs& a, hipStream_t st) {
     const int items = a.c.heads * a.c.n_seq;
-    kv4_move_kernel<D><<<(unsigned)((int64_t)(items + 7) / 8 * 8 * (D / 8)), EV_T, 0, st>>>(a, items);
+    kv4_move_kernel<D><<<(unsigned)(4 * items), EV_T, 0, st>>>(a, items);
 }
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, int D, hipStream_t st) {
     if (a.c.n_seq <= 0) return hipSuccess;
-    if ((int64_t)(a.c.heads * (int64_t)a.c.n_seq + 7) / 8 * 8 * (D / 8) > INT32_MAX) return hipErrorInvalidValue;
-    kv4_select_kernel<<<dim3((unsigned)a.c.heads, (unsigned)a.c.n_seq), EV_T, 0, st>>>(a);
+    if (4 * (int64_t)a.c.heads * a.c.n_seq > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t room = (int64_t)a.c.max_blocks * a.c.bt;
+    const dim3 g((unsigned)a.c.heads, (unsigned)a.c.n_seq);
+    if (room <= 4 * EV_T) kv4_select_kernel<4, false><<<g, EV_T, 0, st>>>(a);
+    else if (room <= 16 * EV_T) kv4_select_kernel<16, false><<<g, EV_T, 0, st>>>(a);
+    else kv4_select_kernel<16, true><<<g, EV_T, 0, st>>>(a);
     if (a.c.n_blocks <= 0 || a.c.max_blocks <= 0 || a.max_keep <= 0) return hipGetLastError();
     switch (D) {
         case 64: kv4_move_go<64>(a, st); break;
