@@ -213,6 +213,16 @@ __device__ __forceinline__ uint32_t evict_key(float x, bool there) {
 }
 __device__ __forceinline__ int lanes_below(uint64_t m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
 
+// The sum of v over this lane and those before it: shifts within rows of 16 lanes, then the rows' last lanes to those after
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+}
+
 // Counts of a workgroup's wavefronts, 64 PER of them in the order of tokens, to the sums of those before each; the sum of
 // all goes behind them.  The first wavefront does it.
 template <int PER>
@@ -228,11 +238,7 @@ __device__ __forceinline__ void scan_counts(uint32_t* count) {
             v[i] = mine;
             mine += x;
         }
-        uint32_t before = mine;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t x = __shfl_up(before, o, 64);
-            if ((int)threadIdx.x >= o) before += x;
-        }
+        uint32_t before = wave_scan(mine);
         if (threadIdx.x == 63) count[64 * PER] = before;
         before -= mine;
 #pragma unroll
@@ -243,7 +249,7 @@ __device__ __forceinline__ void scan_counts(uint32_t* count) {
 }
 
 // The tokens that one sequence and head keeps, in their order, and their sums: a workgroup each.  The m-th largest key
-// among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each); what lies above
+// among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each, until a bin's are all needed); what lies above
 // it is kept, and of its equals the first ones, as many as are missing.  Eight copies of the histogram, by lane, keep a
 // wavefront's lanes off one another's counter, and the digit of its first lane is counted at once, since many sums may be alike.
 // A thread has PER tokens in registers, 1024 apart.  Longer sequences (LONG) are walked PER at a time, once for each digit and
@@ -254,7 +260,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
     constexpr int W = EV_T / 64, SPAN = PER * EV_T;
     __shared__ uint32_t hist[2048][8];
     __shared__ __attribute__((aligned(16))) uint32_t count[PER * W + 1];
-    __shared__ uint32_t found[2];
+    __shared__ uint32_t found[3];  // the bin, how many of it are needed, how many it has
     const Kv4View& c = a.c;
     const int h = blockIdx.x, s = blockIdx.y, t = threadIdx.x, w = t >> 6;
     const EvictSpan e = evict_span(a, s);
@@ -322,11 +328,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
                 b[z] = u32x4{0, 0, 0, 0};
             }
         }
-        uint32_t above = v[0] + v[1];
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t z = __shfl_up(above, o, 64);
-            if ((t & 63) >= o) above += z;
-        }
+        uint32_t above = wave_scan(v[0] + v[1]);
         if ((t & 63) == 63) count[w] = above;
         __syncthreads();
         above -= v[0] + v[1];
@@ -336,11 +338,13 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
             const bool low = above + v[0] < need;
             found[0] = 2 * (EV_T - 1 - t) + (low ? 0 : 1);
             found[1] = need - above - (low ? v[0] : 0);
+            found[2] = v[low];
         }
         __syncthreads();
         cut |= found[0] << shift;
         mask |= (uint32_t)(bins - 1) << shift;
         need = found[1];
+        if (need == found[2]) break;  // all that have these digits
     }
     __syncthreads();
     // kept: the first and the last ones, keys above cut, and the first `need` that equal it
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         uint64_t eq[PER], keep[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            eq[j] = __builtin_amdgcn_ballot_w64(need > 0 && middle(step * SPAN + j * EV_T + t) && key[j] == cut);
+            eq[j] = __builtin_amdgcn_ballot_w64(need > 0 && middle(step * SPAN + j * EV_T + t) && (key[j] & mask) == cut);
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(eq[j]);
         }
         scan_counts<PER * W / 64>(count);
@@ -364,7 +368,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         for (int j = 0; j < PER; ++j) {
             const int i = step * SPAN + j * EV_T + t;
             const bool equal = eq[j] >> (t & 63) & 1;
-            keep[j] = __builtin_amdgcn_ballot_w64(i < e.n && (!middle(i) || (need > 0 && (equal ? before[j] + lanes_below(eq[j]) < need : key[j] > cut))));
+            keep[j] = __builtin_amdgcn_ballot_w64(i < e.n && (!middle(i) || (need > 0 && (equal ? before[j] + lanes_below(eq[j]) < need : (key[j] & mask) > cut))));
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(keep[j]);
         }
         scan_counts<PER * W / 64>(count);
@@ -381,88 +385,78 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
     for (int i = e.keep + t; i < e.n; i += EV_T) out[i] = 0.0f;
 }
 
-// Kept rows go to their places, in order and in place: place j's row comes from kept[j] >= j.  Four workgroups to a sequence
-// and head: keys, values, and the scales of either.  U rows to a thread at a time: all of the workgroup's are read before any place is
-// written, and no later place's source is among the places before it; the next rows are asked for meanwhile.
-// 8 sequences, 8 heads of 128, half of 16384 tokens: 32 us.
+// Kept rows go to their places, in order and in place: place j's row comes from kept[j] >= j.  A workgroup moves the
+// keys or values of a sequence and head (heads of 128: half of each row) or either's scales, U rows to a thread at a time: all of
+// these rows are read before any place is written, and no later place's source is among the places before it.
+// Each such round is a chain of loads (index, block, row) behind the last round's stores, about 8 us, so that rounds are few and
+// long: half of 16384 tokens of 8 sequences and 8 heads of 128 in 33 us, 55 with rounds of 1536 rows.
 template <int D>
 __global__ __launch_bounds__(EV_T) void kv4_move_kernel(const Kv4EvictArgs a, const int items) {
-    constexpr int G = D / 32, U = 6;
+    constexpr int G = D / 32, L = D == 96 ? 3 : 2, NS = D / 32 / L, U = 8;  // groups, 16-byte lanes of a slice, slices
     const Kv4View& c = a.c;
-    const int item = blockIdx.x >> 2, what = blockIdx.x & 3;
-    const bool val = what & 1, wide = what < 2;
+    const int item = blockIdx.x % items, what = blockIdx.x / items;  // (what: the slices of keys, of values, and the scales, which are short)
+    const bool wide = what < 2 * NS, val = wide ? what >= NS : what > 2 * NS;
     const int h = item % c.heads, s = item / c.heads;
     const EvictSpan e = evict_span(a, s);
     if (e.keep == e.n) return;
     const int32_t* kept = a.kept + (int64_t)item * a.max_keep;
-    // rows: G lanes of 16 bytes each; scales: a lane
-    const int lanes = wide ? G : 1, tokens = EV_T / lanes, tok0 = (int)threadIdx.x / lanes, part = (int)threadIdx.x - tok0 * lanes;
+    const int lanes = wide ? L : 1, tokens = EV_T / lanes, tok0 = (int)threadIdx.x / lanes, part = (int)threadIdx.x - tok0 * lanes;
     const bool on = tok0 < tokens;
-    char* rows = reinterpret_cast<char*>(val ? c.v : c.k) + 16 * part;
+    char* rows = reinterpret_cast<char*>(val ? c.v : c.k) + 16 * (part + L * (what % NS));
     auto wide_at = [&](int id, int tok) { return reinterpret_cast<u32x4*>(rows + (((int64_t)id * c.heads + h) * c.bt + tok) * (D / 2)); };
     auto scale_at = [&](int id, int tok, int g) {
         const int64_t at = ((int64_t)id * c.heads + h) * c.bt;
         return val ? c.v_scale + at * G + g * c.bt + tok : c.k_scale + (at + tok) * G + g;
     };
-    struct Places {
-        int src[U], from[U], to[U];
-    };
+    int src[U], to[U], next[U], next_to[U];
     auto look_up = [&](int j0) {
-        Places p;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int j = j0 + u * tokens + tok0;
             const bool in = on && j < e.keep;
-            p.src[u] = in ? kept[j] : -1;
-            p.to[u] = in ? kv4_block(c, s, j) : -1;
-            if (p.src[u] <= j) p.to[u] = -1;  // (where it is already)
+            next[u] = in ? kept[j] : -1;
+            next_to[u] = in ? kv4_block(c, s, j) : -1;
+            if (next[u] <= j) next_to[u] = -1;  // (where it is already)
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) p.from[u] = p.to[u] >= 0 ? kv4_block(c, s, p.src[u]) : -1;
-        return p;
     };
-    auto read = [&](const Places& p, u32x4* x) {
+    look_up(0);
+    for (int j0 = 0; j0 < e.keep; j0 += U * tokens) {
+        int from[U];
+        u32x4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            src[u] = next[u];
+            to[u] = next_to[u];
+            from[u] = to[u] >= 0 ? kv4_block(c, s, src[u]) : -1;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             x[u] = u32x4{0, 0, 0, 0};
-            const int tok = p.src[u] & (c.bt - 1);
-            if (p.from[u] < 0) {  // a row whose block is not there leaves NaN scales: its place never shows what stood there
+            const int tok = src[u] & (c.bt - 1);
+            if (from[u] < 0) {  // a row whose block is not there leaves NaN scales: its place never shows what stood there
                 if (!wide) x[u] = u32x4{KV4_NAN, KV4_NAN, KV4_NAN, KV4_NAN};
             } else if (wide) {
-                x[u] = *wide_at(p.from[u], tok);
+                x[u] = *wide_at(from[u], tok);
             } else {
 #pragma unroll
-                for (int g = 0; g < G; ++g) x[u][g] = *scale_at(p.from[u], tok, g);
+                for (int g = 0; g < G; ++g) x[u][g] = *scale_at(from[u], tok, g);
             }
         }
-    };
-    Places p = look_up(0);
-    u32x4 x[U];
-    read(p, x);
-    for (int j0 = 0; j0 < e.keep; j0 += U * tokens) {
-        Places next = p;
-        u32x4 ahead[U];
-        if (j0 + U * tokens < e.keep) {
-            next = look_up(j0 + U * tokens);
-            read(next, ahead);
-        }
+        if (j0 + U * tokens < e.keep) look_up(j0 + U * tokens);
 #pragma unroll
         for (int u = 0; u < U; ++u) asm volatile("" ::"v"(x[u]) : "memory");  // (these rows have arrived)
         lds_barrier();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int tok = (j0 + u * tokens + tok0) & (c.bt - 1);
-            if (p.to[u] >= 0) {
-                if (wide) {
-                    if (p.from[u] >= 0) *wide_at(p.to[u], tok) = x[u];
-                } else {
+            if (to[u] < 0) continue;
+            if (wide) {
+                if (from[u] >= 0) *wide_at(to[u], tok) = x[u];
+            } else {
 #pragma unroll
-                    for (int g = 0; g < G; ++g) *scale_at(p.to[u], tok, g) = (uint16_t)x[u][g];
-                }
+                for (int g = 0; g < G; ++g) *scale_at(to[u], tok, g) = (uint16_t)x[u][g];
             }
-            x[u] = ahead[u];
         }
-        p = next;
     }
 }
 
@@ -505,12 +499,12 @@ hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t
 template <int D>
 static void kv4_move_go(const Kv4EvictArgs& a, hipStream_t st) {
     const int items = a.c.heads * a.c.n_seq;
-    kv4_move_kernel<D><<<(unsigned)(4 * items), EV_T, 0, st>>>(a, items);
+    kv4_move_kernel<D><<<(unsigned)((D == 128 ? 6 : 4) * items), EV_T, 0, st>>>(a, items);
 }
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, int D, hipStream_t st) {
     if (a.c.n_seq <= 0) return hipSuccess;
-    if (4 * (int64_t)a.c.heads * a.c.n_seq > INT32_MAX) return hipErrorInvalidValue;
+    if (6 * (int64_t)a.c.heads * a.c.n_seq > INT32_MAX) return hipErrorInvalidValue;
     const int64_t room = (int64_t)a.c.max_blocks * a.c.bt;
     const dim3 g((unsigned)a.c.heads, (unsigned)a.c.n_seq);
     if (room <= 4 * EV_T) kv4_select_kernel<4, false><<<g, EV_T, 0, st>>>(a);
