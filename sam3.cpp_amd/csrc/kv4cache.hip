@@ -211,7 +211,9 @@ __device__ __forceinline__ uint32_t evict_key(float x, bool there) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return !there ? 0u : x != x ? 1u : u >> 31 ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ int lanes_below(uint64_t m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
+__device__ __forceinline__ uint32_t lanes_below(uint64_t m) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
 
 // The sum of v over this lane and those before it: shifts within rows of 16 lanes, then the rows' last lanes to those after
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
@@ -258,7 +260,7 @@ __device__ __forceinline__ void scan_counts(uint32_t* count) {
 template <int PER, bool LONG>
 __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) {
     constexpr int W = EV_T / 64, SPAN = PER * EV_T;
-    __shared__ uint32_t hist[2048][8];
+    __shared__ __attribute__((aligned(16))) uint32_t hist[8][2048 + 8];  // (a digit's copies in different banks)
     __shared__ __attribute__((aligned(16))) uint32_t count[PER * W + 1];
     __shared__ uint32_t found[3];  // the bin, how many of it are needed, how many it has
     const Kv4View& c = a.c;
@@ -295,7 +297,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
     if (!LONG) load(0);
     const int steps = LONG ? (e.n + SPAN - 1) / SPAN : 1;
     if (need > 0) {
-        for (int i = t; i < 2048 * 2; i += EV_T) reinterpret_cast<u32x4*>(&hist[0][0])[i] = u32x4{0, 0, 0, 0};
+        for (int i = t; i < 2056 * 2; i += EV_T) reinterpret_cast<u32x4*>(&hist[0][0])[i] = u32x4{0, 0, 0, 0};
         __syncthreads();
     }
     for (int pass = 0; need > 0 && pass < 3; ++pass) {
@@ -311,22 +313,20 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
                 if (act == 0) continue;
                 const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(act));
                 const uint64_t same = __builtin_amdgcn_ballot_w64(on && digit == lead);
-                if ((t & 63) == 0) atomicAdd(&hist[lead][0], (uint32_t)__popcll(same));
-                if (on && digit != lead) atomicAdd(&hist[digit][t & 7], 1u);
+                if ((t & 63) == 0) atomicAdd(&hist[0][lead], (uint32_t)__popcll(same));
+                if (on && digit != lead) atomicAdd(&hist[t & 7][digit], 1u);
             }
         }
         __syncthreads();
         // from the top: the bin in which the need-th lies.  A thread has the bins 2 (1023 - t) + 1 and 2 (1023 - t), and clears them.
-        uint32_t v[2] = {0, 0};
+        uint32_t v[2] = {0, 0};  // (the higher bin first)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            u32x4* b = reinterpret_cast<u32x4*>(&hist[2 * (EV_T - 1 - t) + 1 - y][0]);
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                const u32x4 n = b[z];
-                v[y] += (n[0] + n[1]) + (n[2] + n[3]);
-                b[z] = u32x4{0, 0, 0, 0};
-            }
+        for (int i = 0; i < 8; ++i) {
+            u32x2* b = reinterpret_cast<u32x2*>(&hist[i][2 * (EV_T - 1 - t)]);
+            const u32x2 n = *b;
+            *b = u32x2{0, 0};
+            v[0] += n[1];
+            v[1] += n[0];
         }
         uint32_t above = wave_scan(v[0] + v[1]);
         if ((t & 63) == 63) count[w] = above;
@@ -353,9 +353,11 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
     for (int step = 0; step < steps; ++step) {
         if (LONG) load(step * SPAN);
         uint64_t eq[PER], keep[PER];
+        bool equal[PER], kept_here[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            eq[j] = __builtin_amdgcn_ballot_w64(need > 0 && middle(step * SPAN + j * EV_T + t) && (key[j] & mask) == cut);
+            equal[j] = need > 0 && middle(step * SPAN + j * EV_T + t) && (key[j] & mask) == cut;
+            eq[j] = __builtin_amdgcn_ballot_w64(equal[j]);
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(eq[j]);
         }
         scan_counts<PER * W / 64>(count);
@@ -367,15 +369,15 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = step * SPAN + j * EV_T + t;
-            const bool equal = eq[j] >> (t & 63) & 1;
-            keep[j] = __builtin_amdgcn_ballot_w64(i < e.n && (!middle(i) || (need > 0 && (equal ? before[j] + lanes_below(eq[j]) < need : (key[j] & mask) > cut))));
+            kept_here[j] = i < e.n && (!middle(i) || (need > 0 && (equal[j] ? before[j] + lanes_below(eq[j]) < need : (key[j] & mask) > cut)));
+            keep[j] = __builtin_amdgcn_ballot_w64(kept_here[j]);
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(keep[j]);
         }
         scan_counts<PER * W / 64>(count);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (!(keep[j] >> (t & 63) & 1)) continue;
-            const int to = at + (int)count[j * W + w] + lanes_below(keep[j]);
+            if (!kept_here[j]) continue;
+            const int to = at + (int)(count[j * W + w] + lanes_below(keep[j]));
             kept[to] = step * SPAN + j * EV_T + t;
             out[to] = x[j];
         }
