@@ -550,7 +550,8 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
     if (ws != MI355_STATUS_SUCCESS) return ws;
     a.part = static_cast<float*>(ctx->ws);
     a.arrived = static_cast<uint32_t*>(ctx->arrived);
-    Timed tm(ctx, p.rows == 16 ? "kv_cache4_attn_16" : "kv_cache4_attn_128");  // by the rows of a workgroup
+    // by the rows of a workgroup, and whether the tokens' halves were made before
+    Timed tm(ctx, p.rows == 16 ? "kv_cache4_attn_16" : p.pre ? "kv_cache4_attn_128_halves" : "kv_cache4_attn_128");
     return hip_check(ctx, tm.done(launch_kv4_attn(a, p, cache->head_dim, ctx->stream)), "kv_cache4_attn launch");
 }
 
