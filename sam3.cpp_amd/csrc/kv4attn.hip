@@ -1024,17 +1024,25 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
     bool there[2][2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        // a lane's token, and chunks 8 g on of 16 elements: its row's words come a group at a time
+        // a lane's token, half g of its row's words one after another (the queries' chunks follow that order)
         const int t = t0 + 32 * b + lr, id = kv4_block(c, s, t);
 #pragma unroll
         for (int u = 0; u < 2; ++u) there[b][u] = __builtin_amdgcn_readlane(id, 16 * u) >= 0;
         const int64_t tok = ((int64_t)max(id, 0) * c.heads + hk) * c.bt + (t & (c.bt - 1));
+        const uint8_t* row = c.k + tok * (D / 2) + 4 * NC * g;
+        const uint16_t* scale = c.k_scale + tok * (D / 32);
+        uint32_t words[NC];
+#pragma unroll
+        for (int m = 0; m < NC; m += 2) {  // (a row starts on 16 bytes, its half on 8)
+            const u32x2 x = *reinterpret_cast<const u32x2*>(row + 4 * m);
+            words[m] = x[0];
+            words[m + 1] = x[1];
+        }
 #pragma unroll
         for (int m = 0; m < NC; ++m) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(c.k + tok * (D / 2) + 8 * m + 4 * g);
-            const _Float16 d = __builtin_bit_cast(_Float16, c.k_scale[tok * (D / 32) + m / 2]);
+            const _Float16 d = __builtin_bit_cast(_Float16, scale[(NC * g + m) >> 2]);
             uint32_t o[4];
-            word_halves(word, h2v{d, d}, o);
+            word_halves(words[m], h2v{d, d}, o);
             k8[b][m] = __builtin_bit_cast(v8h, u32x4{o[0], o[1], o[2], o[3]});
         }
     }
@@ -1119,7 +1127,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
                 for (int i = 0; i < 16; ++i) S[b][i] = 0.0f;
 #pragma unroll
             for (int m = 0; m < NC; ++m) {
-                const int at = lr * D + 8 * ((2 * m + g) ^ kswz<D>(lr));
+                const int at = lr * D + 8 * ((NC * g + m) ^ kswz<D>(lr));
                 const v8h q = *reinterpret_cast<const v8h*>(&sQ[buf][0][at]);
 #pragma unroll
                 for (int b = 0; b < 2; ++b) S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, k8[b][m], S[b], 0, 0, 0);
@@ -1290,8 +1298,8 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hi
 
 // The sums' ranges.  Up to 16 rows of the tokens, to eight workgroups a CU: one token of 32 sequences over 16384, 8 key heads, 57 us
 // with eight ranges, 73 with four, 60 with 32; of one sequence 6.0 us with 128, 11.4 with 16.  Beyond, of the rows, to twelve
-// workgroups a CU and no fewer than 512 rows each: 2 x 2048 queries over 4099, 32 heads of 128 over 8, 134 us with
-// twelve ranges, 151 with four, 312 with one; 64 rows of 64 heads over 2048 12.6 us with one, 20.2 with two.
+// workgroups a CU and no fewer than 512 rows each: 2 x 2048 queries over 4099, 32 heads of 128 over 8, 125 us with
+// twelve ranges, 145 with four, 304 with one; 64 rows of 64 heads over 2048 12.6 us with one, 20.2 with two.
 Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t room, int window, int cus) {
     const int64_t tokens = window > 0 ? std::min<int64_t>(room, (int64_t)window + n_q + KV4_TILE) : room;
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);

@@ -271,5 +271,7 @@ def test_nan_token_under_prompts(mi, ctx, D_):
     assert torch.isfinite(a).all()
     assert b[0, first:, 12:18].isnan().all() and torch.isfinite(b[1]).all()
     assert torch.isfinite(b[0, :first]).all() and torch.isfinite(b[0, :, :12]).all() and torch.isfinite(b[0, :, 18:]).all()
-    # what does not see it: the same numbers, but for the references that rows of a wavefront move together
-    assert ((a - b).abs()[0, :first] <= 1e-5 * (1 + a[0, :first].abs())).all() and ((a - b).abs()[1] <= 1e-5 * (1 + a[1].abs())).all()
+    # what does not see it: the same numbers, but for the references that rows of a wavefront move together, which change the
+    # fp32 sums of n terms, (n + 8) U each, and the probabilities' halves, 2^-22, of the largest value (the weights are one in all)
+    tol = 2 * ((n + 8) * U + 2.0 ** -22) * float(c.values(0, "v")[0].nan_to_num(0.0).abs().max())
+    assert ((a - b).abs()[0, :first] <= tol).all() and ((a - b).abs()[1] <= tol).all()
