@@ -229,6 +229,10 @@ __device__ __forceinline__ void join_ranges(const Kv4AttnArgs& a, int splits, in
 //           eight places of its column in the B operand.
 // PS: for an F32 output the probabilities enter as two halves; for an F16 one the fp32 sum is of the halves that the
 // product takes, whose roundings then cancel, and lse has a sum of its own of the probabilities before them.
+// With many conversations the cache's bytes bound it, with four workgroups on a CU: 32 of 16384 tokens, 32 heads of 128 over 8,
+// 459 MB in 104 us (4.4 TB/s; a step's 300 vector instructions are half of its time).  With few tokens the chain of
+// latencies does: 777 tokens, 16 heads of 64 over 2 in 7.1 us.  Values asked for a step ahead as the keys are took the registers of
+// the fourth workgroup and were no faster (110 us).
 template <int D, bool QS, bool PS>
 __global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(const Kv4AttnArgs a, const int splits, const int tiles) {
     constexpr int KM = D / 32, NB = D / 16;
@@ -472,7 +476,12 @@ __global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(con
 // nibbles becoming halves once for all four on the way: a thread loads its words of a row ahead of time and
 // writes them after the previous tile's products.  Scores and output as fattn.hip's (v_mfma_f32_32x32x16_f16, S^T = K Q^T,
 // the probabilities' registers as the operand of O^T += V^T P^T, V^T by transposing reads); a tile's scores are
-// computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU.
+// computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU: between a tile's score products go the
+// first half's probabilities of the tile before, between that tile's first output products the second half's.
+// 2 x 4096 causal F16 queries over 5120 tokens, 32 heads of 128 over 8: 336 us (940 TFLOP/s; to 367 from one run to another), 20 of
+// them for the halves; matrix pipe busy 45 % of the time, VALU 41 %, LDS reads 85 % of their rate, at a clock of 1.7 GHz.
+// 5184 F32 queries over 15552 tokens, 8 heads of 64, two halves of either operand: 330 us for 330 GFLOP.  64 rows to a wavefront
+// would halve the LDS reads, but leave one wavefront a SIMD: 673 and 407 us.
 //
 // V row slot of 16-byte chunk c in row r: c ^ this.  The transposing reads take four chunks from each of four rows, which lie
 // in distinct quarters of the banks (as fattn.hip's vswz); with heads of 128 the chunks are turned within their
@@ -914,7 +923,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnArgs a, cons
 // difference, so that the largest weights, which have the smallest ones, lose least.
 
 // Up to 16 rows: a wavefront keeps their queries and walks over the tokens, every fourth 32 of its workgroup's range, the
-// next ones' keys and sums asked for a step ahead.
+// next ones' keys and sums asked for a step ahead.  Bound by memory: 32 sequences of 16384 tokens, 8 key heads of 128, 254 MB in
+// 57 us (4.5 TB/s).
 template <int D, bool QS>
 __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(const Kv4AttnArgs a, float* sums, const int splits) {
     constexpr int KM = D / 32;
@@ -998,7 +1008,8 @@ __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(const Kv4AttnA
 // More rows: a workgroup takes 256 tokens, 64 to a wavefront as halves in registers, and a range of the rows, which pass
 // through LDS 32 at a time (an F32 row as two halves, times a power of two).  A lane sums a tile's sixteen rows of a token in a
 // tree, 32 tiles one after another and then those, for 32 bits to hold them.  A range's sums go to part, or are added at once
-// where there is one range.
+// where there is one range.  Bound by the VALU's work of a weight (difference, product, exponential, sum): 2 x 2048 causal F16
+// queries over 4099, 32 heads of 128 over 8, 77 GFLOP in 125 us; VALU busy 55 % of the time, matrix pipe 24 %.
 template <int D, bool QS>
 __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4AttnArgs a, float* sums, const int splits, const int chunks) {
     constexpr int NC = D / 16, NP = D / 32;  // products, pieces of four elements of a thread

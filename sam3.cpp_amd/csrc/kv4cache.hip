@@ -105,6 +105,8 @@ struct Eight4 {
 // group.  A token with an element that is not finite, or whose group's scale would pass 8160, has NaN scales in all its
 // groups, of keys and values: a key's NaN score is then what stands for it wherever it is seen, and its values need not be
 // told apart.
+// Bound by memory: 4 sequences of 5101 tokens, 8 heads of 128 halves, 87 MB in 19.6 us (with a division's remainder for each
+// element 27.8); several tokens to a lane were no faster.
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const KvRows r) {
     constexpr int L = D / 4, TW = 64 / L;  // lanes of a token, tokens of a wavefront
@@ -145,7 +147,8 @@ __global__ __launch_bounds__(256) void kv4_write_kernel(const Kv4View c, const K
 }
 
 // Four lanes to a group of a row: eight elements each; a workgroup takes 256 / (D / 8) rows of a sequence and head at a time,
-// keys and values, so that a lane's places follow from its row's alone.
+// keys and values, so that a lane's places follow from its row's alone.  Bound by memory: the same tokens read back, 87 MB in
+// 14.0 us (24.3 with a place worked out for every eight elements of either).
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const Kv4View c, const KvRows r) {
     constexpr int D8 = D / 8, G = D / 32, R = 256 / D8;
@@ -253,10 +256,10 @@ __device__ __forceinline__ void scan_counts(uint32_t* count) {
 // The tokens that one sequence and head keeps, in their order, and their sums: a workgroup each.  The m-th largest key
 // among the tokens that are not kept anyway is found digit by digit (11, 11 and 10 bits, a histogram each, until a bin's are all needed); what lies above
 // it is kept, and of its equals the first ones, as many as are missing.  Eight copies of the histogram, by lane, keep a
-// wavefront's lanes off one another's counter, and the digit of its first lane is counted at once, since many sums may be alike.
+// wavefront's lanes off one another's counter: many sums may be alike.
 // A thread has PER tokens in registers, 1024 apart.  Longer sequences (LONG) are walked PER at a time, once for each digit and
-// twice at the end.  Bound by the chain of loads, three histograms and two scans: 8 sequences of 16384 tokens and 8 heads in
-// 17 us, one of 1280 in 9.
+// twice at the end.  Bound by what one CU does for a sequence and head (the loads, two or three histograms, two scans, the
+// lists): 8 sequences of 16384 tokens and 8 heads in 24 us, 1280 tokens in 7.5.
 template <int PER, bool LONG>
 __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) {
     constexpr int W = EV_T / 64, SPAN = PER * EV_T;
@@ -278,20 +281,26 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         }
         return;
     }
+    const int32_t* table = c.table + (int64_t)s * c.max_blocks;
     float x[PER];
-    uint32_t key[PER];
+    uint32_t key[PER], in = 0, middle = 0;  // bit j: token j is one of the sequence's, is one to choose among
     auto load = [&](int i0) {
-        bool there[PER];
+        int id[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = i0 + j * EV_T + t;
             x[j] = i < e.n ? sums[i] : 0.0f;
-            there[j] = i < e.n && kv4_block(c, s, i) >= 0;
+            id[j] = i < e.n ? table[i >> c.bt_log2] : -1;
         }
+        in = middle = 0;
 #pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = evict_key(x[j], there[j]);
+        for (int j = 0; j < PER; ++j) {
+            const int i = i0 + j * EV_T + t;
+            key[j] = evict_key(x[j], (uint32_t)id[j] < (uint32_t)c.n_blocks);
+            in |= (uint32_t)(i < e.n) << j;
+            middle |= (uint32_t)(i >= e.first && i < e.body) << j;
+        }
     };
-    auto middle = [&](int i) { return i >= e.first && i < e.body; };
     uint32_t need = e.keep - e.first - (e.n - e.body);  // of the middle ones; fewer than there are
     uint32_t cut = 0, mask = 0;                         // the key's digits so far
     if (!LONG) load(0);
@@ -306,15 +315,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
             if (LONG) load(step * SPAN);
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                const int i = step * SPAN + j * EV_T + t;
-                const bool on = middle(i) && (key[j] & mask) == cut;
-                const uint32_t digit = key[j] >> shift & (bins - 1);
-                const uint64_t act = __builtin_amdgcn_ballot_w64(on);
-                if (act == 0) continue;
-                const uint32_t lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(act));
-                const uint64_t same = __builtin_amdgcn_ballot_w64(on && digit == lead);
-                if ((t & 63) == 0) atomicAdd(&hist[0][lead], (uint32_t)__popcll(same));
-                if (on && digit != lead) atomicAdd(&hist[t & 7][digit], 1u);
+                if ((middle >> j & 1) && ((key[j] ^ cut) & mask) == 0) atomicAdd(&hist[t & 7][key[j] >> shift & (bins - 1)], 1u);
             }
         }
         __syncthreads();
@@ -356,7 +357,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         bool equal[PER], kept_here[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            equal[j] = need > 0 && middle(step * SPAN + j * EV_T + t) && (key[j] & mask) == cut;
+            equal[j] = need > 0 && (middle >> j & 1) && ((key[j] ^ cut) & mask) == 0;
             eq[j] = __builtin_amdgcn_ballot_w64(equal[j]);
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(eq[j]);
         }
@@ -368,8 +369,7 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const int i = step * SPAN + j * EV_T + t;
-            kept_here[j] = i < e.n && (!middle(i) || (need > 0 && (equal[j] ? before[j] + lanes_below(eq[j]) < need : (key[j] & mask) > cut)));
+            kept_here[j] = (in >> j & 1) && (!(middle >> j & 1) || (need > 0 && (equal[j] ? before[j] + lanes_below(eq[j]) < need : (key[j] & mask) > cut)));
             keep[j] = __builtin_amdgcn_ballot_w64(kept_here[j]);
             if ((t & 63) == 0) count[j * W + w] = (uint32_t)__popcll(keep[j]);
         }
@@ -391,7 +391,8 @@ __global__ __launch_bounds__(EV_T) void kv4_select_kernel(const Kv4EvictArgs a) 
 // keys or values of a sequence and head (heads of 128: half of each row) or either's scales, U rows to a thread at a time: all of
 // these rows are read before any place is written, and no later place's source is among the places before it.
 // Each such round is a chain of loads (index, block, row) behind the last round's stores, about 8 us, so that rounds are few and
-// long: half of 16384 tokens of 8 sequences and 8 heads of 128 in 33 us, 55 with rounds of 1536 rows.
+// long: half of 16384 tokens of 8 sequences and 8 heads of 128, 120 MB read and written, in 42 us, 49 with rounds of 1536
+// whole rows, 53 with 16 bytes of 4096.
 template <int D>
 __global__ __launch_bounds__(EV_T) void kv4_move_kernel(const Kv4EvictArgs a, const int items) {
     constexpr int G = D / 32, L = D == 96 ? 3 : 2, NS = D / 32 / L, U = 8;  // groups, 16-byte lanes of a slice, slices

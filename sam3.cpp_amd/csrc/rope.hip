@@ -202,7 +202,8 @@ hipError_t launch_rope_multi(const RopeArgs& a, hipStream_t st) {
 // The norm of a head and its rotation in one pass: y = turned(x / sqrt(mean(x^2) + eps) * w).
 // G lanes to a head, four pairs or eight elements behind them each; a thread's H heads share its angles and weights.
 // Queries and keys are one list of heads, H neighbours at a time, so that each thread has heads of one side.  The squares
-// and their sum are fp32, in a tree over the lanes.  Bound by memory, every element moving once.
+// and their sum are fp32, in a tree over the lanes.  Bound by memory, every element moving once: 2 x 4096 tokens of 40
+// heads of 128 floats to halves, 252 MB in 53 us (4.7 TB/s); 32 single tokens are a launch, 4.7 us.
 template <bool S16, bool D16, bool HALVES, int G, int H>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkArgs a, const int qb, const int blocks, const int64_t items) {
     const RopeArgs& p = a.r;
