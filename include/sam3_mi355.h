@@ -432,6 +432,7 @@ mi355_status mi355_kv_cache4_read(mi355_context* ctx, const mi355_kv_cache4* cac
  * nothing gives zeros, one that sees a token with NaN scales NaN.  lse (device F32
  * [n_seq][n_q][n_head], or NULL) takes log sum exp(scale q . k) over the tokens that the
  * query sees, -inf where there is none; rows from n_q[s] on are left as they are.
+ * Scores are fp32, and hold a fraction up to magnitudes of 2^23: the softmax of larger ones means nothing.
  * mi355_kv_cache4_attn_workspace_size as mi355_kv_cache_attn_workspace_size. */
 int mi355_supports_kv_cache4_attn(const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                                   const mi355_tensor* dst);

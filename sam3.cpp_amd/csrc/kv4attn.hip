@@ -18,6 +18,7 @@ constexpr float KV4_NONE = -1e30f;   // a reference that nothing has been taken 
 constexpr float KV4_LIFT = 12.0f;    // probabilities are raised by 2^12 to keep small ones in fp16's normal range, and their reference moves when one passes 2^15
 constexpr float KV4_LIFT_SUM = 8.0f; // the same where a lane's sum of 32 of them, and not each, is held below 2^15
 constexpr int KV4_TILE = 64;         // tokens of a tile of the many rows' kernel; where a sequence's seen tokens begin
+constexpr int64_t KV4_GRID = UINT32_MAX / 256;  // workgroups of a launch, at most
 constexpr int KV4_RANGES = 64;       // ranges of a row that one workgroup joins, at most
 }  // namespace
 
@@ -1197,7 +1198,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
         const float y = xsum32(total[b] + some[b]);
         const int t = t0 + 32 * b + lr;
         if (g == 0 && (lr < 16 ? there[b][0] : there[b][1]) && t < kr.hi) {
-            if (splits > 1) a.part[((int64_t)sp * c.heads * c.n_seq + item) * room + t] = y;
+            if (splits > 1) a.part[((int64_t)sp * c.heads * c.n_seq + item) * chunks * 256 + (t - kr.lo)] = y;
             else sums[(int64_t)item * room + t] += y;
         }
     }
@@ -1210,10 +1211,10 @@ __global__ __launch_bounds__(256) void kv4_weights_join_kernel(const Kv4AttnArgs
     const KvRange kr = kv_range<KV4_TILE>(a, s);
     const int t = kr.lo + blockIdx.x * 256 + threadIdx.x;
     if (kr.nq == 0 || t >= kr.hi || kv4_block(c, s, t) < 0) return;
-    const int64_t room = (int64_t)c.max_blocks * c.bt, at = (int64_t)item * room + t;
+    const int64_t span = (int64_t)gridDim.x * 256, at = (int64_t)item * span + (t - kr.lo);  // (of the tokens that are seen)
     float x = 0.0f;
-    for (int i = 0; i < splits; ++i) x += a.part[(int64_t)i * c.heads * c.n_seq * room + at];
-    sums[at] += x;
+    for (int i = 0; i < splits; ++i) x += a.part[(int64_t)i * c.heads * c.n_seq * span + at];
+    sums[(int64_t)item * c.max_blocks * c.bt + t] += x;
 }
 
 // The kernel, its row tiles and the ranges of the tokens for n_q queries: of 16 rows, of 128, and of 128 with the tokens'
@@ -1296,7 +1297,7 @@ static hipError_t kv4_attn_d(const Kv4AttnArgs& a, const Kv4AttnPlan& p, hipStre
 hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hipStream_t st) {
     if ((int64_t)a.n_q * a.heads * a.c.n_seq <= 0) return hipSuccess;
     const int64_t items = (int64_t)p.splits * a.c.heads * a.c.n_seq;
-    if ((items + 7) / 8 * 8 * p.tiles > INT32_MAX || (int64_t)a.n_q * a.heads * a.c.n_seq * (D / 4) > (int64_t)INT32_MAX * 256 ||
+    if ((items + 7) / 8 * 8 * p.tiles > KV4_GRID || (int64_t)a.n_q * a.heads * a.c.n_seq * (D / 4) > KV4_GRID * 256 ||
         (p.bytes && !a.part) || (p.splits > 1 && p.rows == 16 && !a.arrived))
         return hipErrorInvalidValue;
     switch (D) {
@@ -1320,14 +1321,14 @@ Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int
     p.chunks = (int)((tokens + 255) / 256);
     const int64_t have = p.few ? items : items * std::max(p.chunks, 1), most = p.few ? (tokens + KV_SPAN - 1) / KV_SPAN : rows / 512;
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({((p.few ? 8 : 12) * (int64_t)cus + have - 1) / have, most, p.few ? 2048 : 32}));
-    p.bytes = p.few || p.splits == 1 ? 0 : (size_t)p.splits * items * room * 4;
+    p.bytes = p.few || p.splits == 1 ? 0 : (size_t)p.splits * items * p.chunks * 1024;
     return p;
 }
 
 template <int D, bool QS>
 static hipError_t kv4_weights_go(const Kv4AttnArgs& a, float* sums, const Kv4WeightsPlan& p, hipStream_t st) {
     const int64_t items = (int64_t)a.c.heads * a.c.n_seq, n = p.few ? items * p.splits : (items + 7) / 8 * 8 * p.chunks * p.splits;
-    if (n > INT32_MAX) return hipErrorInvalidValue;
+    if (n > KV4_GRID) return hipErrorInvalidValue;
     if (p.few) kv4_weights_rows_kernel<D, QS><<<(unsigned)n, 256, 0, st>>>(a, sums, p.splits);
     else kv4_weights_tiles_kernel<D, QS><<<(unsigned)n, 256, 0, st>>>(a, sums, p.splits, p.chunks);
     if (!p.few && p.splits > 1)

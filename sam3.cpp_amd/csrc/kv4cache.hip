@@ -507,7 +507,7 @@ static void kv4_move_go(const Kv4EvictArgs& a, hipStream_t st) {
 
 hipError_t launch_kv4_evict(const Kv4EvictArgs& a, int D, hipStream_t st) {
     if (a.c.n_seq <= 0) return hipSuccess;
-    if (6 * (int64_t)a.c.heads * a.c.n_seq > INT32_MAX) return hipErrorInvalidValue;
+    if (6 * EV_T * (int64_t)a.c.heads * a.c.n_seq > UINT32_MAX) return hipErrorInvalidValue;
     const int64_t room = (int64_t)a.c.max_blocks * a.c.bt;
     const dim3 g((unsigned)a.c.heads, (unsigned)a.c.n_seq);
     if (room <= 4 * EV_T) kv4_select_kernel<4, false><<<g, EV_T, 0, st>>>(a);

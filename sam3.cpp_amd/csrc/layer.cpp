@@ -177,6 +177,10 @@ mi355_status check_qk_norm_rope(mi355_context* ctx, const mi355_tensor* q, const
         if (q->ne[0] != k->ne[0] || q->ne[2] != k->ne[2] || q->ne[3] != k->ne[3])
             return fail(ctx, MI355_STATUS_INVALID_ARG, "qk_norm_rope: q and k must have the same head size, tokens and batches");
     }
+    // the lanes that four heads can need; a grid has fewer than 2^32 threads
+    const mi355_tensor* one = q ? q : k;
+    if ((double)one->ne[2] * one->ne[3] * ((q ? (q->ne[1] + 3) / 4 : 0) + (k ? (k->ne[1] + 3) / 4 : 0)) * (one->ne[0] > 128 ? 64 : one->ne[0] > 64 ? 32 : 16) > 4294967040.0)
+        return fail(ctx, MI355_STATUS_UNSUPPORTED, "qk_norm_rope: sizes beyond the launch limits");
     return MI355_STATUS_SUCCESS;
 }
 
@@ -272,6 +276,13 @@ KvAttnPlan attn_plan(const mi355_context* ctx, const mi355_kv_cache* c, const mi
                      int window) {
     return kv_attn_plan((int)q->ne[1], (int)q->ne[2], c->n_head_kv, s->n_seq, (int64_t)s->max_blocks * c->block_tokens, window, c->head_dim,
                         q->type == T_F16, ctx->cus);
+}
+
+// Sizes that the plans can be made for
+bool plannable(const mi355_context* ctx, const mi355_kv_cache4* c, const mi355_kv_seqs* s, const mi355_tensor* q) {
+    return ctx && c && s && q && dims_ok(q) && rows_fit(q) && q->ne[0] == c->head_dim && !empty(q) && c->n_head_kv > 0 &&
+           q->ne[2] % c->n_head_kv == 0 && q->ne[1] <= INT_MAX / 2 && s->n_seq == q->ne[3] && s->max_blocks >= 0 &&
+           c->block_tokens > 0 && (int64_t)s->max_blocks * c->block_tokens <= 1 << 30;
 }
 
 Kv4AttnPlan attn4_plan(const mi355_context* ctx, const mi355_kv_cache4* c, const mi355_kv_seqs* s, const mi355_tensor* q,
@@ -502,6 +513,7 @@ mi355_status mi355_kv_cache4_write(mi355_context* ctx, const mi355_kv_cache4* ca
     KvRows r;
     st = kv_rows(ctx, "kv_cache4_write", cache, seqs, k, v, n_new, &r);
     if (st != MI355_STATUS_SUCCESS) return st;
+    if (r.n_tok > 1 << 27) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache4_write: sizes beyond the launch limits");
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_write: null context");
     (void)hipSetDevice(ctx->device);
     Timed tm(ctx, "kv_cache4_write");
@@ -516,6 +528,7 @@ mi355_status mi355_kv_cache4_read(mi355_context* ctx, const mi355_kv_cache4* cac
     KvRows r;
     st = kv_rows(ctx, "kv_cache4_read", cache, seqs, k, v, pos, &r);
     if (st != MI355_STATUS_SUCCESS) return st;
+    if (r.n_tok > 1 << 27) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache4_read: sizes beyond the launch limits");
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_read: null context");
     (void)hipSetDevice(ctx->device);
     Timed tm(ctx, "kv_cache4_read");
@@ -528,7 +541,7 @@ int mi355_supports_kv_cache4_attn(const mi355_kv_cache4* cache, const mi355_kv_s
 
 size_t mi355_kv_cache4_attn_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
                                            const mi355_tensor* q, int32_t window) {
-    if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
+    if (!plannable(ctx, cache, seqs, q)) return 0;
     return attn4_plan(ctx, cache, seqs, q, window).bytes;
 }
 
@@ -557,7 +570,7 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
 
 size_t mi355_kv_cache4_weights_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs,
                                               const mi355_tensor* q, int32_t window) {
-    if (!ctx || !cache || !seqs || !q || q->ne[0] * q->ne[1] * q->ne[2] * q->ne[3] == 0 || cache->n_head_kv < 1) return 0;
+    if (!plannable(ctx, cache, seqs, q)) return 0;
     return weights4_plan(ctx, cache, seqs, q, window).bytes;
 }
 
@@ -592,6 +605,7 @@ mi355_status mi355_kv_cache4_evict(mi355_context* ctx, const mi355_kv_cache4* ca
     if ((reinterpret_cast<uintptr_t>(sums) | reinterpret_cast<uintptr_t>(sums_out) | reinterpret_cast<uintptr_t>(n_keep) |
          reinterpret_cast<uintptr_t>(kept) | reinterpret_cast<uintptr_t>(n_out)) & 3)
         return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: sums, counts and kept must be 4-byte aligned");
+    if ((int64_t)cache->n_head_kv * seqs->n_seq > 600000) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache4_evict: sizes beyond the launch limits");
     if (seqs->n_seq && (n_out == seqs->n_kv || n_out == n_keep || (sums && sums == sums_out)))
         return fail(ctx, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: outputs must not be the inputs");
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_evict: null context");

@@ -184,3 +184,13 @@ def test_evict_many(mi, ctx, D):
             for x, was in zip("kv", before[s][h]):
                 now = c.rows(s, h, x)[0]
                 assert torch.equal(now[:m], was[order]) and torch.equal(now[m:], was[m:])
+
+
+def test_weights_of_a_window_in_a_long_table(mi, ctx):
+    """Ranges of the rows hold sums of the tokens that a window leaves, not of all places of the table."""
+    c = Big(mi, [20000, 16411], 2, 64, 128, seed=5)
+    g = torch.Generator(DEV).manual_seed(6)
+    q = torch.randn((2, 1100, 8, 128), generator=g, device=DEV).to(F16)
+    size = ctx.kv_cache4_weights_workspace_size(c.cache, c.seqs, tensor(mi, q.transpose(1, 2)), 100)
+    assert 0 < size <= 32 * 2 * 2 * (100 + 1100 + 320) * 4  # at most 32 ranges; 64 tokens where the first one begins and 256 to a workgroup
+    check(mi, ctx, c, q, [1100, 1097], True, 100, F16, "kv_cache4_attn_128_halves")

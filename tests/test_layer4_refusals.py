@@ -20,8 +20,9 @@ def test_format():
     y = (R4.nibbles(x, d).to(F64) - 8) * d[:, None]
     assert torch.equal(y.half().to(F64), y)  # every value is an fp16 number
     top = x.abs().amax(-1, keepdim=True).to(F64)
-    # half a step where the nibbles reach; 7 of 8 steps on the other side, and the scale's rounding by 2^-9
-    assert ((x - y).abs() <= top / 8 * (1 + 2.0 ** -8)).all()
+    # Half a step where the nibbles reach.  On the other side they end at 7 d, and d = top / 8 (1 - r) with r up to half a step
+    # of eight significant bits, 2^-8: top - 7 d = top / 8 (1 + 7 r).
+    assert ((x - y).abs() <= top / 8 * (1 + 7 * 2.0 ** -8)).all()
     assert ((x - y).abs().mean() < 0.5 * (top / 8).mean())
 
 
@@ -147,3 +148,28 @@ def test_python_descriptions(mi):
                 (z(3, 2, 16, 32), z(3, 16, 2, 32).transpose(1, 2), h(3, 2, 16, 2), h(3, 2, 2, 16))):
         with pytest.raises(ValueError):
             mi.kv_cache4(*bad)
+
+
+def test_sizes_beyond_a_launch(mi):
+    c, n = cache4(mi, n_head_kv=1), (1 << 27) + 1
+    wide = t(mi, F16, [64, n, 1, 3])
+    refused(mi, mi.lib().mi355_kv_cache4_write(None, c, seqs(mi), wide, wide, None), UNSUPPORTED, "launch limits")
+    refused(mi, mi.lib().mi355_kv_cache4_read(None, c, seqs(mi), None, wide, None), UNSUPPORTED, "launch limits")
+    refused(mi, call(mi, "evict", cache4(mi, n_head_kv=300), seqs(mi, n_seq=2001)), UNSUPPORTED, "launch limits")
+    for ne0, tokens in ((64, 1 << 28), (128, 1 << 27), (256, 1 << 26)):
+        q, fits = t(mi, F16, [ne0, 4, tokens, 1]), t(mi, F16, [ne0, 4, tokens - 64, 1])
+        p = mi.rope_params(ne0, [ne0 // 2])
+        refused(mi, qk(mi, q, None, p, q, None), UNSUPPORTED, "launch limits")
+        refused(mi, qk(mi, fits, None, p, fits, None), INVALID, "null context")
+
+
+def test_workspace_of_what_has_no_plan(mi):
+    ctx = C.create_string_buffer(1 << 16)  # (no field is read of a call that has no plan)
+    q = t(mi, F16, [64, 5, 4, 3])
+    for size in (mi.lib().mi355_kv_cache4_attn_workspace_size, mi.lib().mi355_kv_cache4_weights_workspace_size):
+        assert size(None, cache4(mi), seqs(mi), q, 0) == 0
+        for c, s, x in ((None, seqs(mi), q), (cache4(mi), None, q), (cache4(mi), seqs(mi), None), (cache4(mi, n_head_kv=0), seqs(mi), q),
+                        (cache4(mi, n_head_kv=8), seqs(mi), q), (cache4(mi, block_tokens=0), seqs(mi), q), (cache4(mi), seqs(mi, max_blocks=-1), q),
+                        (cache4(mi), seqs(mi, n_seq=2), q), (cache4(mi), seqs(mi), t(mi, F16, [64, -5, 4, 3])),
+                        (cache4(mi), seqs(mi), t(mi, F16, [64, 5, 0, 3])), (cache4(mi), seqs(mi), t(mi, F16, [32, 5, 4, 3]))):
+            assert size(ctx, c, s, x, 0) == 0
