@@ -921,7 +921,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnArgs a, cons
 
 // ---- the weights' sums by token
 // S[row][token] = Q K^T gives a lane some rows of one token, whose sum it keeps.  exp(scale q . k - lse) is taken of the
-// difference, so that the largest weights, which have the smallest ones, lose least.
+// difference, so that the largest weights, which have the smallest ones, lose least: an error of log2(e) acts on it alone.
 
 // Up to 16 rows: a wavefront keeps their queries and walks over the tokens, every fourth 32 of its workgroup's range, the
 // next ones' keys and sums asked for a step ahead.  Bound by memory: 32 sequences of 16384 tokens, 8 key heads of 128, 254 MB in
@@ -1010,27 +1010,32 @@ __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(const Kv4AttnA
 // through LDS 32 at a time (an F32 row as two halves, times a power of two).  A lane sums a tile's sixteen rows of a token in a
 // tree, 32 tiles one after another and then those, for 32 bits to hold them.  A range's sums go to part, or are added at once
 // where there is one range.  Bound by the VALU's work of a weight (difference, product, exponential, sum): 2 x 2048 causal F16
-// queries over 4099, 32 heads of 128 over 8, 77 GFLOP in 125 us; VALU busy 55 % of the time, matrix pipe 24 %.
+// queries over 4099, 32 heads of 128 over 8, 77 GFLOP in 124 us (139 with equal ranges, chunk by chunk, the product with log2(e) of
+// each difference, and each row's place by a division); VALU busy 53 % of the time, matrix pipe 28 %, three wavefronts a SIMD.  The next
+// tile's scores between this one's weights leave two of them and took 1.13 times as long, 32 tokens to a wavefront and four of
+// them 1.12 times, rows loaded two tiles ahead the same.
 template <int D, bool QS>
 __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4AttnArgs a, float* sums, const int splits, const int chunks) {
     constexpr int NC = D / 16, NP = D / 32;  // products, pieces of four elements of a thread
     const Kv4View& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, g = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // all chunks of a sequence and key head, the first ones first (causal ones are the longest), on one XCD
+    // a sequence and key head on one XCD: all chunks of its first rows, then of the next ones
     const int per = 8 * chunks * splits, gb = blockIdx.x / per, rb = blockIdx.x % per;
-    const int item = gb * 8 + (rb & 7), x = (rb >> 3) / splits, sp = (rb >> 3) % splits;
+    const int item = gb * 8 + (rb & 7), sp = (rb >> 3) / chunks, x = (rb >> 3) % chunks;
     if (item >= c.heads * c.n_seq) return;
     const int hk = item % c.heads, s = item / c.heads;
     const KvRange kr = kv_range<KV4_TILE>(a, s);
     const int wg0 = kr.lo + 256 * x, t0 = wg0 + 64 * w;
     if (wg0 >= kr.hi) return;
     const int64_t room = (int64_t)c.max_blocks * c.bt;
-    // rows of this range that see one of these tokens
-    const int rows = kr.nq * a.group, share = ((rows + splits - 1) / splits + 31) / 32 * 32;
+    // rows of this range that see one of these tokens.  The first ranges are three times as long as the last ones, which end the
+    // launch together.
+    const int rows = kr.nq * a.group, all = (rows + 31) / 32;
+    auto begin = [&](int i) { return (int)((int64_t)all * i * (3 * splits - i) / (2 * (int64_t)splits * splits)) * 32; };
     const int q_lo = a.causal ? max(wg0 - kr.pos0, 0) : 0;
     const int q_hi = a.window > 0 ? (int)max(min((int64_t)kr.nq, (int64_t)wg0 + 255 + a.window - kr.pos0), (int64_t)0) : kr.nq;
-    const int r_lo = (int)max((int64_t)sp * share, (int64_t)q_lo * a.group) & ~31, r_hi = (int)min(min(((int64_t)sp + 1) * share, (int64_t)rows), (int64_t)q_hi * a.group);
+    const int r_lo = (int)max((int64_t)begin(sp), (int64_t)q_lo * a.group) & ~31, r_hi = (int)min(min((int64_t)begin(sp + 1), (int64_t)rows), (int64_t)q_hi * a.group);
 
     v8h k8[2][NC];
     bool there[2][2];
@@ -1069,11 +1074,15 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
         v4h h[QS ? 1 : NP];
         int pos;
     };
-    auto load = [&](int row0) {
+    // the thread's row of the next tile, 32 rows at a time: its query, head of the group, place in q and in lse
+    const int step_q = 32 / a.group, step_h = 32 - step_q * a.group;
+    int r = r_lo + sr, iq = r / a.group, hg = r - iq * a.group;
+    const char* q_row = row_at(a, s, iq, hk * a.group + hg) + part * (D / 8) * (QS ? 4 : 2);
+    const float* lse_row = a.lse + ((int64_t)s * a.n_q + iq) * a.heads + hk * a.group + hg;
+    auto load = [&]() {
         Staged z;
-        const int r = row0 + sr, iq = r / a.group, h = hk * a.group + (r - iq * a.group);
-        const bool on = r >= r_lo && r < r_hi;
-        const char* p = row_at(a, s, iq, h) + part * (D / 8) * (QS ? 4 : 2);
+        const bool on = r < r_hi;
+        const char* p = q_row;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if constexpr (QS) {
@@ -1084,10 +1093,23 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
                 z.h[j] = on ? *reinterpret_cast<const v4h_a2*>(p + 8 * j) : v4h{0, 0, 0, 0};
             }
         }
-        z.lse = on && part == 0 ? a.lse[((int64_t)s * a.n_q + iq) * a.heads + h] : 0.0f;
+        z.lse = on && part == 0 ? *lse_row : 0.0f;
         z.pos = on ? kr.pos0 + iq : INT32_MIN;
+        r += 32;
+        iq += step_q;
+        hg += step_h;
+        q_row += step_q * a.q_nb[0] + step_h * a.q_nb[1];
+        lse_row += (int64_t)step_q * a.heads + step_h;
+        if (hg >= a.group) {
+            hg -= a.group;
+            ++iq;
+            q_row += a.q_nb[0] - a.group * a.q_nb[1];
+            lse_row += a.heads - a.group;
+        }
         return z;
     };
+    // in base 2: scale log2(e) is off by its rounding, and lse takes the same error, so that it acts on their difference alone
+    const float f2 = a.scale * KV4_LOG2E, ratio = a.scale != 0.0f ? f2 / a.scale : KV4_LOG2E;
     auto store = [&](const Staged& z, int buf) {
         float up = 1.0f, down = 1.0f;
         if constexpr (QS) {
@@ -1117,8 +1139,8 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
         }
         if (part == 0) {
             const bool on = z.pos != INT32_MIN;
-            sL[buf][sr] = z.lse;
-            sF[buf][sr] = a.scale * up;
+            sL[buf][sr] = z.lse * ratio;
+            sF[buf][sr] = f2 * up;
             sHi[buf][sr] = on ? (a.causal ? min(z.pos + 1, kr.hi) : kr.hi) : 0;
             sLo[buf][sr] = on && a.window > 0 ? z.pos - a.window + 1 : 0;
         }
@@ -1126,12 +1148,12 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
     float total[2] = {0, 0}, some[2] = {0, 0};
     const bool all_there = there[0][0] && there[0][1] && there[1][0] && there[1][1];
     if (r_lo < r_hi) {
-        store(load(r_lo), 0);
+        store(load(), 0);
         __syncthreads();
         int n = 0, buf = 0;
         for (int row0 = r_lo; row0 < r_hi; row0 += 32, buf ^= 1) {
             Staged z;
-            if (row0 + 32 < r_hi) z = load(row0 + 32);
+            if (row0 + 32 < r_hi) z = load();
             v16f S[2];
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -1154,11 +1176,11 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const v4f l = *reinterpret_cast<const v4f*>(&sL[buf][8 * j + 4 * g]);
-                const v4f f = QS ? *reinterpret_cast<const v4f*>(&sF[buf][8 * j + 4 * g]) : v4f{a.scale, a.scale, a.scale, a.scale};
+                const v4f f = QS ? *reinterpret_cast<const v4f*>(&sF[buf][8 * j + 4 * g]) : v4f{f2, f2, f2, f2};
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) p[b][4 * j + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][4 * j + i], f[i], -l[i]) * KV4_LOG2E);
+                    for (int i = 0; i < 4; ++i) p[b][4 * j + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[b][4 * j + i], f[i], -l[i]));
             }
             // whether every row of the tile sees all of the wavefront's tokens
             const int first = kr.pos0 + row0 / a.group, last = kr.pos0 + (row0 + 31) / a.group;
@@ -1310,8 +1332,8 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs& a, const Kv4AttnPlan& p, int D, hi
 
 // The sums' ranges.  Up to 16 rows of the tokens, to eight workgroups a CU: one token of 32 sequences over 16384, 8 key heads, 57 us
 // with eight ranges, 73 with four, 60 with 32; of one sequence 6.0 us with 128, 11.4 with 16.  Beyond, of the rows, to twelve
-// workgroups a CU and no fewer than 512 rows each: 2 x 2048 queries over 4099, 32 heads of 128 over 8, 125 us with
-// twelve ranges, 145 with four, 304 with one; 64 rows of 64 heads over 2048 12.6 us with one, 20.2 with two.
+// workgroups a CU and no fewer than 512 rows each: 2 x 2048 queries over 4099, 32 heads of 128 over 8, 124 us with
+// twelve ranges, 1.2 times that with four, 2.4 with one; 64 rows of 64 heads over 2048 12.6 us with one, 20.2 with two.
 Kv4WeightsPlan kv4_weights_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t room, int window, int cus) {
     const int64_t tokens = window > 0 ? std::min<int64_t>(room, (int64_t)window + n_q + KV4_TILE) : room;
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
