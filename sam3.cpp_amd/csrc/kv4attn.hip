@@ -479,7 +479,7 @@ __global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(con
 // the probabilities' registers as the operand of O^T += V^T P^T, V^T by transposing reads); a tile's scores are
 // computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU: between a tile's score products go the
 // first half's probabilities of the tile before, between that tile's first output products the second half's.
-// 2 x 4096 causal F16 queries over 5120 tokens, 32 heads of 128 over 8: 336 us (940 TFLOP/s; to 367 from one run to another), 20 of
+// 2 x 4096 causal F16 queries over 5120 tokens, 32 heads of 128 over 8: 336 to 390 us from one run to another (940 TFLOP/s), 20 of
 // them for the halves; matrix pipe busy 45 % of the time, VALU 41 %, LDS reads 85 % of their rate, at a clock of 1.7 GHz.
 // 5184 F32 queries over 15552 tokens, 8 heads of 64, two halves of either operand: 330 us for 330 GFLOP.  64 rows to a wavefront
 // would halve the LDS reads, but leave one wavefront a SIMD: 673 and 407 us.
