@@ -541,3 +541,34 @@ def test_blocks_past_4_gib(mi, ctx):
     ctx.synchronize()
     for h in range(heads):
         assert torch.equal(back.cpu()[0, h, :200].to(F64), old[h, kept.cpu()[0, h].long()])
+
+
+# ---------------------------------------------------------------- many heads to a key head, scales of any sign
+def check_weights(mi, ctx, c, d, q, n_q, causal, window, scale):
+    _, lse = attend(mi, ctx, c, d, q, n_q, causal, window, F32, scale)
+    add, tol = c.weights(q, n_q, lse, scale, causal, window, q.dtype == F32)
+    sums, qd, ld = torch.zeros(add.shape, device="cuda"), q.cuda().transpose(1, 2), lse.cuda()
+    ctx.kv_cache4_weights(d["cache"], d["seqs"], tensor(mi, qd), ld.data_ptr(), sums.data_ptr(), scale, n_q=ints(n_q).data_ptr(), causal=causal, window=window)
+    ctx.synchronize()
+    close(sums.cpu(), add, tol + U * add)
+
+
+@pytest.mark.parametrize("q_type", [F16, F32])
+@pytest.mark.parametrize("nq,heads,kv,causal,window", [(1, 71, 1, True, 0), (5, 80, 2, True, 0), (30, 33, 1, True, 40), (3, 130, 1, False, 0), (64, 48, 1, True, 9)])
+def test_many_heads_of_a_key_head(mi, ctx, nq, heads, kv, causal, window, q_type):
+    """More heads to a key head than a step of the kernels has rows."""
+    c = R4.Cache4(2, 12, kv, 32, 64, seed=heads).fill([300, 77])
+    d = c.on_gpu(mi)
+    q = torch.randn((2, nq, heads, 64), generator=torch.Generator().manual_seed(nq)).to(q_type)
+    check_attn(mi, ctx, c, d, q, [nq, max(nq - 1, 1)], causal, window, q_type)
+    check_weights(mi, ctx, c, d, q, [nq, max(nq - 1, 1)], causal, window, 0.125)
+
+
+@pytest.mark.parametrize("q_type", [F16, F32])
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 0.7])
+def test_weights_of_any_scale(mi, ctx, scale, q_type):
+    c = R4.Cache4(1, 20, 2, 16, 128, seed=4).fill([290])
+    d = c.on_gpu(mi)
+    for nq in (1, 90):
+        q = torch.randn((1, nq, 4, 128), generator=torch.Generator().manual_seed(nq)).to(q_type)
+        check_weights(mi, ctx, c, d, q, [nq], True, 0, scale)
