@@ -16,12 +16,13 @@ DEV = "cuda"
 class Big:
     """A cache of random nibbles and scales on the GPU, and a sequence's values in float64."""
 
-    def __init__(self, mi, n_kv, heads, bt, D, seed=0, miss=True):
+    def __init__(self, mi, n_kv, heads, bt, D, seed=0, miss=True, before=0):
         g = torch.Generator(DEV).manual_seed(seed)
         S, per = len(n_kv), max(n_kv) // bt + 1
         n = S * per + 2
         self.heads, self.bt, self.D = heads, bt, D
-        self.table = torch.randperm(n, generator=g, device=DEV)[:S * per].reshape(S, per).to(I32)
+        self.table = before + torch.randperm(n, generator=g, device=DEV)[:S * per].reshape(S, per).to(I32)
+        n += before  # (blocks that no sequence has)
         if miss and per > 3:
             self.table[0, 2] = -1
         self.n_kv = torch.tensor(n_kv, dtype=I32, device=DEV)
@@ -194,3 +195,12 @@ def test_weights_of_a_window_in_a_long_table(mi, ctx):
     size = ctx.kv_cache4_weights_workspace_size(c.cache, c.seqs, tensor(mi, q.transpose(1, 2)), 100)
     assert 0 < size <= 32 * 2 * 2 * (100 + 1100 + 320) * 4  # at most 32 ranges; 64 tokens where the first one begins and 256 to a workgroup
     check(mi, ctx, c, q, [1100, 1097], True, 100, F16, "kv_cache4_attn_128_halves")
+
+
+@pytest.mark.parametrize("nq,heads,want", [(1, 16, "kv_cache4_attn_16"), (300, 16, "kv_cache4_attn_128"), (1501, 64, "kv_cache4_attn_128_halves")])
+def test_kernels_past_4_gib(mi, ctx, nq, heads, want):
+    """Every kernel over blocks that begin more than 4 GiB into the keys and the values."""
+    c = Big(mi, [1800], 8, 128, 128, seed=nq, before=70000)
+    q = torch.randn((1, nq, heads, 128), generator=torch.Generator(DEV).manual_seed(nq), device=DEV).to(F16)
+    assert int(c.table[0, 0]) * 8 * 128 * 64 > 1 << 32
+    check(mi, ctx, c, q, [nq], True, 0, F16, want)
