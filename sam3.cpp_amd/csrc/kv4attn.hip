@@ -1263,7 +1263,7 @@ Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t m
         {{{2.45f, 4.2f}, {1.75f, 2.2f, 3.4f}}, {{3.4f, 6.0f}, {2.0f, 3.4f}}}};
     double best = 1e300;
     for (int kind = 0; kind < 3; ++kind) {
-        if ((kind > 0 && rows <= 16) || (kind == 2 && pre > (double)(1 << 30))) break;
+        if ((kind > 0 && rows <= 16) || (kind == 2 && (pre > (double)(1 << 30) || max_tokens <= 0))) break;  // (a table without blocks has no halves)
         const float *wide = us[kind][q16 ? 0 : 1][0], *narrow = us[kind][q16 ? 0 : 1][1];
         const int64_t row = kind ? 128 : 16, tiles = (rows + row - 1) / row;
         const int cap = kind == 0 ? (q16 || D == 64 ? 4 : 3) : kind == 2 && q16 && D == 64 ? 3 : 2;  // workgroups of a CU
