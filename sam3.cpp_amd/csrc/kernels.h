@@ -386,6 +386,8 @@ struct Kv4View {
     const int32_t* n_kv;
     int n_seq, max_blocks;
 };
+// tokens of a workgroup of the write's 256 threads, D / 4 lanes each in whole wavefronts
+constexpr int kv4_write_tokens(int D) { return 4 * (64 / (D / 4)); }
 hipError_t launch_kv4_write(const Kv4View& c, const KvRows& r, int D, hipStream_t st);
 hipError_t launch_kv4_read(const Kv4View& c, const KvRows& r, int D, hipStream_t st);
 struct Kv4EvictArgs {

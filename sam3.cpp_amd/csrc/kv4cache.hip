@@ -465,8 +465,8 @@ __global__ __launch_bounds__(EV_T) void kv4_move_kernel(const Kv4EvictArgs a, co
 
 template <int D>
 static void kv4_write_go(const Kv4View& c, const KvRows& r, hipStream_t st) {
-    constexpr int per = 4 * (64 / (D / 4));
-    const dim3 g((unsigned)((r.n_tok + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seq);
+    constexpr int per = kv4_write_tokens(D);
+    const dim3 g((unsigned)(((int64_t)r.n_tok + per - 1) / per), (unsigned)c.heads, (unsigned)c.n_seq);
     if (r.f16) kv4_write_kernel<D, true><<<g, 256, 0, st>>>(c, r);
     else kv4_write_kernel<D, false><<<g, 256, 0, st>>>(c, r);
 }

@@ -513,7 +513,9 @@ mi355_status mi355_kv_cache4_write(mi355_context* ctx, const mi355_kv_cache4* ca
     KvRows r;
     st = kv_rows(ctx, "kv_cache4_write", cache, seqs, k, v, n_new, &r);
     if (st != MI355_STATUS_SUCCESS) return st;
-    if (r.n_tok > 1 << 27) return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache4_write: sizes beyond the launch limits");
+    // a grid has fewer than 2^32 threads
+    if (r.n_tok > 1 << 27 || r.n_tok > (int64_t)kv4_write_tokens(cache->head_dim) * (UINT32_MAX / 256))
+        return fail(ctx, MI355_STATUS_UNSUPPORTED, "kv_cache4_write: sizes beyond the launch limits");
     if (!ctx) return fail(nullptr, MI355_STATUS_INVALID_ARG, "kv_cache4_write: null context");
     (void)hipSetDevice(ctx->device);
     Timed tm(ctx, "kv_cache4_write");
