@@ -104,6 +104,12 @@ __device__ __forceinline__ const char* row_at(const Kv4AttnArgs& a, int s, int i
     return a.q + (int64_t)iq * a.q_nb[0] + (int64_t)h * a.q_nb[1] + (int64_t)s * a.q_nb[2];
 }
 
+// What turns a row's products into exponents of 2.  The row's power of two comes first, for the scale to be a normal number
+// where the scores are of a size that counts.  Neither zero nor infinite: hidden scores are -inf, products may be zero.
+__device__ __forceinline__ float score_factor(float scale, float up) {
+    return fminf(fmaxf(fabsf(scale) * up * KV4_LOG2E, 1e-37f), 3e38f);
+}
+
 // A lane's words of the values of eight tokens, 4 g .. 4 g + 3 of both halves of 32, and their scales
 template <int D>
 struct Values {
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(con
     row.load(row_at(a, s, iq, hk * a.group + (r - iq * a.group)), on, g);
     const int pos = kr.pos0 + iq;
     const int see_hi = on ? (a.causal ? min(pos + 1, te) : te) : 0, see_lo = a.window > 0 ? pos - a.window + 1 : 0;
-    const float f = fmaxf(fabsf(a.scale) * KV4_LOG2E * row.up, 1e-37f);  // (0 times a hidden score)
+    const float f = score_factor(a.scale, row.up);
     if (a.scale < 0.0f)
 #pragma unroll
         for (int m = 0; m < KM; ++m) {
@@ -622,7 +628,7 @@ __global__ __launch_bounds__(256, 2) void kv4_tiles_kernel(const Kv4AttnArgs a, 
             qscale = 1.0f;
         }
     }
-    const float f = fmaxf(fabsf(a.scale) * KV4_LOG2E * qscale, 1e-37f);  // (0 times a hidden score)
+    const float f = score_factor(a.scale, qscale);
 
     int tile0 = 0;  // the step's tile
     // blocks of 16 tokens each, of the sixteen tiles that the step's tile is of, and of the sixteen after

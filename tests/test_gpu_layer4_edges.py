@@ -1,4 +1,5 @@
-"""The operators of a layer with a 4-bit cache on the GPU at the ends of what they take: nothing at all."""
+"""The operators of a layer with a 4-bit cache on the GPU at the ends of what they take: nothing at all, and scales at the ends
+of fp32."""
 import math
 
 import pytest
@@ -6,6 +7,7 @@ import torch
 
 import layer4_refs as R4
 from layer_refs import tensor
+from test_gpu_layer4_ops import check_attn
 
 pytestmark = pytest.mark.gpu
 F16, F32, I32 = torch.float16, torch.float32, torch.int32
@@ -81,3 +83,33 @@ def test_empty_calls(mi, ctx):
     ctx.synchronize()
     assert n_out.tolist() == [0, 0] and out[0, 0].tolist() == [0, 0, 0] + [7] * 13 and out[1, 0].tolist() == [0] * 4 + [7] * 12
     assert all(torch.equal(d[n].view(torch.uint8), before[n].view(torch.uint8)) for n in before)
+
+
+# ---------------------------------------------------------------- scales at the ends of fp32
+# (scale, size of the queries' elements or None: zeros, of the cache's): scores of a few units, or all zero
+ENDS = [(1.4e-45, 1.0, 1.0), (1e-44, 1.0, 1.0), (-1e-42, 1.0, 1.0), (1e-43, 8e37, 2000.0), (-1e-41, 8e37, 40.0), (3e38, None, 1.0), (-3e38, 1e-38, 0.06)]
+
+
+def at_the_end(scale, size, std, D, nq, dtype):
+    scale = float(torch.tensor(scale, dtype=F32))
+    c = R4.Cache4(1, 20, 1, 16, D, seed=5).fill([290], std=std)
+    assert all(torch.isfinite(c.values(0, n)[0]).all() for n in "kv")
+    q = torch.randn((1, nq, 2, D), generator=torch.Generator().manual_seed(nq))
+    q = torch.zeros_like(q) if size is None else (q * size).clamp(-3e38, 3e38)
+    if size is not None and size < 1:
+        q[..., 0] = 2.0 ** -125  # the rows' largest elements are normal numbers
+    return scale, c, q.to(dtype)
+
+
+@pytest.mark.parametrize("scale,size,std", ENDS)
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("nq", [1, 140])
+def test_attn_at_the_ends(mi, ctx, scale, size, std, D, nq):
+    """Scales whose product with log2(e) is subnormal or infinite: the scores are what counts."""
+    for dtype in (F32, F16):
+        if dtype == F16 and size not in (None, 1.0):
+            continue
+        s, c, q = at_the_end(scale, size, std, D, nq, dtype)
+        d = c.on_gpu(mi)
+        for dt in (F16, F32):
+            check_attn(mi, ctx, c, d, q, [nq], nq == 1, 0, dt, s)
