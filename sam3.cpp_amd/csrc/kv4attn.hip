@@ -1114,8 +1114,12 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
         }
         return z;
     };
-    // in base 2: scale log2(e) is off by its rounding, and lse takes the same error, so that it acts on their difference alone
-    const float f2 = a.scale * KV4_LOG2E, ratio = a.scale != 0.0f ? f2 / a.scale : KV4_LOG2E;
+    // In base 2: scale log2(e) is off by its rounding, and lse takes the same error, so that it acts on their difference alone.
+    // Both of the scale's mantissa, whatever its size; its exponent joins the row's power of two.
+    int scale_e;
+    const float scale_m = frexpf(a.scale, &scale_e), f1 = scale_m * KV4_LOG2E, ratio = scale_m != 0.0f ? f1 / scale_m : KV4_LOG2E;
+    auto factor = [&](float up) { return fmaxf(fminf(f1 * ldexpf(up, scale_e), 3e38f), -3e38f); };  // (times a product of zero)
+    const float f2 = factor(1.0f);
     auto store = [&](const Staged& z, int buf) {
         float up = 1.0f, down = 1.0f;
         if constexpr (QS) {
@@ -1146,7 +1150,7 @@ __global__ __launch_bounds__(256, 2) void kv4_weights_tiles_kernel(const Kv4Attn
         if (part == 0) {
             const bool on = z.pos != INT32_MIN;
             sL[buf][sr] = z.lse * ratio;
-            sF[buf][sr] = f2 * up;
+            sF[buf][sr] = factor(up);
             sHi[buf][sr] = on ? (a.causal ? min(z.pos + 1, kr.hi) : kr.hi) : 0;
             sLo[buf][sr] = on && a.window > 0 ? z.pos - a.window + 1 : 0;
         }

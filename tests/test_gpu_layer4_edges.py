@@ -6,8 +6,8 @@ import pytest
 import torch
 
 import layer4_refs as R4
-from layer_refs import tensor
-from test_gpu_layer4_ops import check_attn
+from layer_refs import U, tensor
+from test_gpu_layer4_ops import check_attn, close
 
 pytestmark = pytest.mark.gpu
 F16, F32, I32 = torch.float16, torch.float32, torch.int32
@@ -113,3 +113,21 @@ def test_attn_at_the_ends(mi, ctx, scale, size, std, D, nq):
         d = c.on_gpu(mi)
         for dt in (F16, F32):
             check_attn(mi, ctx, c, d, q, [nq], nq == 1, 0, dt, s)
+
+
+@pytest.mark.parametrize("scale,size,std", ENDS)
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("nq", [1, 140])
+def test_weights_at_the_ends(mi, ctx, scale, size, std, D, nq):
+    """The same of the weights' sums, from the definition's logarithms."""
+    for dtype in (F32, F16):
+        if dtype == F16 and size not in (None, 1.0):
+            continue
+        s, c, q = at_the_end(scale, size, std, D, nq, dtype)
+        d = c.on_gpu(mi)
+        lse = c.attn(q, [nq], s, nq == 1, 0, dtype == F32, True)[2].float()
+        add, tol = c.weights(q, [nq], lse, s, nq == 1, 0, dtype == F32)
+        sums, qd, ld = torch.zeros(add.shape, device="cuda"), q.cuda().transpose(1, 2), lse.cuda()
+        ctx.kv_cache4_weights(d["cache"], d["seqs"], tensor(mi, qd), ld.data_ptr(), sums.data_ptr(), s, causal=nq == 1)
+        ctx.synchronize()
+        close(sums.cpu(), add, tol + U * add)
