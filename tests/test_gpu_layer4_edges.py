@@ -1,5 +1,5 @@
-"""The operators of a layer with a 4-bit cache on the GPU at the ends of what they take: nothing at all, and scales at the ends
-of fp32."""
+"""The operators of a layer with a 4-bit cache on the GPU at the ends of what they take: nothing at all, scales at the ends of
+fp32, and sums over many rows."""
 import math
 
 import pytest
@@ -131,3 +131,30 @@ def test_weights_at_the_ends(mi, ctx, scale, size, std, D, nq):
         ctx.kv_cache4_weights(d["cache"], d["seqs"], tensor(mi, qd), ld.data_ptr(), sums.data_ptr(), s, causal=nq == 1)
         ctx.synchronize()
         close(sums.cpu(), add, tol + U * add)
+
+
+# ---------------------------------------------------------------- sums over many rows
+@pytest.mark.parametrize("seqs,blocks", [(16, 96), (4, 1)])
+def test_weights_of_many_rows(mi, ctx, seqs, blocks):
+    """32768 equal weights a token, in one range of the rows and in 32: 16 rows of a tile in a tree (4 additions deep), 32
+    tiles one after another, then those (32 of one range; 2 of each of 32, which are 32 more), and two lanes' sums: no
+    sum is more than 4 + 32 + 32 + 2 + 1 roundings deep, where one tile after another would be 1024.
+    A weight is e^-lse, whose exponent is off by 4 U (log2(e), its product with the scale, their quotient, lse's product) and
+    the exponential by 2 U: 7 U of it with lse up to 1.1.  (One tile after another is off by 7 to 214 U in these
+    values, as fp32 on the CPU gives.)"""
+    nq, heads, kv = 4096, 32, 4
+    c = R4.Cache4(seqs, 1, kv, 128, 64).fill([64] * seqs)
+    d = c.on_gpu(mi)
+    table = torch.full((seqs, blocks), -1, dtype=I32, device="cuda")
+    table[:, :1] = d["table"]
+    q = torch.zeros((seqs, heads, nq, 64), dtype=F16, device="cuda")
+    one = 0.1 + torch.arange(seqs * kv, device="cuda").reshape(seqs, 1, kv, 1) / (seqs * kv)
+    lse = one.expand(seqs, nq, kv, heads // kv).reshape(seqs, nq, heads).contiguous()
+    sums = torch.zeros((seqs, kv, blocks * 128), device="cuda")
+    s = mi.kv_seqs(table, d["n_kv"])
+    ctx.kv_cache4_weights(d["cache"], s, tensor(mi, q), lse.data_ptr(), sums.data_ptr(), 0.125, causal=False)
+    ctx.synchronize()
+    want = (nq * heads // kv * torch.exp(-one.reshape(seqs, kv, 1).double())).cpu()
+    got = sums.cpu().double()
+    assert (got[..., 64:] == 0).all()
+    assert ((got[..., :64] - want).abs() <= (71 + 7) * U * want).all(), float(((got[..., :64] - want).abs() / want).max() / U)
