@@ -433,6 +433,7 @@ mi355_status mi355_kv_cache4_read(mi355_context* ctx, const mi355_kv_cache4* cac
  * [n_seq][n_q][n_head], or NULL) takes log sum exp(scale q . k) over the tokens that the
  * query sees, -inf where there is none; rows from n_q[s] on are left as they are.
  * Scores are fp32, and hold a fraction up to magnitudes of 2^23: the softmax of larger ones means nothing.
+ * Queries and probabilities enter the products as there; lse's fp32 sum is of the unrounded probabilities.
  * mi355_kv_cache4_attn_workspace_size as mi355_kv_cache_attn_workspace_size. */
 int mi355_supports_kv_cache4_attn(const mi355_kv_cache4* cache, const mi355_kv_seqs* seqs, const mi355_tensor* q,
                                   const mi355_tensor* dst);
@@ -445,7 +446,8 @@ mi355_status mi355_kv_cache4_attn(mi355_context* ctx, const mi355_kv_cache4* cac
  * [max_blocks * block_tokens]) the softmax weight of token t, exp(scale q . k - lse),
  * summed over the queries that see it and the heads of key head h's group.  lse as
  * mi355_kv_cache4_attn gave it for the same queries, scale, causal and window.  Places of
- * tokens that no query sees are left as they are.  The same call gives the same bits.
+ * tokens that no query sees are left as they are.  Queries enter as the attention's; weights and sums are fp32, those
+ * of every 1024 rows (queries and heads) by themselves first.  The same call gives the same bits.
  * mi355_kv_cache4_weights_workspace_size as the attention's. */
 size_t mi355_kv_cache4_weights_workspace_size(const mi355_context* ctx, const mi355_kv_cache4* cache,
                                               const mi355_kv_seqs* seqs, const mi355_tensor* q, int32_t window);

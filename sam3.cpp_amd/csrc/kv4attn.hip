@@ -486,9 +486,10 @@ __global__ __launch_bounds__(256, QS && D > 64 ? 2 : 4) void kv4_rows_kernel(con
 // computed one tile ahead of its softmax, so that the matrix pipe works beside the VALU: between a tile's score products go the
 // first half's probabilities of the tile before, between that tile's first output products the second half's.
 // 2 x 4096 causal F16 queries over 5120 tokens, 32 heads of 128 over 8: 336 to 390 us from one run to another (940 TFLOP/s), 20 of
-// them for the halves; matrix pipe busy 45 % of the time, VALU 41 %, LDS reads 85 % of their rate, at a clock of 1.7 GHz.
-// 5184 F32 queries over 15552 tokens, 8 heads of 64, two halves of either operand: 330 us for 330 GFLOP.  64 rows to a wavefront
-// would halve the LDS reads, but leave one wavefront a SIMD: 673 and 407 us.
+// them for the halves, at a clock of 1.7 to 1.95 GHz.  No unit is full: matrix pipe busy 45 % of the time, VALU 42 %, LDS 23 %, 1.7
+// wavefronts on a SIMD, which leave the first two one after another more often than side by side.
+// 5184 F32 queries over 15552 tokens, 8 heads of 64, two halves of either operand: 330 us for 330 GFLOP (matrix pipe 54 %, VALU
+// 58 %, LDS 13 %).  64 rows to a wavefront would halve the LDS reads, but leave one wavefront a SIMD: 673 and 407 us.
 //
 // V row slot of 16-byte chunk c in row r: c ^ this.  The transposing reads take four chunks from each of four rows, which lie
 // in distinct quarters of the banks (as fattn.hip's vswz); with heads of 128 the chunks are turned within their
@@ -1016,8 +1017,8 @@ __global__ __launch_bounds__(256, 4) void kv4_weights_rows_kernel(const Kv4AttnA
 // through LDS 32 at a time (an F32 row as two halves, times a power of two).  A lane sums a tile's sixteen rows of a token in a
 // tree, 32 tiles one after another and then those, for 32 bits to hold them.  A range's sums go to part, or are added at once
 // where there is one range.  Bound by the VALU's work of a weight (difference, product, exponential, sum): 2 x 2048 causal F16
-// queries over 4099, 32 heads of 128 over 8, 77 GFLOP in 124 us (139 with equal ranges, chunk by chunk, the product with log2(e) of
-// each difference, and each row's place by a division); VALU busy 53 % of the time, matrix pipe 28 %, three wavefronts a SIMD.  The next
+// queries over 4099, 32 heads of 128 over 8, 79 GFLOP in 124 us (139 with equal ranges, chunk by chunk, the product with log2(e) of
+// each difference, and each row's place by a division); VALU busy 53 % of the time, matrix pipe 28 %, LDS 20 %, up to three wavefronts a SIMD.  The next
 // tile's scores between this one's weights leave two of them and took 1.13 times as long, 32 tokens to a wavefront and four of
 // them 1.12 times, rows loaded two tiles ahead the same.
 template <int D, bool QS>
@@ -1254,10 +1255,10 @@ __global__ __launch_bounds__(256) void kv4_weights_join_kernel(const Kv4AttnArgs
 // 128 tokens takes a workgroup so long, in microseconds, with one, two .. workgroups on its CU (heads of 128 and 64, of 96
 // between them; F32 queries); where one row tile reads a sequence's tokens alone, its share of the memory at least.  Then the
 // partial sums, which a last workgroup joins past the caches or a second launch does, and the halves' launch.
-// One token of 32 sequences over 16384, 32 heads of 128 over 8: four ranges 104 us, two 117, eight 106; of one sequence: 24
-// ranges 16.1 us, 16 16.5, 8 22.9.  80 rows of 32 sequences and 4 heads of 3000 tokens: 16 rows 47, 128 41, with halves 90;
-// 126 rows of 16 heads of 2424: 14.5, 18.2, 31; 1024 rows of 64 heads of 2048: 103, 77, 86; 5184 rows of 8 heads of 64 over 15552:
-// 443, 256, 215.
+// One token of 32 sequences over 16384, 32 heads of 128 over 8: four ranges 104 us, two 117, eight 106; of one sequence
+// (26 by these steps): 24 ranges 16.1 us, 16 16.5, 8 22.9.  80 rows of 32 sequences and 4 heads of 3000 tokens: 16 rows 47, 128 41, with halves 90;
+// 126 rows of 16 heads of 2424: 14.5, 18.2, 31; 1024 rows of 64 heads of 2048: 103, 77, 86; 5184 F16 rows of 8 heads of 64 over
+// 15552: 443, 256, 215 (245 to 285 with inputs rotated).
 Kv4AttnPlan kv4_attn_plan(int n_q, int heads, int heads_kv, int n_seq, int64_t max_tokens, int window, int D, bool q16, int cus) {
     if (window > 0) max_tokens = std::min<int64_t>(max_tokens, (int64_t)window + n_q + KV_STEP);  // (kv_range)
     const int64_t rows = (int64_t)n_q * (heads / heads_kv), items = std::max<int64_t>((int64_t)heads_kv * n_seq, 1);
